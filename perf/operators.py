@@ -168,7 +168,7 @@ def _cross_entropy(s):
     at = label.clamp(min=0)
     loss = torch.where(counts, log_sum - logits.gather(1, at), 0.0)
     if not s["case"]["train"]:
-        return loss, log_sum
+        return loss
     factor = torch.where(counts, s["dloss"], 0.0)
     grad = logits.sub_(log_sum).exp_().mul_(factor)
     grad.scatter_add_(1, at, -factor)
@@ -195,7 +195,7 @@ def _distillation(s):
     log_q = x.gather(1, at) - log_sum
     loss = t * t * torch.where(p > 0, p * (log_p - log_q), 0.0).sum(1, keepdim=True)
     if not s["case"]["train"]:
-        return loss, log_sum
+        return loss
     factor = t * s["dloss"]
     grad = x.sub_(log_sum).exp_().mul_(torch.where(some, factor, 0.0))
     grad.scatter_add_(1, at, -p * factor)
@@ -213,15 +213,15 @@ def _own(s):
         y, mean, variance = F.layer_normalization(s["x"], s["beta"], s["gamma"], eps=EPS, output_stat=True)
         return (y,) + tuple(F.layer_normalization_backward(s["x"], s["dy"], s["gamma"], mean, variance, eps=EPS))
     if case["op"] == "cross_entropy":
-        loss, log_sum = F.affine_softmax_cross_entropy(s["x"], s["weight"], s["label"], s["bias"], output_stat=True)
         if not case["train"]:
-            return loss, log_sum
-        return (loss,) + tuple(F.affine_softmax_cross_entropy_backward(s["x"], s["weight"], s["label"], log_sum, s["dloss"],
+            return F.affine_softmax_cross_entropy(s["x"], s["weight"], s["label"], s["bias"])
+        loss, stat = F.affine_softmax_cross_entropy(s["x"], s["weight"], s["label"], s["bias"], output_stat=True)
+        return (loss,) + tuple(F.affine_softmax_cross_entropy_backward(s["x"], s["weight"], s["label"], stat, s["dloss"],
                                                                        s["bias"]))
-    loss, log_sum = F.top_k_distillation(s["x"], s["index"], s["teacher"], case["temperature"], output_stat=True)
     if not case["train"]:
-        return loss, log_sum
-    return loss, F.top_k_distillation_backward(s["x"], s["index"], s["teacher"], log_sum, s["dloss"], case["temperature"])
+        return F.top_k_distillation(s["x"], s["index"], s["teacher"], case["temperature"])
+    loss, stat = F.top_k_distillation(s["x"], s["index"], s["teacher"], case["temperature"], output_stat=True)
+    return loss, F.top_k_distillation_backward(s["x"], s["index"], s["teacher"], stat, s["dloss"], case["temperature"])
 
 
 def run(state):
@@ -242,7 +242,7 @@ def work(case):
         size, classes = case["size"], case["classes"]
         operands = (rows * size + size * classes + (classes if case["bias"] else 0)) * e
         # the products: the logits, and for training dx and dW
-        return dict(bytes=(2 if case["train"] else 1) * operands + rows * (20 if case["train"] else 16),
+        return dict(bytes=(2 if case["train"] else 1) * operands + rows * (20 if case["train"] else 12),
                     flops=(6 if case["train"] else 2) * rows * size * classes)
     n, best = rows * case["classes"], case["best"]
     return dict(bytes=(2 if case["train"] else 1) * n * e + rows * (best * (8 + e) + 8), flops=(8 if case["train"] else 4) * n)
@@ -269,7 +269,7 @@ def exact(case, seed):
     if case["op"] == "cross_entropy":
         w, label, rows = double["weight"], s["label"], case["rows"]
         bias = double.get("bias")
-        losses, sums, dx = [], [], []
+        losses, dx = [], []
         dw = torch.zeros_like(w) if case["train"] else None
         db = torch.zeros(case["classes"], dtype=torch.float64, device="cuda")
         for a in range(0, rows, 2048):  # (some rows at a time: the logits in 64 bits are large)
@@ -281,7 +281,6 @@ def exact(case, seed):
             loss = torch.zeros_like(log_sum)
             loss[valid] = log_sum[valid] - logits[row, at[valid]]
             losses.append(loss)
-            sums.append(log_sum)
             if case["train"]:
                 probability = torch.softmax(logits, 1)
                 probability[row, at[valid]] -= 1.0
@@ -291,11 +290,11 @@ def exact(case, seed):
                 db += probability.sum(0)
         loss = torch.cat(losses)[:, None]
         if not case["train"]:
-            return loss, torch.cat(sums)[:, None]
+            return loss
         return loss, torch.cat(dx), dw, (db if bias is not None else None)
     t = case["temperature"]
     index, rows = s["index"], case["rows"]
-    losses, sums, grads = [], [], []
+    losses, grads = [], []
     for a in range(0, rows, 1024):
         part, at, teacher = x[a:a + 1024] / t, index[a:a + 1024], double["teacher"][a:a + 1024] / t
         log_sum = torch.logsumexp(part, 1, keepdim=True)
@@ -304,10 +303,9 @@ def exact(case, seed):
         entropy = torch.special.entr(p).sum(1, keepdim=True)
         cross = (p * (part.gather(1, at.clamp(min=0)) - log_sum)).sum(1, keepdim=True)
         losses.append(-t * t * (entropy + cross))
-        sums.append(log_sum)
         if case["train"]:
             q = torch.softmax(part, 1) * p.sum(1, keepdim=True)
             grads.append((q.scatter_add(1, at.clamp(min=0), -p) * (t * double["dloss"][a:a + 1024])))
     if not case["train"]:
-        return torch.cat(losses), torch.cat(sums)
+        return torch.cat(losses)
     return torch.cat(losses), torch.cat(grads)
