@@ -644,6 +644,45 @@ int nb200_convolution_f32(const float *x, const float *w, const float *bias, flo
                           int height, int width, int outmaps, int kernel_h, int kernel_w, int pad_h, int pad_w,
                           int stride_h, int stride_w, int dilation_h, int dilation_w, int group, void *stream);
 
+/* ---- the end of a network that is trained: normalization over features, its losses ----
+ * Operands in one of three types: float, bfloat16 or half (`type`); arithmetic, sums and
+ * statistics in fp32, one rounding where a result is stored. */
+#define NB200_F32 0
+#define NB200_BF16 1
+#define NB200_F16 2
+
+/* LayerNormalization over the trailing axes: x, y [rows, size], beta / gamma [size] (NULL: none)
+ * of x's type or fp32 (param_type); y = (x - mean) / sqrt(variance + eps) * gamma + beta with
+ * mean and variance (biased) of each row, also stored where `mean` / `variance` are not NULL.
+ * y == x is allowed. */
+int nb200_layer_normalization(const void *x, const void *beta, const void *gamma, void *y, float *mean,
+                              float *variance, int64_t rows, int64_t size, float eps, int type, int param_type,
+                              void *stream);
+/* Its gradients from the statistics that the forward pass stored. dx, dbeta, dgamma may each be NULL (not
+ * propagated); the accum flags add to what the buffers hold. The sums over the rows are block partials added
+ * in a fixed order (deterministic). dx == dy and dx == x are allowed. */
+int nb200_layer_normalization_backward(const void *x, const void *dy, const void *gamma, const float *mean,
+                                       const float *variance, void *dx, void *dbeta, void *dgamma, int64_t rows,
+                                       int64_t size, float eps, int type, int param_type, int accum_dx,
+                                       int accum_dbeta, int accum_dgamma, void *stream);
+
+/* Distillation from the teacher's best classes: x [rows, classes] the student's logits, index [rows, best] the
+ * classes (int32 or int64: index_bytes) and teacher [rows, best] their logits in x's type; an entry whose class is
+ * negative is none.
+ *   p = softmax(teacher / temperature) over a row's entries, q = softmax(x / temperature)
+ *   loss = temperature^2 * sum p (log p - log q)   (fp32, [rows])
+ * stat [rows, 2], fp32: the row's maximum, and log sum exp((x - maximum) / temperature).
+ * A class named twice counts twice. A row without entries has the loss 0. A class >= classes makes its row's loss
+ * NaN. best is 1 to 1024. */
+int nb200_top_k_distillation(const void *x, const void *index, const void *teacher, float *loss, float *stat,
+                             int64_t rows, int64_t classes, int best, float temperature, int type, int index_bytes,
+                             void *stream);
+/* dx (+)= temperature * (q - p) * dloss of each row, zero for a row without entries; stat is the forward
+ * pass's. dx == x is allowed. */
+int nb200_top_k_distillation_backward(const void *x, const void *index, const void *teacher, const float *log_sum,
+                                      const float *dloss, void *dx, int64_t rows, int64_t classes, int best,
+                                      float temperature, int type, int index_bytes, int accum, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,420 @@
+// Distillation from a teacher of which each row's K best classes and their logits are known.
+//
+//   p = softmax(teacher / tau) over the row's entries (class >= 0), q = softmax(x / tau) over all classes
+//   loss = tau^2 sum_k p_k (log p_k - log q_k)
+//   dx_v = tau (q_v [the row has an entry] - sum of p_k over the entries k of class v) dloss
+//
+// HBM bound: the forward pass reads x once, with the running maximum and sum of the softmax; with those two kept, the
+// gradient is one pass that reads x and writes dx, and then corrects the few classes that the teacher names. Differences to
+// the maximum are taken before anything is scaled: a row masked with the type's lowest value overflows nowhere.
+#include <algorithm>
+
+#include "pdl.cuh"
+#include "typed.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxEntries = 1024;
+
+__device__ __forceinline__ float ex2(float v) { // 2^v; results below 2^-126 are zero
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Running maximum and sum of 2^((v - maximum) * scale). A maximum of -infinity has the sum 0.
+struct MaxSum {
+  float m, s;
+};
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float scale) {
+  const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
+  return {m, a.s * ex2((a.m - base) * scale) + b.s * ex2((b.m - base) * scale)};
+}
+__device__ __forceinline__ MaxSum warp_join(MaxSum v, float scale) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1)
+    v = join(v, MaxSum{__shfl_xor_sync(0xffffffffu, v.m, d), __shfl_xor_sync(0xffffffffu, v.s, d)}, scale);
+  return v;
+}
+
+// The row's teacher, by one warp: each lane's entries are k = lane, lane + 32, ... An entry is one with a class that is not
+// negative.
+template <typename T, typename I>
+__device__ __forceinline__ MaxSum teacher_sums(const I *index, const T *teacher, int best, float scale, int lane) {
+  MaxSum t{-INFINITY, 0.0f};
+  float top = -INFINITY;
+  bool nan = false;
+  for (int k = lane; k < best; k += 32)
+    if (index[k] >= 0) {
+      const float v = to_f32(teacher[k]);
+      top = fmaxf(top, v);
+      nan |= v != v;
+    }
+  top = __any_sync(0xffffffffu, nan) ? NAN : warp_max(top);
+  t.m = top;
+  const float base = top == -INFINITY ? 0.0f : top;
+  for (int k = lane; k < best; k += 32)
+    if (index[k] >= 0)
+      t.s += ex2((to_f32(teacher[k]) - base) * scale);
+  t.s = warp_sum(t.s);
+  return t;
+}
+
+// [start, start + n) of x cut into values before the first 16-byte boundary, whole 16-byte packs, and the rest.
+template <typename T> struct Run {
+  const T *head, *body, *tail;
+  int heads, tails;
+  int64_t packs;
+  __device__ __forceinline__ Run(const T *start, int64_t n) {
+    constexpr int V = kPackOf<T>;
+    int h = (int)((16 - (reinterpret_cast<uintptr_t>(start) & 15)) & 15) / (int)sizeof(T);
+    heads = h < n ? h : (int)n;
+    head = start;
+    body = start + heads;
+    packs = (n - heads) / V;
+    tail = body + packs * V;
+    tails = (int)(n - heads - packs * V);
+  }
+};
+
+// One row a cluster of blocks (one block where the rows are many). stat: the row's maximum, and log sum exp((x - maximum) / tau).
+template <typename T, typename I>
+__global__ void __launch_bounds__(512) distill_forward_kernel(const T *__restrict__ x, const I *__restrict__ index,
+                                                              const T *__restrict__ teacher, float *__restrict__ loss,
+                                                              float2 *__restrict__ stat, int64_t classes, int best,
+                                                              float tau, int parts) {
+  constexpr int V = kPackOf<T>;
+  __shared__ float shared_m[16], shared_s[16];
+  __shared__ float whole[2];
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = blockIdx.x / parts;
+  const int part = blockIdx.x - (int)row * parts;
+  const int64_t each = ((classes + parts - 1) / parts + V - 1) / V * V;
+  const int64_t c0 = part * each < classes ? part * each : classes, c1 = c0 + each < classes ? c0 + each : classes;
+  const T *xr = x + row * classes;
+  const float scale = kLog2e / tau;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const Run<T> run(xr + c0, c1 - c0);
+  float m = -INFINITY, s = 0.0f;
+  auto add = [&](auto &v, int n) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < n; ++j)
+      top = fmaxf(top, v[j]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    s *= ex2((m - base) * scale);
+#pragma unroll
+    for (int j = 0; j < n; ++j)
+      s += ex2((v[j] - base) * scale);
+    m = top;
+  };
+  const int64_t step = blockDim.x;
+  int64_t i = threadIdx.x;
+  for (; i + 3 * step < run.packs; i += 4 * step) {
+    Pack<T, V> p[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      p[u] = load_pack_stream<T, V>(run.body + (i + u * step) * V);
+    float v[4 * V];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        v[u * V + j] = p[u].f(j);
+    add(v, 4 * V);
+  }
+  for (; i < run.packs; i += step) {
+    const Pack<T, V> p = load_pack_stream<T, V>(run.body + i * V);
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      v[j] = p.f(j);
+    add(v, V);
+  }
+  if ((int)threadIdx.x < run.heads + run.tails) {
+    float v[1] = {to_f32((int)threadIdx.x < run.heads ? run.head[threadIdx.x] : run.tail[threadIdx.x - run.heads])};
+    add(v, 1);
+  }
+  MaxSum t = warp_join({m, s}, scale);
+  if (lane == 0)
+    shared_m[warp] = t.m, shared_s[warp] = t.s;
+  __syncthreads();
+  if (warp == 0) {
+    t = warp_join(lane < warps ? MaxSum{shared_m[lane], shared_s[lane]} : MaxSum{-INFINITY, 0.0f}, scale);
+    if (lane == 0)
+      whole[0] = t.m, whole[1] = t.s;
+  }
+  if (parts > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (part == 0 && warp == 0) {
+      MaxSum o{-INFINITY, 0.0f};
+      if (lane < parts) {
+        uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(whole)), theirs;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(lane));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(theirs) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.s) : "r"(theirs + 4u) : "memory");
+      }
+      t = warp_join(o, scale);
+    }
+  }
+  if (part == 0 && warp == 0) {
+    const float log_sum = log2f(t.s) * kLn2;
+    const I *ir = index + row * best;
+    const T *tr = teacher + row * best;
+    const MaxSum p = teacher_sums(ir, tr, best, scale, lane);
+    // In 64 bits, and divided by the shares' own sum: a class that the student masks with the type's lowest value and the
+    // teacher names gives a loss next to the largest float.
+    double sum = 0.0, mass = 0.0;
+    if (p.m != -INFINITY) {
+      const double log_mass = log((double)p.s);
+      for (int k = lane; k < best; k += 32) {
+        const int64_t c = (int64_t)ir[k];
+        if (c < 0)
+          continue;
+        const float d = to_f32(tr[k]) - p.m, share = ex2(d * scale);
+        mass += share;
+        if (c >= classes)
+          sum = NAN;
+        else if (!(share == 0.0f))
+          sum += share * (((double)d / tau - log_mass) - (((double)to_f32(xr[c]) - t.m) / tau - log_sum));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    }
+    if (p.m != -INFINITY)
+      sum /= mass;
+    if (lane == 0) {
+      loss[row] = (float)(sum * tau * tau);
+      stat[row] = make_float2(t.m, log_sum);
+    }
+  }
+  if (parts > 1) // no block leaves while another may still read its sums
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+constexpr int kGradThreads = 256, kGradPacks = 4;
+
+// dx (+)= gradient, a piece of a row a block: kGradThreads * kGradPacks packs of 16 bytes and the values around them. The
+// loads are on their way while warp 0 takes the teacher's sums and lists the entries whose class lies in the piece; those
+// classes are stored a second time, with their correction, by the first of the entries that name them.
+template <typename T, typename I>
+__global__ void __launch_bounds__(kGradThreads) distill_backward_kernel(
+    const T *x, const I *__restrict__ index, const T *__restrict__ teacher, const float2 *__restrict__ stat,
+    const float *__restrict__ dloss, T *dx, int64_t classes, int best, float tau, int pieces, bool accum, bool keep) {
+  constexpr int V = kPackOf<T>;
+  constexpr int64_t kPiece = (int64_t)kGradThreads * kGradPacks * V;
+  __shared__ int at[kMaxEntries];
+  __shared__ float share[kMaxEntries];
+  __shared__ int entries;
+  __shared__ float weight; // 1 where the row has an entry, 0 where it has none, NaN where an entry's class does not exist
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = blockIdx.x / pieces;
+  const int piece = blockIdx.x - (int)row * pieces;
+  const T *xr = x + row * classes;
+  T *out = dx + row * classes;
+  // pieces begin at 16-byte boundaries of x but for the row's first
+  const int64_t lead = (int64_t)(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / sizeof(T));
+  int64_t c0 = piece == 0 ? 0 : lead + piece * kPiece, c1 = lead + (piece + 1) * kPiece;
+  c1 = c1 < classes && piece + 1 < pieces ? c1 : classes;
+  c0 = c0 < c1 ? c0 : c1;
+  const Run<T> run(xr + c0, c1 - c0);
+  Pack<T, V> p[kGradPacks];
+#pragma unroll
+  for (int u = 0; u < kGradPacks; ++u)
+    if (threadIdx.x + u * kGradThreads < run.packs)
+      p[u] = load_pack_stream<T, V>(run.body + (threadIdx.x + u * kGradThreads) * V);
+  const float scale = kLog2e / tau, d = dloss[row] * tau, top = stat[row].x, log2_sum = stat[row].y * kLog2e;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const I *ir = index + row * best;
+    const T *tr = teacher + row * best;
+    const MaxSum t = teacher_sums(ir, tr, best, scale, lane);
+    int n = 0;
+    bool bad = false;
+    if (t.m != -INFINITY) {
+      const float log2_p = log2f(t.s);
+      for (int k0 = 0; k0 < best; k0 += 32) {
+        const int k = k0 + lane;
+        const int64_t c = k < best ? (int64_t)ir[k] : -1;
+        bad |= c >= classes;
+        const bool here = c >= c0 && c < c1;
+        const unsigned all = __ballot_sync(0xffffffffu, here);
+        if (here) {
+          const int to = n + __popc(all & ((1u << lane) - 1u));
+          at[to] = (int)(c - c0);
+          share[to] = ex2(fmaf(to_f32(tr[k]) - t.m, scale, -log2_p));
+        }
+        n += __popc(all);
+      }
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+      entries = n;
+      weight = bad ? NAN : (t.m == -INFINITY ? 0.0f : 1.0f);
+    }
+  }
+  __syncthreads();
+  const float factor = d * weight;
+  auto q = [&](float v) { return ex2(fmaf(v - top, scale, -log2_sum)); };
+  auto value = [&](float v) { return weight == 0.0f ? 0.0f : q(v) * factor; };
+  // the corrected classes, read before anything is written: dx may be x
+  float fixed[kMaxEntries / kGradThreads];
+  bool first[kMaxEntries / kGradThreads];
+#pragma unroll
+  for (int u = 0; u < kMaxEntries / kGradThreads; ++u) {
+    const int i = threadIdx.x + u * kGradThreads;
+    first[u] = i < entries;
+    if (!first[u])
+      continue;
+    float sum = 0.0f;
+    for (int j = 0; j < entries; ++j)
+      if (at[j] == at[i]) {
+        first[u] &= j >= i;
+        sum += share[j];
+      }
+    if (first[u]) {
+      fixed[u] = (q(to_f32(xr[c0 + at[i]])) - sum) * factor;
+      if (accum)
+        fixed[u] += to_f32(out[c0 + at[i]]);
+    }
+  }
+  if (entries > 0)
+    __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kGradPacks; ++u) {
+    const int64_t i = threadIdx.x + u * kGradThreads;
+    if (i >= run.packs)
+      continue;
+    T *to = out + (run.body - xr) + i * V;
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      o[j] = value(p[u].f(j));
+    if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      if (accum) {
+        const Pack<T, V> old = load_pack<T, V>(to);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          o[j] += old.f(j);
+      }
+      store_pack<T, V>(to, o, keep);
+    } else { // (dx lies differently from x)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        to[j] = from_f32<T>(accum ? o[j] + to_f32(to[j]) : o[j]);
+    }
+  }
+  if ((int)threadIdx.x < run.heads + run.tails) {
+    const T *from = (int)threadIdx.x < run.heads ? run.head + threadIdx.x : run.tail + (threadIdx.x - run.heads);
+    T *to = out + (from - xr);
+    const float o = value(to_f32(*from));
+    *to = from_f32<T>(accum ? o + to_f32(*to) : o);
+  }
+  if (entries == 0)
+    return;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kMaxEntries / kGradThreads; ++u)
+    if (first[u])
+      out[c0 + at[threadIdx.x + u * kGradThreads]] = from_f32<T>(fixed[u]);
+}
+
+int check(int64_t rows, int64_t classes, int best, float temperature, int index_bytes) {
+  NB_CHECK(rows >= 0 && rows < (1ll << 24), NB200_EVALUE, "%lld rows", (long long)rows);
+  NB_CHECK(classes > 0 && classes < (1ll << 24), NB200_EVALUE, "%lld classes outside [1, 2^24)", (long long)classes);
+  NB_CHECK(best >= 1 && best <= kMaxEntries, NB200_EVALUE, "%d entries a row outside [1, %d]", best, kMaxEntries);
+  NB_CHECK(temperature > 0.0f && temperature < INFINITY, NB200_EVALUE, "temperature = %g is not positive", temperature);
+  NB_CHECK(index_bytes == 4 || index_bytes == 8, NB200_EVALUE, "the classes are 4 or 8 byte integers, not %d", index_bytes);
+  return NB200_OK;
+}
+
+template <typename T, typename I>
+int forward(const T *x, const I *index, const T *teacher, float *loss, float *stat, int64_t rows, int64_t classes,
+            int best, float tau, cudaStream_t st) {
+  // blocks of up to 512 threads with four packs each; few long rows go to clusters
+  const int64_t packs = (classes + kPackOf<T> - 1) / kPackOf<T>;
+  int parts = 1;
+  while (parts < 8 && rows * parts < sm_count() && packs >= 1024 * parts)
+    parts *= 2;
+  int threads = 128;
+  while (threads < 512 && threads * 4 * parts < packs)
+    threads *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * parts));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  NB_CUDA(cudaLaunchKernelEx(&cfg, distill_forward_kernel<T, I>, x, index, teacher, loss, reinterpret_cast<float2 *>(stat), classes, best, tau, parts));
+  return NB200_OK;
+}
+
+template <typename T, typename I>
+int backward(const T *x, const I *index, const T *teacher, const float *stat, const float *dloss, T *dx, int64_t rows,
+             int64_t classes, int best, float tau, bool accum, cudaStream_t st) {
+  constexpr int64_t kPiece = (int64_t)kGradThreads * kGradPacks * kPackOf<T>;
+  const int64_t pieces = (classes + kPiece - 1) / kPiece;
+  NB_CHECK(rows * pieces < (1ll << 31), NB200_EVALUE, "too many rows and classes");
+  const bool keep = (size_t)rows * classes * sizeof(T) <= kKeepBytes;
+  NB_CUDA(launch_dependent(distill_backward_kernel<T, I>, dim3((unsigned)(rows * pieces)), dim3(kGradThreads), 0, st, x,
+                           index, teacher, reinterpret_cast<const float2 *>(stat), dloss, dx, classes, best, tau, (int)pieces, accum, keep));
+  return NB200_OK;
+}
+
+} // namespace
+} // namespace nb200
+
+using namespace nb200;
+
+extern "C" int nb200_top_k_distillation(const void *x, const void *index, const void *teacher, float *loss, float *stat,
+                                        int64_t rows, int64_t classes, int best, float temperature, int type,
+                                        int index_bytes, void *stream) {
+  NB_TRY(check(rows, classes, best, temperature, index_bytes));
+  if (rows == 0)
+    return NB200_OK;
+  NB_CHECK(x && index && teacher && loss && stat, NB200_EVALUE, "null data pointer");
+  NB_CHECK((reinterpret_cast<uintptr_t>(stat) & 7) == 0, NB200_EVALUE, "stat holds pairs: 8-byte aligned");
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    auto run = [&](auto i) {
+      using I = decltype(i);
+      return forward<T, I>(static_cast<const T *>(x), static_cast<const I *>(index), static_cast<const T *>(teacher), loss,
+                           stat, rows, classes, best, temperature, as_stream(stream));
+    };
+    return index_bytes == 8 ? run(int64_t{}) : run(int32_t{});
+  });
+}
+
+extern "C" int nb200_top_k_distillation_backward(const void *x, const void *index, const void *teacher,
+                                                 const float *stat, const float *dloss, void *dx, int64_t rows,
+                                                 int64_t classes, int best, float temperature, int type, int index_bytes,
+                                                 int accum, void *stream) {
+  NB_TRY(check(rows, classes, best, temperature, index_bytes));
+  if (rows == 0)
+    return NB200_OK;
+  NB_CHECK(x && index && teacher && stat && dloss && dx, NB200_EVALUE, "null data pointer");
+  NB_CHECK((reinterpret_cast<uintptr_t>(stat) & 7) == 0, NB200_EVALUE, "stat holds pairs: 8-byte aligned");
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    auto run = [&](auto i) {
+      using I = decltype(i);
+      return backward<T, I>(static_cast<const T *>(x), static_cast<const I *>(index), static_cast<const T *>(teacher),
+                            stat, dloss, static_cast<T *>(dx), rows, classes, best, temperature, accum != 0,
+                            as_stream(stream));
+    };
+    return index_bytes == 8 ? run(int64_t{}) : run(int32_t{});
+  });
+}

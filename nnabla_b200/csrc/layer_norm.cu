@@ -1,0 +1,564 @@
+// LayerNormalization over the trailing axes, forward and backward, in fp32, bf16 or fp16.
+//
+//   mean = sum x / C, variance = sum (x - mean)^2 / C, r = 1 / sqrt(variance + eps), u = (x - mean) r
+//   y = u gamma + beta
+//   g = dy gamma:  dx = r (g - mean(g) - u mean(g u));  dgamma = sum over rows of dy u, dbeta = sum over rows of dy
+//
+// HBM bound: a row is read once into registers (a warp's, for short rows, or a block's), the variance is taken from the
+// centred values there, so that a large mean costs no digits.
+#include <algorithm>
+
+#include "pdl.cuh"
+#include "typed.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr int kNormMaxWarps = 32;
+
+// Sums of N values over the threads of a row: a warp's, or (row_warps > 1) the block's. Every thread gets them.
+// `turn` alternates the shared slots, so that one barrier a sum is enough.
+template <int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int row_warps, float (*slots)[N][kNormMaxWarps], int &turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v[i] = warp_sum(v[i]);
+  if (row_warps == 1)
+    return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float(*s)[kNormMaxWarps] = slots[turn];
+  turn ^= 1;
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      s[i][warp] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v[i] = warp_sum(lane < row_warps ? s[i][lane] : 0.0f);
+}
+
+// VEC values an access, NV accesses a thread; a row belongs to row_warps warps, and a block holds one row or (row_warps == 1)
+// a row a warp.
+template <typename T, typename P, int VEC, int NV>
+__global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ x, const P *__restrict__ beta,
+                                                          const P *__restrict__ gamma, T *__restrict__ y,
+                                                          float *__restrict__ mean_out, float *__restrict__ var_out,
+                                                          int64_t rows, int size, float inv_size, float eps, int row_warps,
+                                                          bool keep) {
+  __shared__ float slots[2][1][kNormMaxWarps];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
+  if (row >= rows) // (whole warps, and never where the block shares a row)
+    return;
+  const int at = (row_warps == 1 ? lane : (int)threadIdx.x) * VEC, step = row_warps * 32 * VEC;
+  const T *xr = x + row * size;
+  Pack<T, VEC> v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (at + i * step < size)
+      v[i] = load_pack_stream<T, VEC>(xr + at + i * step);
+  int turn = 0;
+  float sum[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (at + i * step < size)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        sum[0] += v[i].f(j);
+  row_sums<1>(sum, row_warps, slots, turn);
+  const float mean = sum[0] * inv_size;
+  float sq[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (at + i * step < size)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = v[i].f(j) - mean;
+        sq[0] = fmaf(d, d, sq[0]);
+      }
+  row_sums<1>(sq, row_warps, slots, turn);
+  const float var = sq[0] * inv_size;
+  const float r = 1.0f / sqrtf(var + eps);
+  if (at == 0) {
+    if (mean_out)
+      mean_out[row] = mean;
+    if (var_out)
+      var_out[row] = var;
+  }
+  T *yr = y + row * size;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = at + i * step;
+    if (c >= size)
+      continue;
+    Pack<P, VEC> g, b;
+    if (gamma)
+      g = load_pack<P, VEC>(gamma + c);
+    if (beta)
+      b = load_pack<P, VEC>(beta + c);
+    float o[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      o[j] = (v[i].f(j) - mean) * r;
+      if (gamma)
+        o[j] *= g.f(j);
+      if (beta)
+        o[j] += b.f(j);
+    }
+    store_pack<T, VEC>(yr + c, o, keep);
+  }
+}
+
+// Sums over the blocks of a cluster: each leaves its own in its shared memory and reads the others'. Fixed order.
+template <int N> __device__ __forceinline__ void cluster_sums(float (&v)[N], float *slot, int blocks) {
+  // (all threads hold the block's sums; slot: N floats of shared memory, not used again before the next cluster barrier)
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      slot[i] = v[i];
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v[i] = 0.0f;
+  for (int b = 0; b < blocks; ++b)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(slot + i));
+      uint32_t theirs;
+      float f;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(b));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(theirs) : "memory");
+      v[i] += f;
+    }
+}
+
+constexpr int kLongThreads = 512, kLongBlocks = 8;
+
+// Rows that no block holds in registers, or a few long ones: a cluster of eight blocks a row, each with an eighth of it,
+// which it reads three times (from the second time on mostly from L2). kBackward: dx instead of y, with dy, mean and
+// variance given.
+template <typename T, typename P, bool kBackward>
+__global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThreads)
+    layer_norm_long_kernel(const T *__restrict__ x, const T *__restrict__ dy, const P *__restrict__ beta,
+                           const P *__restrict__ gamma, T *y, float *mean_io, float *var_io, int64_t size, float eps,
+                           bool accum) {
+  __shared__ float slots[2][kBackward ? 2 : 1][kNormMaxWarps];
+  __shared__ float shared_sums[2][2];
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = blockIdx.x / kLongBlocks;
+  const int part = blockIdx.x % kLongBlocks;
+  const int64_t each = (size + kLongBlocks - 1) / kLongBlocks, c0 = part * each;
+  const int64_t c1 = c0 + each < size ? c0 + each : size;
+  const T *xr = x + row * size;
+  T *yr = y + row * size;
+  const double inv = 1.0 / (double)size;
+  int turn = 0;
+  // f(c, sums) for this thread's values, 64 at a time in fp32 and those sums in 64 bits
+  auto sum_up = [&](auto &s, auto f) {
+    constexpr int kN = sizeof(s) / sizeof(float);
+    double total[kN] = {};
+    for (int64_t base = c0 + threadIdx.x; base < c1; base += 64 * kLongThreads) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        s[i] = 0.0f;
+#pragma unroll 8
+      for (int k = 0; k < 64; ++k)
+        if (base + k * kLongThreads < c1)
+          f(base + k * kLongThreads);
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        total[i] += s[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      s[i] = (float)total[i];
+  };
+  if constexpr (!kBackward) {
+    float s[1];
+    sum_up(s, [&](int64_t c) { s[0] += to_f32(xr[c]); });
+    row_sums<1>(s, kLongThreads / 32, slots, turn);
+    cluster_sums<1>(s, shared_sums[0], kLongBlocks);
+    const float mean = (float)(s[0] * inv);
+    sum_up(s, [&](int64_t c) {
+      const float d = to_f32(xr[c]) - mean;
+      s[0] = fmaf(d, d, s[0]);
+    });
+    row_sums<1>(s, kLongThreads / 32, slots, turn);
+    cluster_sums<1>(s, shared_sums[1], kLongBlocks);
+    const float var = (float)(s[0] * inv), r = 1.0f / sqrtf(var + eps);
+    if (part == 0 && threadIdx.x == 0) {
+      if (mean_io)
+        mean_io[row] = mean;
+      if (var_io)
+        var_io[row] = var;
+    }
+#pragma unroll 8
+    for (int64_t c = c0 + threadIdx.x; c < c1; c += kLongThreads) {
+      float o = (to_f32(xr[c]) - mean) * r;
+      if (gamma)
+        o *= to_f32(gamma[c]);
+      if (beta)
+        o += to_f32(beta[c]);
+      yr[c] = from_f32<T>(o);
+    }
+  } else {
+    const T *dr = dy + row * size;
+    const float mean = mean_io[row], r = 1.0f / sqrtf(var_io[row] + eps);
+    float s[2];
+    sum_up(s, [&](int64_t c) {
+      const float g = gamma ? to_f32(dr[c]) * to_f32(gamma[c]) : to_f32(dr[c]);
+      s[0] += g;
+      s[1] = fmaf(g, (to_f32(xr[c]) - mean) * r, s[1]);
+    });
+    row_sums<2>(s, kLongThreads / 32, slots, turn);
+    cluster_sums<2>(s, shared_sums[0], kLongBlocks);
+    const float m1 = (float)(s[0] * inv), m2 = (float)(s[1] * inv);
+#pragma unroll 8
+    for (int64_t c = c0 + threadIdx.x; c < c1; c += kLongThreads) {
+      const float g = gamma ? to_f32(dr[c]) * to_f32(gamma[c]) : to_f32(dr[c]);
+      float o = r * (g - m1 - (to_f32(xr[c]) - mean) * r * m2);
+      if (accum)
+        o += to_f32(yr[c]);
+      yr[c] = from_f32<T>(o);
+    }
+  }
+  // no block leaves while another may still read its sums
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// dx, and where kParams the sums over this block's rows of dy and dy u, each thread for the columns that it holds: a block
+// (or a warp of it, for short rows) walks over the rows, and leaves partial sums [blocks][2][size] for
+// layer_norm_param_kernel.
+template <typename T, typename P, int VEC, int NV, bool kParams>
+__global__ void __launch_bounds__(512) layer_norm_backward_kernel(
+    const T *__restrict__ x, const T *__restrict__ dy, const P *__restrict__ gamma, const float *__restrict__ mean,
+    const float *__restrict__ var, T *dx, float *__restrict__ partial, int64_t rows, int size, float inv_size, float eps,
+    int row_warps, bool accum, bool keep) {
+  __shared__ float slots[2][2][kNormMaxWarps];
+  extern __shared__ float combine[]; // [warps][2][size], where a row is a warp's
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int at = (row_warps == 1 ? lane : (int)threadIdx.x) * VEC, step = row_warps * 32 * VEC;
+  const int64_t first = row_warps == 1 ? (int64_t)blockIdx.x * warps + warp : (int64_t)blockIdx.x;
+  const int64_t stride = row_warps == 1 ? (int64_t)gridDim.x * warps : (int64_t)gridDim.x;
+  float sum_dy[NV * VEC], sum_dyu[NV * VEC];
+#pragma unroll
+  for (int i = 0; i < NV * VEC; ++i)
+    sum_dy[i] = sum_dyu[i] = 0.0f;
+  int turn = 0;
+  for (int64_t row = first; row < rows; row += stride) {
+    const T *xr = x + row * size, *dr = dy + row * size;
+    Pack<T, VEC> xv[NV], dv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (at + i * step < size) {
+        xv[i] = load_pack_stream<T, VEC>(xr + at + i * step);
+        dv[i] = load_pack_stream<T, VEC>(dr + at + i * step);
+      }
+    const float mu = mean[row], r = 1.0f / sqrtf(var[row] + eps);
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = at + i * step;
+      if (c >= size)
+        continue;
+      Pack<P, VEC> g;
+      if (gamma)
+        g = load_pack<P, VEC>(gamma + c);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g.f(j) : d;
+        s[0] += gd;
+        s[1] = fmaf(gd, u, s[1]);
+        if (kParams) {
+          sum_dy[i * VEC + j] += d;
+          sum_dyu[i * VEC + j] = fmaf(d, u, sum_dyu[i * VEC + j]);
+        }
+      }
+    }
+    if (!dx)
+      continue;
+    row_sums<2>(s, row_warps, slots, turn);
+    const float m1 = s[0] * inv_size, m2 = s[1] * inv_size;
+    T *out = dx + row * size;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = at + i * step;
+      if (c >= size)
+        continue;
+      Pack<P, VEC> g;
+      if (gamma)
+        g = load_pack<P, VEC>(gamma + c);
+      Pack<T, VEC> old;
+      if (accum)
+        old = load_pack<T, VEC>(out + c);
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g.f(j) : d;
+        o[j] = r * (gd - m1 - u * m2);
+        if (accum)
+          o[j] += old.f(j);
+      }
+      store_pack<T, VEC>(out + c, o, keep);
+    }
+  }
+  if constexpr (kParams) {
+    float *mine = partial + (int64_t)blockIdx.x * 2 * size;
+    if (row_warps > 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (at + i * step + j < size) {
+            mine[at + i * step + j] = sum_dy[i * VEC + j];
+            mine[size + at + i * step + j] = sum_dyu[i * VEC + j];
+          }
+      return;
+    }
+    float *own = combine + (size_t)warp * 2 * size;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (at + i * step + j < size) {
+          own[at + i * step + j] = sum_dy[i * VEC + j];
+          own[size + at + i * step + j] = sum_dyu[i * VEC + j];
+        }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * size; c += blockDim.x) {
+      float s = 0.0f;
+      for (int w = 0; w < warps; ++w)
+        s += combine[(size_t)w * 2 * size + c];
+      mine[c] = s;
+    }
+  }
+}
+
+// The same sums for rows too long for the kernel above: a thread a column, a slab of rows a block, partial sums
+// [slabs][2][size].
+template <typename T>
+__global__ void __launch_bounds__(256) layer_norm_columns_kernel(const T *__restrict__ x, const T *__restrict__ dy,
+                                                                 const float *__restrict__ mean,
+                                                                 const float *__restrict__ var,
+                                                                 float *__restrict__ partial, int64_t rows, int64_t size,
+                                                                 int64_t slab, float eps) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= size)
+    return;
+  const int64_t r0 = blockIdx.y * slab, r1 = r0 + slab < rows ? r0 + slab : rows;
+  float a = 0.0f, b = 0.0f;
+#pragma unroll 4
+  for (int64_t row = r0; row < r1; ++row) {
+    const float d = to_f32(dy[row * size + c]);
+    a += d;
+    b = fmaf(d, (to_f32(x[row * size + c]) - mean[row]) * (1.0f / sqrtf(var[row] + eps)), b);
+  }
+  partial[(int64_t)blockIdx.y * 2 * size + c] = a;
+  partial[(int64_t)blockIdx.y * 2 * size + size + c] = b;
+}
+
+// dbeta (+)= sum over the parts of [part][0][c], dgamma of [part][1][c], in a fixed order: a block takes 32 columns, its 16
+// warps the parts in turn.
+template <typename P>
+__global__ void __launch_bounds__(512) layer_norm_param_kernel(const float *__restrict__ partial, int parts, int64_t size,
+                                                               P *dbeta, P *dgamma, bool accum_beta, bool accum_gamma) {
+  __shared__ float sums[16][33];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  P *out = blockIdx.y == 0 ? dbeta : dgamma;
+  if (!out)
+    return;
+  const bool accum = blockIdx.y == 0 ? accum_beta : accum_gamma;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (c < size) {
+    const float *p = partial + (int64_t)blockIdx.y * size + c;
+#pragma unroll 8
+    for (int k = warp; k < parts; k += 16)
+      s += p[(int64_t)k * 2 * size];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < size) {
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+      s += sums[w][lane];
+    if (accum)
+      s += to_f32(out[c]);
+    out[c] = from_f32<P>(s);
+  }
+}
+
+// Threads of a row and accesses of a thread. Rows of up to four accesses a lane are a warp's (no barrier); longer ones a
+// block's, two accesses a thread where that is enough threads to fill the SMs, one where the rows are fewer than them.
+struct RowShape {
+  int row_warps, nv;
+  bool fits;
+};
+RowShape row_shape(int64_t size, int vec, int64_t rows, int max_threads, int max_nv) {
+  const int64_t packs = (size + vec - 1) / vec;
+  if (packs <= 32)
+    return {1, 1, true};
+  const bool few = rows < 2 * sm_count();
+  if (packs <= 128 && !few)
+    return {1, packs <= 64 ? 2 : 4, true};
+  int threads = 64;
+  while (threads < max_threads && (int64_t)threads * (few ? 1 : 2) < packs)
+    threads *= 2;
+  int nv = 1;
+  while (nv < max_nv && (int64_t)threads * nv < packs)
+    nv *= 2;
+  return {threads / 32, nv, (int64_t)threads * nv >= packs};
+}
+
+template <int... N, typename F> int with_count(int n, std::integer_sequence<int, N...>, F f) {
+  int rc = NB200_EVALUE;
+  ((n == N ? (rc = f(std::integral_constant<int, N>{}), 0) : 0), ...);
+  return rc;
+}
+using Counts = std::integer_sequence<int, 1, 2, 4, 8, 16, 32>;
+
+int check_sizes(int64_t rows, int64_t size, int64_t per_row_blocks) {
+  NB_CHECK(size > 0, NB200_EVALUE, "an empty row has no mean");
+  NB_CHECK(size < (1ll << 31), NB200_EVALUE, "a row has 2^31 values or more");
+  NB_CHECK(rows >= 0 && rows * per_row_blocks < (1ll << 31), NB200_EVALUE, "too many rows");
+  return NB200_OK;
+}
+
+template <typename T, typename P>
+int forward(const T *x, const P *beta, const P *gamma, T *y, float *mean, float *var, int64_t rows, int64_t size, float eps,
+            cudaStream_t st) {
+  const bool keep = (size_t)rows * size * sizeof(T) <= kKeepBytes;
+  auto run = [&](auto vec) -> int {
+    constexpr int kVec = decltype(vec)::value;
+    const RowShape s = row_shape(size, kVec, rows, 1024, kVec == 1 ? 32 : 8);
+    if (!s.fits || (rows <= sm_count() / kLongBlocks && size >= 32768)) {
+      NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, false>, dim3((unsigned)(rows * kLongBlocks)), dim3(kLongThreads),
+                               0, st, x, (const T *)nullptr, beta, gamma, y, mean, var, size, eps, false));
+      return NB200_OK;
+    }
+    const int per_block = s.row_warps == 1 ? 4 : 1;
+    return with_count(s.nv, Counts{}, [&](auto nv) -> int {
+      constexpr int kNv = decltype(nv)::value;
+      if constexpr (kVec == 1 || kNv <= 8)
+        NB_CUDA(launch_dependent(layer_norm_kernel<T, P, kVec, kNv>, dim3((unsigned)((rows + per_block - 1) / per_block)),
+                                 dim3(32 * s.row_warps * per_block), 0, st, x, beta, gamma, y, mean, var, rows, (int)size,
+                                 1.0f / (float)size, eps, s.row_warps, keep));
+      return NB200_OK;
+    });
+  };
+  const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(beta);
+  return vec ? run(std::integral_constant<int, kPackOf<T>>{}) : run(std::integral_constant<int, 1>{});
+}
+
+template <typename T, typename P>
+int backward(const T *x, const T *dy, const P *gamma, const float *mean, const float *var, T *dx, P *dbeta, P *dgamma,
+             int64_t rows, int64_t size, float eps, bool accum_dx, bool accum_beta, bool accum_gamma, cudaStream_t st) {
+  const bool params = dbeta || dgamma, keep = (size_t)rows * size * sizeof(T) <= kKeepBytes;
+  AsyncScratch scratch(st);
+  int parts = 0;
+  auto run = [&](auto vec) -> int {
+    constexpr int kVec = decltype(vec)::value;
+    const RowShape s = row_shape(size, kVec, rows, 512, kVec == 1 ? 16 : 4);
+    if (!s.fits) {
+      if (params) {
+        const int64_t columns = (size + 255) / 256;
+        const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, 8 * sm_count() / columns));
+        const int64_t slab = (rows + slabs - 1) / slabs;
+        parts = (int)((rows + slab - 1) / slab);
+        NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));
+        NB_CUDA(launch_dependent(layer_norm_columns_kernel<T>, dim3((unsigned)columns, (unsigned)parts), dim3(256), 0, st, x,
+                                 dy, mean, var, static_cast<float *>(scratch.p), rows, size, slab, eps));
+      }
+      if (dx) // (after the sums: it may overwrite x or dy)
+        NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, true>, dim3((unsigned)(rows * kLongBlocks)),
+                                 dim3(kLongThreads), 0, st, x, dy, (const P *)nullptr, gamma, dx, const_cast<float *>(mean),
+                                 const_cast<float *>(var), size, eps, accum_dx));
+      return NB200_OK;
+    }
+    const int per_block = s.row_warps == 1 ? 8 : 1, threads = 32 * s.row_warps * per_block;
+    const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, (int64_t)sm_count() * (1024 / threads));
+    if (params) {
+      parts = (int)blocks;
+      NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));
+    }
+    const size_t smem = params && s.row_warps == 1 ? (size_t)per_block * 2 * size * 4 : 0;
+    return with_count(s.nv, Counts{}, [&](auto nv) -> int {
+      constexpr int kNv = decltype(nv)::value;
+      if constexpr (kNv <= (kVec == 1 ? 16 : 4)) {
+        auto kernel = params ? layer_norm_backward_kernel<T, P, kVec, kNv, true>
+                             : layer_norm_backward_kernel<T, P, kVec, kNv, false>;
+        if (smem > 48 * 1024)
+          NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        NB_CUDA(launch_dependent(kernel, dim3((unsigned)blocks), dim3(threads), smem, st, x, dy, gamma, mean, var, dx,
+                                 static_cast<float *>(scratch.p), rows, (int)size, 1.0f / (float)size, eps, s.row_warps,
+                                 accum_dx, keep));
+      }
+      return NB200_OK;
+    });
+  };
+  if (rows > 0) {
+    const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gamma);
+    NB_TRY(vec ? run(std::integral_constant<int, kPackOf<T>>{}) : run(std::integral_constant<int, 1>{}));
+  }
+  if (params)
+    NB_CUDA(launch_dependent(layer_norm_param_kernel<P>, dim3((unsigned)((size + 31) / 32), 2), dim3(512), 0, st,
+                             static_cast<const float *>(scratch.p), parts, size, dbeta, dgamma, accum_beta, accum_gamma));
+  return NB200_OK;
+}
+
+// f(T{}, P{}) for a type and a parameter type that is the same or fp32
+template <typename F> int with_types(int type, int param_type, F f) {
+  NB_CHECK(param_type == type || param_type == NB200_F32, NB200_EVALUE, "beta and gamma have x's type or float32");
+  return with_type(type, [&](auto t) -> int {
+    using T = decltype(t);
+    return param_type == type ? f(T{}, T{}) : f(T{}, float{});
+  });
+}
+
+} // namespace
+} // namespace nb200
+
+using namespace nb200;
+
+extern "C" int nb200_layer_normalization(const void *x, const void *beta, const void *gamma, void *y, float *mean,
+                                         float *variance, int64_t rows, int64_t size, float eps, int type, int param_type,
+                                         void *stream) {
+  NB_TRY(check_sizes(rows, size, kLongBlocks));
+  if (rows == 0)
+    return NB200_OK;
+  NB_CHECK(x && y, NB200_EVALUE, "null data pointer");
+  return with_types(type, param_type, [&](auto t, auto p) {
+    using T = decltype(t);
+    using P = decltype(p);
+    return forward<T, P>(static_cast<const T *>(x), static_cast<const P *>(beta), static_cast<const P *>(gamma),
+                         static_cast<T *>(y), mean, variance, rows, size, eps, as_stream(stream));
+  });
+}
+
+extern "C" int nb200_layer_normalization_backward(const void *x, const void *dy, const void *gamma, const float *mean,
+                                                  const float *variance, void *dx, void *dbeta, void *dgamma, int64_t rows,
+                                                  int64_t size, float eps, int type, int param_type, int accum_dx,
+                                                  int accum_dbeta, int accum_dgamma, void *stream) {
+  NB_TRY(check_sizes(rows, size, kLongBlocks));
+  NB_CHECK(rows == 0 || (x && dy && mean && variance), NB200_EVALUE, "null data pointer");
+  if (!dx && !dbeta && !dgamma)
+    return NB200_OK;
+  return with_types(type, param_type, [&](auto t, auto p) {
+    using T = decltype(t);
+    using P = decltype(p);
+    return backward<T, P>(static_cast<const T *>(x), static_cast<const T *>(dy), static_cast<const P *>(gamma), mean,
+                          variance, static_cast<T *>(dx), static_cast<P *>(dbeta), static_cast<P *>(dgamma), rows, size, eps,
+                          accum_dx != 0, accum_dbeta != 0, accum_dgamma != 0, as_stream(stream));
+  });
+}

@@ -902,6 +902,10 @@ PyMethodDef methods[] = {
     ENTRY(nb200_prune_backward_f32),
     ENTRY(nb200_inq_restore_f32),
     ENTRY(nb200_inq_quantize_f32),
+    ENTRY(nb200_layer_normalization),
+    ENTRY(nb200_layer_normalization_backward),
+    ENTRY(nb200_top_k_distillation),
+    ENTRY(nb200_top_k_distillation_backward),
     ENTRY(nb200_affine_f32),
     ENTRY(nb200_affine_fxp8_f32),
     ENTRY(nb200_affine_codes_i8_f32),

@@ -1,0 +1,74 @@
+// Operands in fp32, bf16 or fp16: the kernels that take all three read them into fp32 registers, compute there, and round
+// once where they store.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace nb200 {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// N neighbouring values as they lie in memory (16-byte accesses where N values are 16 bytes or a multiple of it)
+template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+  T v[N];
+  __device__ __forceinline__ float f(int i) const { return to_f32(v[i]); }
+};
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
+  return *reinterpret_cast<const Pack<T, N> *>(p);
+}
+// The same for data that this pass reads once (kStream) and for results: ordinary or streaming.
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack_stream(const T *p) {
+  if constexpr (N * sizeof(T) == 16) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
+    return *reinterpret_cast<const Pack<T, N> *>(&u);
+  } else {
+    return load_pack<T, N>(p);
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const float (&v)[N], bool keep = true) {
+  Pack<T, N> o;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    o.v[i] = from_f32<T>(v[i]);
+  if constexpr (N * sizeof(T) == 16)
+    st_result(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(&o), keep);
+  else
+    *reinterpret_cast<Pack<T, N> *>(p) = o;
+}
+
+template <typename T> constexpr int kPackOf = (int)(16 / sizeof(T)); // values in 16 bytes
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1)
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+
+// Calls f(T{}) with the C++ type of an NB200_F32 / _BF16 / _F16 code.
+template <typename F> int with_type(int code, F f) {
+  switch (code) {
+  case NB200_F32: return f(float{});
+  case NB200_BF16: return f(__nv_bfloat16{});
+  case NB200_F16: return f(__half{});
+  }
+  return fail(NB200_EVALUE, "unknown type code %d", code);
+}
+inline size_t type_bytes(int code) { return code == NB200_F32 ? 4 : 2; }
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+} // namespace nb200

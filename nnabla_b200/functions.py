@@ -1413,3 +1413,202 @@ def prune_backward(dy, accum=False, dx=None):
     _, dy, dx = _grad_buffers(dy, dy, dx, accum)
     L.nb200_prune_backward_f32(dy, dx, dy.numel(), bool(accum))
     return dx
+
+
+# ---------------------------------------------------------------------------
+# The end of a network that is trained: normalization over features, and its
+# losses. These take float32, bfloat16 or float16 tensors; sums, statistics and
+# losses are float32.
+# ---------------------------------------------------------------------------
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # NB200_F32, NB200_BF16, NB200_F16
+
+
+def _typed(t, name, like=None, dtypes=None):
+    """`t` as a contiguous CUDA tensor of one of `dtypes` (default: the three types), on the device of `like`."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor on a CUDA device" % name)
+    if not t.is_cuda:
+        raise RuntimeError("nnabla_b200 has no CPU path: %s is on %s" % (name, t.device))
+    if t.dtype not in (dtypes or _TYPES):
+        raise TypeError("%s must be %s, got %s" % (
+            name, " or ".join(str(d).replace("torch.", "") for d in (dtypes or _TYPES)), t.dtype))
+    if like is not None and t.device != like.device:
+        raise RuntimeError("%s is on %s, x on %s" % (name, t.device, like.device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _buffer(t, name, like, accum, shape=None):
+    """The gradient or output buffer `t` of `like`'s type and of `shape` (default: like's), or a new one."""
+    shape = tuple(like.shape if shape is None else shape)
+    if t is None:
+        if accum:
+            raise RuntimeError("accum needs the gradient buffer to add to (%s)" % name)
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if (not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != like.dtype or t.device != like.device
+            or not t.is_contiguous()):
+        raise RuntimeError("%s must be a contiguous %s tensor of shape %s on %s" % (
+            name, str(like.dtype).replace("torch.", ""), shape, like.device))
+    _wrote(t)
+    return t
+
+
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
+        return False
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
+def _disjoint(written, read):
+    """`written` and `read`: (name, tensor or None) pairs; no result may lie in an operand, nor in another result."""
+    for i, (name, t) in enumerate(written):
+        for other, u in list(read) + list(written[:i]):
+            if _overlap(t, u):
+                raise RuntimeError("%s and %s share memory" % (name, other))
+
+
+def _batch_axes(x, batch_axis):
+    """The number of leading axes of x that batch_axis names; LayerNormalization normalizes over the others."""
+    axes = [batch_axis] if isinstance(batch_axis, int) else list(batch_axis)
+    axes = sorted(a + x.dim() if a < 0 else a for a in axes)
+    if axes and (axes[0] < 0 or axes[-1] >= x.dim()) or len(set(axes)) != len(axes):
+        raise RuntimeError("batch_axis %s does not fit an input with %d axes" % (batch_axis, x.dim()))
+    if axes != list(range(len(axes))):
+        raise C.NB200Error(4, "batch_axis must name the leading axes (got %s)" % (batch_axis,))
+    if len(axes) == x.dim():
+        raise RuntimeError("batch_axis leaves no axis to normalize over")
+    return len(axes)
+
+
+def _norm_operands(x, parameters, batch_axis):
+    """(x, its checked parameters, their dtype, rows, size, number of batch axes) of a layer normalization."""
+    x = _typed(x, "x")
+    lead = _batch_axes(x, batch_axis)
+    shapes = (tuple(x.shape[lead:]), (1,) * lead + tuple(x.shape[lead:]))
+    rows = size = 1
+    for s in x.shape[:lead]:
+        rows *= int(s)
+    for s in x.shape[lead:]:
+        size *= int(s)
+    out, dtype = [], None
+    for t, name in parameters:
+        if t is not None:
+            t = _typed(t, name, x, (x.dtype, torch.float32))
+            if tuple(t.shape) not in shapes:
+                raise RuntimeError("%s must have the shape %s or %s, got %s" % (name, shapes[1], shapes[0], tuple(t.shape)))
+            if dtype is not None and t.dtype != dtype:
+                raise TypeError("beta and gamma must have one type")
+            dtype = t.dtype
+        out.append(t)
+    return x, out, dtype or x.dtype, rows, size, lead
+
+
+def layer_normalization(x, beta, gamma, batch_axis=0, eps=1e-05, output_stat=False, n_outputs=None, outputs=None):
+    """Layer normalization (nnabla.functions.layer_normalization): y = (x - mean) / sqrt(variance + eps) * gamma + beta,
+    with the mean and the biased variance over all axes but batch_axis.
+
+    x: float32, bfloat16 or float16. batch_axis: an axis or a list of axes, the leading ones of x. beta, gamma: of x's shape
+    with 1 for the batch axes (or without those axes), in x's type or float32, or None. output_stat=True also returns the
+    mean and the variance, float32, of x's shape with 1 for the normalized axes: what the backward pass needs.
+    outputs: [y], a contiguous tensor like x, which may be x itself."""
+    x, (beta, gamma), dtype, rows, size, lead = _norm_operands(x, ((beta, "beta"), (gamma, "gamma")), batch_axis)
+    y = _buffer(None if outputs is None else outputs[0], "outputs[0]", x, False)
+    if outputs is not None:
+        _disjoint([("outputs[0]", y)], [("beta", beta), ("gamma", gamma)])
+        if y.data_ptr() != x.data_ptr():
+            _disjoint([("outputs[0]", y)], [("x", x)])
+    mean = variance = None
+    if output_stat:
+        stat_shape = tuple(x.shape[:lead]) + (1,) * (x.dim() - lead)
+        mean, variance = L.empty(stat_shape, x), L.empty(stat_shape, x)
+    L.nb200_layer_normalization(x, beta, gamma, y, mean, variance, rows, size, eps, _TYPES[x.dtype], _TYPES[dtype])
+    return (y, mean, variance) if output_stat else y
+
+
+def layer_normalization_backward(x, dy, gamma, mean, variance, batch_axis=0, eps=1e-05, propagate_down=(True, True, True),
+                                 accum=(False, False, False), grads=(None, None, None), beta=None):
+    """The gradients of layer_normalization. mean, variance: what the forward pass returned with output_stat=True (no
+    gradient arrives at them). Returns (dx, dbeta, dgamma), None where propagate_down is False. dbeta and dgamma have
+    gamma's shape and type, or beta's where gamma is None; without both, (1, ..., size) and float32. The sums over the rows
+    are added in a fixed order. grads[0] may be dy or x."""
+    x, (gamma, beta), dtype, rows, size, lead = _norm_operands(x, ((gamma, "gamma"), (beta, "beta")), batch_axis)
+    dy = _typed(dy, "dy", x, (x.dtype,))
+    if dy.shape != x.shape:
+        raise RuntimeError("dy must have x's shape")
+    mean, variance = _typed(mean, "mean", x, (torch.float32,)), _typed(variance, "variance", x, (torch.float32,))
+    if mean.numel() != rows or variance.numel() != rows:
+        raise RuntimeError("mean and variance must have %d values, one a row" % rows)
+    like = gamma if gamma is not None else beta
+    if like is None:
+        dtype = torch.float32
+        like = L.empty((1,) * lead + tuple(x.shape[lead:]), x)
+    dx = _buffer(grads[0], "grads[0]", x, accum[0]) if propagate_down[0] else None
+    db = _buffer(grads[1], "grads[1]", like, accum[1]) if propagate_down[1] else None
+    dg = _buffer(grads[2], "grads[2]", like, accum[2]) if propagate_down[2] else None
+    if any(g is not None for g in grads):
+        operands = [("gamma", gamma), ("mean", mean), ("variance", variance)]
+        _disjoint([("grads[0]", dx), ("grads[1]", db), ("grads[2]", dg)], operands)
+        _disjoint([("grads[1]", db), ("grads[2]", dg)], [("x", x), ("dy", dy)])
+        for name, t in (("x", x), ("dy", dy)):
+            if dx is not None and dx.data_ptr() != t.data_ptr():
+                _disjoint([("grads[0]", dx)], [(name, t)])
+    L.nb200_layer_normalization_backward(x, dy, gamma, mean, variance, dx, db, dg, rows, size, eps, _TYPES[x.dtype],
+                                         _TYPES[dtype], bool(accum[0]), bool(accum[1]), bool(accum[2]))
+    return dx, db, dg
+
+
+_INTEGERS = (torch.int32, torch.int64)
+
+
+def _distillation_operands(x, index, teacher, temperature):
+    x = _typed(x, "x")
+    if x.dim() < 1:
+        raise RuntimeError("x needs an axis of classes")
+    index, teacher = _typed(index, "index", x, _INTEGERS), _typed(teacher, "teacher", x, (x.dtype,))
+    if index.shape != teacher.shape or index.shape[:-1] != x.shape[:-1] or index.dim() != x.dim():
+        raise RuntimeError("index and teacher must have one shape, x's but for the last axis")
+    if not 0 < temperature < float("inf"):
+        raise RuntimeError("temperature must be positive")
+    classes = int(x.shape[-1])
+    if classes == 0:
+        raise RuntimeError("x has no classes")
+    return x, index, teacher, x.numel() // classes, classes, int(index.shape[-1])
+
+
+def top_k_distillation(x, index, teacher, temperature=1.0, output_stat=False, n_outputs=-1, outputs=None):
+    """Distillation from the best classes of a teacher: of each row, temperature^2 * KL(p || q) with p the softmax of
+    teacher / temperature over the row's entries, q the softmax of x / temperature over all classes.
+
+    x: logits (..., classes), float32, bfloat16 or float16. index, teacher: (..., K), the classes (int32 or int64) and the
+    teacher's logits for them (x's type), K up to 1024. An entry with a negative class is none: a row may have fewer than
+    K, and one without any has the loss 0 and no gradient. A class that is named twice counts twice; one that does not exist
+    makes its row's loss and gradient NaN. Returns the loss (..., 1), float32; with output_stat=True also
+    (..., 2), float32, what the backward pass needs: the row's maximum, and log sum exp((x - maximum) / temperature)."""
+    x, index, teacher, rows, classes, best = _distillation_operands(x, index, teacher, temperature)
+    shape = tuple(x.shape[:-1]) + (1,)
+    like = L.empty(shape, x)
+    loss = like if outputs is None else _buffer(outputs[0], "outputs[0]", like, False)
+    stat = L.empty(tuple(x.shape[:-1]) + (2,), x)
+    if outputs is not None:
+        _disjoint([("outputs[0]", loss)], [("x", x), ("index", index), ("teacher", teacher)])
+    L.nb200_top_k_distillation(x, index, teacher, loss, stat, rows, classes, best, temperature, _TYPES[x.dtype],
+                               index.element_size())
+    return (loss, stat) if output_stat else loss
+
+
+def top_k_distillation_backward(x, index, teacher, stat, dloss, temperature=1.0, accum=False, dx=None):
+    """The gradient of top_k_distillation for x: temperature * (q - p) * dloss. stat: the forward pass's; dloss: float32,
+    one value a row. dx receives it, or (accum=True) has it added; it may be x itself."""
+    x, index, teacher, rows, classes, best = _distillation_operands(x, index, teacher, temperature)
+    stat, dloss = _typed(stat, "stat", x, (torch.float32,)), _typed(dloss, "dloss", x, (torch.float32,))
+    if stat.numel() != 2 * rows or dloss.numel() != rows:
+        raise RuntimeError("stat and dloss must have two values and one value a row")
+    given, dx = dx, _buffer(dx, "dx", x, accum)
+    if given is not None:
+        operands = [("index", index), ("teacher", teacher), ("stat", stat), ("dloss", dloss)]
+        _disjoint([("dx", dx)], operands if dx.data_ptr() == x.data_ptr() else operands + [("x", x)])
+    L.nb200_top_k_distillation_backward(x, index, teacher, stat, dloss, dx, rows, classes, best, temperature,
+                                        _TYPES[x.dtype], index.element_size(), bool(accum))
+    return dx
