@@ -666,6 +666,24 @@ int nb200_layer_normalization_backward(const void *x, const void *dy, const void
                                        int64_t size, float eps, int type, int param_type, int accum_dx,
                                        int accum_dbeta, int accum_dgamma, void *stream);
 
+/* Softmax cross entropy of an affine layer's classes: l = x [rows, size] . w [size, classes] + bias [classes] (NULL:
+ * none), all of one type; label [rows] int32 or int64 (label_bytes).
+ *   loss = log sum exp(l) - l[label]   (fp32, [rows])
+ * stat [rows, 2], fp32: the row's largest l, and log sum exp(l - largest).
+ * A row with a negative label has the loss 0; a label >= classes makes its row's loss NaN. The logits are never
+ * kept: the scratch that a call takes grows with the rows and not with rows * classes. */
+int nb200_affine_softmax_cross_entropy(const void *x, const void *w, const void *bias, const void *label,
+                                       float *loss, float *stat, int64_t rows, int64_t size, int64_t classes,
+                                       int type, int label_bytes, void *stream);
+/* Its gradients: G = (softmax(l) - onehot(label)) * dloss, zero in rows with a negative label; dx (+)= G . w^T,
+ * dw (+)= x^T . G, db (+)= the sums of G over the rows; each may be NULL (not propagated). stat is the forward
+ * pass's. Deterministic: sums are added in a fixed order. No result may lie in an operand. */
+int nb200_affine_softmax_cross_entropy_backward(const void *x, const void *w, const void *bias, const void *label,
+                                                const float *stat, const float *dloss, void *dx, void *dw, void *db,
+                                                int64_t rows, int64_t size, int64_t classes, int type,
+                                                int label_bytes, int accum_dx, int accum_dw, int accum_db,
+                                                void *stream);
+
 /* Distillation from the teacher's best classes: x [rows, classes] the student's logits, index [rows, best] the
  * classes (int32 or int64: index_bytes) and teacher [rows, best] their logits in x's type; an entry whose class is
  * negative is none.

@@ -904,6 +904,8 @@ PyMethodDef methods[] = {
     ENTRY(nb200_inq_quantize_f32),
     ENTRY(nb200_layer_normalization),
     ENTRY(nb200_layer_normalization_backward),
+    ENTRY(nb200_affine_softmax_cross_entropy),
+    ENTRY(nb200_affine_softmax_cross_entropy_backward),
     ENTRY(nb200_top_k_distillation),
     ENTRY(nb200_top_k_distillation_backward),
     ENTRY(nb200_affine_f32),

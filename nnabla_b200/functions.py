@@ -1424,6 +1424,9 @@ def prune_backward(dy, accum=False, dx=None):
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # NB200_F32, NB200_BF16, NB200_F16
 
 
+_INTEGERS = (torch.int32, torch.int64)
+
+
 def _typed(t, name, like=None, dtypes=None):
     """`t` as a contiguous CUDA tensor of one of `dtypes` (default: the three types), on the device of `like`."""
     if not isinstance(t, torch.Tensor):
@@ -1559,7 +1562,62 @@ def layer_normalization_backward(x, dy, gamma, mean, variance, batch_axis=0, eps
     return dx, db, dg
 
 
-_INTEGERS = (torch.int32, torch.int64)
+def _loss_operands(x, weight, label, bias, base_axis):
+    x = _typed(x, "x")
+    weight = _typed(weight, "weight", x, (x.dtype,))
+    bias = _typed(bias, "bias", x, (x.dtype,)) if bias is not None else None
+    if weight.dim() != 2:
+        raise RuntimeError("weight must be a matrix (inputs, classes)")
+    rows, size, classes, out_shape = _affine_dims(x, weight, base_axis, bias)
+    label = _typed(label, "label", x, _INTEGERS)
+    if tuple(label.shape) not in (out_shape[:-1], out_shape[:-1] + (1,)):
+        raise RuntimeError("label must have the shape %s or %s, got %s" % (
+            out_shape[:-1] + (1,), out_shape[:-1], tuple(label.shape)))
+    if size == 0 or classes == 0:
+        raise RuntimeError("weight is empty")
+    return x, weight, label, bias, rows, size, classes, out_shape[:-1]
+
+
+def affine_softmax_cross_entropy(x, weight, label, bias=None, base_axis=1, output_stat=False, n_outputs=-1, outputs=None):
+    """softmax_cross_entropy(affine(x, weight, bias, base_axis), label) without its logits: the loss of a classifying head
+    whose classes are many. Of each row, log sum exp(l) - l[label] with l = x . weight + bias.
+
+    x, weight (inputs, classes), bias (classes,): one type, float32, bfloat16 or float16. label: int32 or int64, one value
+    a row. A row with a negative label does not count: its loss is 0. A label >= classes makes its row's loss NaN.
+    Returns the loss, float32, x.shape[:base_axis] + (1,); with output_stat=True also x.shape[:base_axis] + (2,), float32,
+    what the backward pass needs: the row's largest logit, and log sum exp(l - largest)."""
+    x, weight, label, bias, rows, size, classes, lead = _loss_operands(x, weight, label, bias, base_axis)
+    loss = L.empty(lead + (1,), x)
+    if outputs is not None:
+        loss = _buffer(outputs[0], "outputs[0]", loss, False)
+        _disjoint([("outputs[0]", loss)], [("x", x), ("weight", weight), ("bias", bias), ("label", label)])
+    stat = L.empty(lead + (2,), x)
+    L.nb200_affine_softmax_cross_entropy(x, weight, bias, label, loss, stat, rows, size, classes, _TYPES[x.dtype],
+                                         label.element_size())
+    return (loss, stat) if output_stat else loss
+
+
+def affine_softmax_cross_entropy_backward(x, weight, label, stat, dloss, bias=None, base_axis=1,
+                                          propagate_down=(True, True, True), accum=(False, False, False),
+                                          grads=(None, None, None)):
+    """The gradients of affine_softmax_cross_entropy, a piece of the classes after the other. stat: the forward pass's;
+    dloss: float32, one value a row. Returns (dx, dweight, dbias) in the operands' type, None where propagate_down is False
+    or there is no bias. In float16 the gradient at a logit is kept relative to the largest dloss, so that small ones are
+    not lost before the products; scale the loss if the results themselves are too small for the type."""
+    x, weight, label, bias, rows, size, classes, _ = _loss_operands(x, weight, label, bias, base_axis)
+    stat, dloss = _typed(stat, "stat", x, (torch.float32,)), _typed(dloss, "dloss", x, (torch.float32,))
+    if stat.numel() != 2 * rows or dloss.numel() != rows:
+        raise RuntimeError("stat and dloss must have two values and one value a row")
+    dx = _buffer(grads[0], "grads[0]", x, accum[0]) if propagate_down[0] else None
+    dw = _buffer(grads[1], "grads[1]", weight, accum[1]) if propagate_down[1] else None
+    db = _buffer(grads[2], "grads[2]", bias, accum[2]) if propagate_down[2] and bias is not None else None
+    if any(g is not None for g in grads):
+        _disjoint([("grads[0]", dx), ("grads[1]", dw), ("grads[2]", db)],
+                  [("x", x), ("weight", weight), ("bias", bias), ("label", label), ("stat", stat), ("dloss", dloss)])
+    L.nb200_affine_softmax_cross_entropy_backward(x, weight, bias, label, stat, dloss, dx, dw, db, rows, size, classes,
+                                                  _TYPES[x.dtype], label.element_size(), bool(accum[0]), bool(accum[1]),
+                                                  bool(accum[2]))
+    return dx, dw, db
 
 
 def _distillation_operands(x, index, teacher, temperature):
