@@ -9,26 +9,11 @@
 // row of G are 0. A label >= classes makes its row's loss, and every gradient that it enters, NaN.
 #include <algorithm>
 
-#include "pdl.cuh"
-#include "softmax_sums.cuh"
+#include "loss_gemm.cuh"
+#include "prepare.cuh"
 
 namespace nb200 {
 namespace {
-
-// What becomes of a tile of the logits. kSums: partial[row][tile of classes] and the label's logit. kGrad: G.
-struct Rows {
-  const void *label; // label_bytes each
-  int label_bytes;
-  const float2 *stat; // kGrad: of the forward pass
-  const float *dloss;
-  float2 *partial; // kSums: [rows][tiles]
-  float *target;
-  int tiles;
-  int64_t classes;
-  __device__ __forceinline__ int64_t label_of(int64_t row) const {
-    return label_bytes == 8 ? static_cast<const int64_t *>(label)[row] : (int64_t) static_cast<const int32_t *>(label)[row];
-  }
-};
 
 // ---- products on the CUDA cores ------------------------------------------------------------------------------------------
 // D[m, n] = sum_k A(m, k) B(k, n) with any strides, in fp32: 64 x 64 tiles, 16 of K at a time, 4 x 4 results a thread.
@@ -36,11 +21,9 @@ template <typename T> struct Strided {
   const T *p;
   int64_t row, col;
 };
-enum class Out { kSums, kGrad, kStore };
-
 template <typename TA, typename TB, typename TO, Out kOut>
 __global__ void __launch_bounds__(256) simt_product_kernel(Strided<TA> a, Strided<TB> b, int64_t M, int64_t N, int64_t K,
-                                                           const TO *__restrict__ bias, Rows rows, int64_t class0, TO *out,
+                                                           const TO *__restrict__ bias, LossRows rows, int64_t class0, TO *out,
                                                            int64_t ldo, bool accum) {
   __shared__ float as[16][65], bs[16][65];
   pdl_wait();
@@ -121,7 +104,7 @@ __global__ void __launch_bounds__(256) simt_product_kernel(Strided<TA> a, Stride
 }
 
 // The rows' loss and statistics from the tiles' maxima and sums: a warp a row.
-__global__ void __launch_bounds__(256) loss_rows_kernel(Rows rows, int64_t count, float *__restrict__ loss,
+__global__ void __launch_bounds__(256) loss_rows_kernel(LossRows rows, int64_t count, float *__restrict__ loss,
                                                         float2 *__restrict__ stat) {
   pdl_wait();
   pdl_trigger();
@@ -143,10 +126,10 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(Rows rows, int64_t count
   }
 }
 
-// db (+)= the column sums of G, a block 32 columns.
+// db (+)= the column sums of G, [planes][rows][ld], a block 32 columns; scale[1] (NULL: 1) undoes G's scaling.
 template <typename G, typename TO>
-__global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ g, int64_t rows, int64_t columns, int64_t ld,
-                                                          TO *db, bool accum) {
+__global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ g, int planes, int64_t rows, int64_t columns,
+                                                          int64_t ld, const float *scale, TO *db, bool accum) {
   __shared__ float sums[16][33];
   pdl_wait();
   pdl_trigger();
@@ -154,7 +137,8 @@ __global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ 
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (c < columns)
-    for (int64_t r = warp; r < rows; r += 16)
+#pragma unroll 8
+    for (int64_t r = warp; r < planes * rows; r += 16)
       s += to_f32(g[r * ld + c]);
   sums[warp][lane] = s;
   __syncthreads();
@@ -163,6 +147,8 @@ __global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ 
 #pragma unroll
     for (int w = 0; w < 16; ++w)
       s += sums[w][lane];
+    if (scale)
+      s *= scale[1];
     db[c] = from_f32<TO>(accum ? s + to_f32(db[c]) : s);
   }
 }
@@ -175,14 +161,198 @@ __global__ void __launch_bounds__(256) round_kernel(const float *__restrict__ fr
     to[i] = from_f32<T>(accum ? from[i] + to_f32(to[i]) : from[i]);
 }
 
+// [rows][cols] -> [rows][pitch] of 16-bit values, for rows that a TMA copy cannot read where they lie; eight values a thread.
+__global__ void __launch_bounds__(256) repitch_kernel(const uint16_t *__restrict__ from, uint16_t *__restrict__ to,
+                                                      int64_t rows, int64_t cols, int64_t pitch) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t packs = pitch / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * packs; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / packs, c = (i - r * packs) * 8;
+    Pack<uint16_t, 8> v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v.v[j] = c + j < cols ? from[r * cols + c + j] : (uint16_t)0;
+    *reinterpret_cast<Pack<uint16_t, 8> *>(to + r * pitch + c) = v;
+  }
+}
+
+// scale = {2^e, 2^-e}: |dloss| * 2^e of the rows that count is at most 2^14 and, for the largest, at least 2^13, so that an
+// fp16 G keeps eleven bits down to 2^-28 of the largest gradient.
+__global__ void __launch_bounds__(1024) gradient_scale_kernel(LossRows rows, int64_t count, float *scale) {
+  __shared__ float tops[32];
+  pdl_wait();
+  pdl_trigger();
+  float top = 0.0f;
+  for (int64_t r = threadIdx.x; r < count; r += 1024)
+    if (rows.label_of(r) >= 0)
+      top = fmaxf(top, fabsf(rows.dloss[r]));
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0)
+    tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    top = warp_max(tops[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      int e = top > 0.0f && top < INFINITY ? 13 - ilogbf(top) : 0;
+      e = e < -120 ? -120 : e > 120 ? 120 : e;
+      scale[0] = ldexpf(1.0f, e);
+      scale[1] = ldexpf(1.0f, -e);
+    }
+  }
+}
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// A matrix as an operand of the tensor-core products: as it lies, or (rows that a TMA copy cannot read, fp32) laid out anew
+// in `scratch`, of operand_bytes().
+template <typename T> size_t operand_bytes(const T *p, int64_t rows, int64_t cols) {
+  if (std::is_same<T, float>::value)
+    return (size_t)3 * rows * up(cols, 64) * 2;
+  return cols % 8 == 0 && aligned16(p) ? 0 : (size_t)rows * up(cols, 8) * 2;
+}
+template <typename T> int make_operand(const T *p, int64_t rows, int64_t cols, void *scratch, Operand &o, cudaStream_t st) {
+  o = {scratch, rows, cols, up(cols, std::is_same<T, float>::value ? 64 : 8), rows, 1};
+  if constexpr (std::is_same<T, float>::value) {
+    o.planes = 3;
+    return split_rows_bf16(SplitRows{p, nullptr, scratch, rows, (int)cols, 3}, SplitRows{}, o.pitch, st);
+  } else if (operand_bytes(p, rows, cols) == 0) {
+    o.p = p;
+  } else {
+    const int64_t blocks = (rows * (o.pitch / 8) + 255) / 256;
+    NB_CUDA(launch_dependent(repitch_kernel, dim3((unsigned)std::min<int64_t>(blocks, 64 * sm_count())), dim3(256), 0, st,
+                             reinterpret_cast<const uint16_t *>(p), static_cast<uint16_t *>(scratch), rows, cols, o.pitch));
+  }
+  return NB200_OK;
+}
+Operand columns(Operand o, int64_t c0, int64_t n) {
+  o.p = o.at(c0);
+  o.cols = n;
+  return o;
+}
+
+// Scratch for a call, in parts that begin at 256-byte boundaries.
+struct Parts {
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+};
+
+constexpr int kTileN = 256;
+constexpr int64_t kFewRows = 16;
+
+template <typename T>
+int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *loss, float2 *stat, int64_t rows, int64_t size,
+                   int64_t classes, cudaStream_t st) {
+  r.tiles = (int)(2 * ((classes + kTileN - 1) / kTileN));
+  Parts parts;
+  const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
+  const size_t at_partial = parts.take((size_t)rows * r.tiles * 8), at_target = parts.take((size_t)rows * 4);
+  AsyncScratch scratch(st);
+  NB_TRY(scratch.alloc(parts.bytes));
+  char *base = static_cast<char *>(scratch.p);
+  r.partial = reinterpret_cast<float2 *>(base + at_partial);
+  r.target = reinterpret_cast<float *>(base + at_target);
+  Operand ox, ow;
+  NB_TRY(make_operand(x, rows, size, base + at_x, ox, st));
+  NB_TRY(make_operand(w, size, classes, base + at_w, ow, st));
+  Products prob{};
+  prob.count = 1;
+  prob.bias = bias;
+  prob.rows = r;
+  prob.p[0].M = (int)rows, prob.p[0].N = (int)classes, prob.p[0].kblocks = (int)((size + 63) / 64), prob.p[0].b_mn = 1;
+  NB_TRY((launch_loss_gemm<T, kTileN, Out::kSums>(prob, &ox, &ow, st)));
+  NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, r, rows, loss, stat));
+  return NB200_OK;
+}
+
+template <typename T>
+int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T *dw, T *db, int64_t rows, int64_t size,
+                    int64_t classes, const bool accum[3], cudaStream_t st) {
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  constexpr int kPlanes = kF32 ? 3 : 1;
+  using G = std::conditional_t<kF32, __nv_bfloat16, T>;
+  // A piece's G is 2^26 values, 128 MB in 16 bits: large enough that the tiles of its products end in one round of few
+  // idle SMs, and read from L2 for the most part.
+  int64_t piece = std::max<int64_t>(1024, (int64_t)(1 << 26) / kPlanes / rows);
+  piece = up((classes + (classes + piece - 1) / piece - 1) / ((classes + piece - 1) / piece), kTileN);
+  const bool pieces = piece < classes;
+  Parts parts;
+  const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
+  const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(8);
+  const size_t at_dx = parts.take(pieces && dx && !kF32 ? (size_t)rows * size * 4 : 0);
+  AsyncScratch scratch(st);
+  NB_TRY(scratch.alloc(parts.bytes));
+  char *base = static_cast<char *>(scratch.p);
+  float *dx32 = reinterpret_cast<float *>(base + at_dx);
+  Operand ox, ow;
+  NB_TRY(make_operand(x, rows, size, base + at_x, ox, st));
+  NB_TRY(make_operand(w, size, classes, base + at_w, ow, st));
+  if (std::is_same<T, __half>::value) {
+    float *scale = reinterpret_cast<float *>(base + at_scale);
+    NB_CUDA(launch_dependent(gradient_scale_kernel, dim3(1), dim3(1024), 0, st, r, rows, scale));
+    r.scale = scale;
+  }
+  for (int64_t c0 = 0; c0 < classes; c0 += piece) {
+    const int64_t n = std::min(piece, classes - c0);
+    const Operand og{base + at_g, rows, n, piece, rows, kPlanes}, owc = columns(ow, c0, n);
+    Products prob{};
+    prob.count = 1;
+    prob.bias = bias;
+    prob.class0 = (int)c0;
+    prob.rows = r;
+    Product &l = prob.p[0];
+    l.M = (int)rows, l.N = (int)n, l.kblocks = (int)((size + 63) / 64), l.b_mn = 1;
+    l.out = base + at_g, l.ldo = piece, l.plane = rows * piece;
+    NB_TRY((launch_loss_gemm<T, kTileN, Out::kGrad>(prob, &ox, &owc, st)));
+    Operand a[2], b[2];
+    prob.count = 0;
+    if (dw) {
+      Product &p = prob.p[prob.count];
+      p = Product{};
+      p.M = (int)size, p.N = (int)n, p.kblocks = (int)((rows + 63) / 64), p.a_mn = p.b_mn = 1;
+      p.out = dw + c0, p.ldo = classes, p.accum = accum[1];
+      a[prob.count] = ox, b[prob.count++] = og;
+    }
+    if (dx) {
+      const bool first = c0 == 0, last = c0 + n == classes;
+      Product &p = prob.p[prob.count];
+      p = Product{};
+      p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64);
+      p.ldo = size;
+      if (kF32) {
+        p.out = dx, p.accum = first ? accum[0] : true;
+      } else {
+        p.base = first ? nullptr : dx32;
+        p.out_f32 = !last;
+        p.out = last ? static_cast<void *>(dx) : dx32;
+        p.accum = last && accum[0];
+      }
+      a[prob.count] = og, b[prob.count++] = owc;
+    }
+    if (prob.count)
+      NB_TRY((launch_loss_gemm<T, kTileN, Out::kStore>(prob, a, b, st)));
+    if (db)
+      NB_CUDA(launch_dependent(column_sums_kernel<G, T>, dim3((unsigned)((n + 31) / 32)), dim3(512), 0, st,
+                               reinterpret_cast<const G *>(base + at_g), kPlanes, rows, n, piece, r.scale, db + c0, accum[2]));
+  }
+  return NB200_OK;
+}
+
 template <typename T>
 int forward(const T *x, const T *w, const T *bias, const void *label, int label_bytes, float *loss, float2 *stat,
             int64_t rows, int64_t size, int64_t classes, cudaStream_t st) {
+  LossRows r{};
+  r.label = label, r.label_bytes = label_bytes, r.classes = classes;
+  if (rows > kFewRows)
+    return forward_tensor<T>(x, w, bias, r, loss, stat, rows, size, classes, st);
   const int64_t tiles = (classes + 63) / 64;
+  r.tiles = (int)tiles;
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc((size_t)rows * tiles * 8 + (size_t)rows * 4));
-  Rows r{};
-  r.label = label, r.label_bytes = label_bytes, r.classes = classes, r.tiles = (int)tiles;
   r.partial = static_cast<float2 *>(scratch.p);
   r.target = reinterpret_cast<float *>(r.partial + rows * tiles);
   NB_CUDA(launch_dependent(simt_product_kernel<T, T, T, Out::kSums>, dim3((unsigned)tiles, (unsigned)((rows + 63) / 64)),
@@ -196,13 +366,15 @@ template <typename T>
 int backward(const T *x, const T *w, const T *bias, const void *label, int label_bytes, const float2 *stat,
              const float *dloss, T *dx, T *dw, T *db, int64_t rows, int64_t size, int64_t classes, const bool accum[3],
              cudaStream_t st) {
+  LossRows r{};
+  r.label = label, r.label_bytes = label_bytes, r.classes = classes, r.stat = stat, r.dloss = dloss;
+  if (rows > kFewRows)
+    return backward_tensor<T>(x, w, bias, r, dx, dw, db, rows, size, classes, accum, st);
   const int64_t piece = std::max<int64_t>(64, std::min<int64_t>((classes + 63) / 64 * 64, (16 << 20) / rows / 64 * 64));
   const bool pieces = piece < classes;
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc((size_t)rows * piece * 4 + (pieces && dx ? (size_t)rows * size * 4 : 0)));
   float *g = static_cast<float *>(scratch.p), *dx32 = g + rows * piece;
-  Rows r{};
-  r.label = label, r.label_bytes = label_bytes, r.classes = classes, r.stat = stat, r.dloss = dloss;
   for (int64_t c0 = 0; c0 < classes; c0 += piece) {
     const int64_t n = std::min(piece, classes - c0);
     NB_CUDA(launch_dependent(simt_product_kernel<T, T, T, Out::kGrad>,
@@ -227,7 +399,7 @@ int backward(const T *x, const T *w, const T *bias, const void *label, int label
                                dw + c0, classes, accum[1]));
     if (db)
       NB_CUDA(launch_dependent(column_sums_kernel<float, T>, dim3((unsigned)((n + 31) / 32)), dim3(512), 0, st,
-                               (const float *)g, rows, n, piece, db + c0, accum[2]));
+                               (const float *)g, 1, rows, n, piece, (const float *)nullptr, db + c0, accum[2]));
   }
   if (dx && pieces)
     NB_CUDA(launch_dependent(round_kernel<T>, dim3((unsigned)std::min<int64_t>((rows * size + 255) / 256, 8 * sm_count())),
