@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(LossRows rows, int64_t c
   }
 }
 
-// db (+)= the column sums of G, [planes][rows][ld], a block 32 columns; scale[1] (NULL: 1) undoes G's scaling.
+// db (+)= the column sums of G, [planes][rows][ld], a block 32 columns; scale[2] (scale NULL: 1) undoes G's scaling.
 template <typename G, typename TO>
 __global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ g, int planes, int64_t rows, int64_t columns,
                                                           int64_t ld, const float *scale, TO *db, bool accum) {
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ 
     for (int w = 0; w < 16; ++w)
       s += sums[w][lane];
     if (scale)
-      s *= scale[1];
+      s *= scale[2];
     db[c] = from_f32<TO>(accum ? s + to_f32(db[c]) : s);
   }
 }
@@ -177,9 +177,10 @@ __global__ void __launch_bounds__(256) repitch_kernel(const uint16_t *__restrict
   }
 }
 
-// scale = {2^e, 2^-e}: |dloss| * 2^e of the rows that count is at most 2^14 and, for the largest, at least 2^13, so that an
-// fp16 G keeps eleven bits down to 2^-28 of the largest gradient.
-__global__ void __launch_bounds__(1024) gradient_scale_kernel(LossRows rows, int64_t count, float *scale) {
+// What G is kept relative to: scale = {the largest |dloss| of a row that counts, 2^e, their quotient}. With the largest taken
+// out, the gradient of a mean, the same in every row, is no rounded factor of G: at the label G is -1 + p. e is 14 for an fp16 G,
+// which so has eleven bits down to 2^-28 of the largest gradient, and 0 for the others.
+__global__ void __launch_bounds__(1024) gradient_scale_kernel(LossRows rows, int64_t count, float times, float *scale) {
   __shared__ float tops[32];
   pdl_wait();
   pdl_trigger();
@@ -194,10 +195,11 @@ __global__ void __launch_bounds__(1024) gradient_scale_kernel(LossRows rows, int
   if (threadIdx.x < 32) {
     top = warp_max(tops[threadIdx.x]);
     if (threadIdx.x == 0) {
-      int e = top > 0.0f && top < INFINITY ? 13 - ilogbf(top) : 0;
-      e = e < -120 ? -120 : e > 120 ? 120 : e;
-      scale[0] = ldexpf(1.0f, e);
-      scale[1] = ldexpf(1.0f, -e);
+      // (none, or one that is not finite: G as it is)
+      const bool plain = !(top >= 1.17549435e-38f && top < INFINITY);
+      scale[0] = plain ? 1.0f : top;
+      scale[1] = times;
+      scale[2] = (plain ? 1.0f : top) / times;
     }
   }
 }
@@ -282,7 +284,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   const bool pieces = piece < classes;
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
-  const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(8);
+  const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(12);
   const size_t at_dx = parts.take(pieces && dx && !kF32 ? (size_t)rows * size * 4 : 0);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc(parts.bytes));
@@ -291,11 +293,10 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   Operand ox, ow;
   NB_TRY(make_operand(x, rows, size, base + at_x, ox, st));
   NB_TRY(make_operand(w, size, classes, base + at_w, ow, st));
-  if (std::is_same<T, __half>::value) {
-    float *scale = reinterpret_cast<float *>(base + at_scale);
-    NB_CUDA(launch_dependent(gradient_scale_kernel, dim3(1), dim3(1024), 0, st, r, rows, scale));
-    r.scale = scale;
-  }
+  float *scale = reinterpret_cast<float *>(base + at_scale);
+  NB_CUDA(launch_dependent(gradient_scale_kernel, dim3(1), dim3(1024), 0, st, r, rows,
+                           std::is_same<T, __half>::value ? 16384.0f : 1.0f, scale));
+  r.scale = scale;
   for (int64_t c0 = 0; c0 < classes; c0 += piece) {
     const int64_t n = std::min(piece, classes - c0);
     const Operand og{base + at_g, rows, n, piece, rows, kPlanes}, owc = columns(ow, c0, n);

@@ -28,7 +28,7 @@ struct LossRows {
   int64_t classes;
   const float2 *stat;
   const float *dloss;
-  const float *scale; // fp16: G is kept times scale[0]; scale[1] is its inverse (NULL: 1)
+  const float *scale; // G is kept relative to dloss = scale[0] and times scale[1]; scale[2] = scale[0] / scale[1]
   float2 *partial;    // kSums: [rows][tiles]
   float *target;      // [rows], the label's logit
   int tiles;
@@ -43,7 +43,7 @@ constexpr int kMaxProducts = 2;
 struct Product {
   int M, N, kblocks, m_tiles, n_tiles;
   int a_mn, b_mn; // memory rows run along K
-  // kStore: out [M][ldo] (+)= scale[1] * D (+ base, fp32); kGrad: out is G [planes][M][ldo]
+  // kStore: out [M][ldo] (+)= scale[2] * D (+ base, fp32); kGrad: out is G [planes][M][ldo]
   void *out;
   const float *base;
   int64_t ldo, plane;
@@ -217,14 +217,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             ptx::tc_fence_after_sync();
             const uint32_t st = ptx::smem_u32(smem + stage * kStageBytes);
+            // pieces whose product is below fp32 resolution of the leading one (pa + pb > 2) are skipped; the small ones
+            // come first, while the accumulator is small and its truncation with it
 #pragma unroll
-            for (int pa = 0; pa < PL; ++pa)
+            for (int sum = PL - 1; sum >= 0; --sum)
 #pragma unroll
-              for (int pb = 0; pb < PL; ++pb) {
-                if (pa + pb > 2) // below fp32 resolution of the leading pieces' product
-                  continue;
+              for (int pa = 0; pa <= sum; ++pa) {
                 const uint64_t ad = ptx::smem_desc_k_sw128(st + pa * kABytes) | a_lbo;
-                const uint64_t bd = ptx::smem_desc_k_sw128(st + PL * kABytes + pb * kBBytes) | b_lbo;
+                const uint64_t bd = ptx::smem_desc_k_sw128(st + PL * kABytes + (sum - pa) * kBBytes) | b_lbo;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   ptx::mma_pair_bf16(d, ad + k * a_step, bd + k * b_step, idesc, accumulate);
@@ -253,21 +253,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     float *stg = stage_out + (warp - 2) * (32 * 33);
     int local = 0;
     bool ok = true;
-    float acc[kMyChunks][32];
+    float acc[2 * kMyChunks][16]; // 16 columns at a time: with 32 the sums and a chunk do not fit in 168 registers
     for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
       int m0, n0;
       const Product &p = prob.p[decode(tile, m0, n0)];
       const int row_base = m0 + (int)rank * kTileM + quarter * 32, row = row_base + lane;
       const bool row_ok = row < p.M;
       int64_t label = -1;
-      float top = 0.0f, log2_sum = 0.0f, factor = 0.0f;
-      if constexpr (kOut != Out::kStore) {
+      float top = 0.0f, log2_sum = 0.0f, factor = 0.0f, undo = 1.0f;
+      if constexpr (kOut == Out::kStore) {
+        undo = rows.scale[2];
+      } else {
         if (row_ok) {
           label = rows.label_of(row);
           if constexpr (kOut == Out::kGrad) {
             const float2 s = rows.stat[row];
             top = s.x, log2_sum = s.y * kLog2e;
-            factor = label < 0 ? 0.0f : label >= rows.classes ? NAN : rows.dloss[row] * (rows.scale ? rows.scale[0] : 1.0f);
+            factor = label < 0 ? 0.0f : label >= rows.classes ? NAN : __fdiv_rn(rows.dloss[row], rows.scale[0]) * rows.scale[1];
           }
         }
       }
@@ -284,83 +286,91 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           break;
         }
         ptx::tc_fence_after_sync();
+        const bool last = kc + 1 == chunks;
 #pragma unroll
         for (int ci = 0; ci < kMyChunks; ++ci) {
           const int c0 = 32 * half + 64 * ci, col0 = n0 + c0;
           if (col0 >= p.N)
             break;
-          uint32_t r[32];
-          ptx::tmem_ld_32x32(lanes + (uint32_t)(buf * BN + c0), r);
-          ptx::tmem_ld_wait();
-          if (row_base >= p.M)
-            continue;
-          if (kc + 1 < chunks) {
+          if (kOut != Out::kSums)
+            __syncwarp(); // (the staged chunk before has been read)
+          const int64_t mine = label - prob.class0 - col0; // the label's column in this chunk, if in [0, 32)
+          float b_lane = 0.0f;
+          if constexpr (kOut != Out::kStore)
+            if (prob.bias && last && col0 + lane < p.N)
+              b_lane = to_f32(static_cast<const T *>(prob.bias)[prob.class0 + col0 + lane]);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              acc[ci][j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(acc[ci][j], __uint_as_float(r[j]));
-            continue;
-          }
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = chunks == 1 ? __uint_as_float(r[j]) : __fadd_rn(acc[ci][j], __uint_as_float(r[j]));
-          if constexpr (kOut == Out::kStore) {
-            if (rows.scale) {
-              const float undo = rows.scale[1];
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                v[j] *= undo;
-            }
-          } else {
-            if (prob.bias) {
-              const float b = col0 + lane < p.N ? to_f32(static_cast<const T *>(prob.bias)[prob.class0 + col0 + lane]) : 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                v[j] += __shfl_sync(0xffffffffu, b, j);
-            }
-            const int64_t mine = label - prob.class0 - col0; // the label's column in this chunk, if in [0, 32)
-            if constexpr (kOut == Out::kSums) {
-              if (col0 + 32 > p.N)
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col0 + j >= p.N)
-                    v[j] = -INFINITY;
-              if (row_ok && mine >= 0 && mine < 32) {
-                float l = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  l = j == (int)mine ? v[j] : l;
-                rows.target[row] = l;
-              }
-              float m = t.m;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                m = fmaxf(m, v[j]);
-              const float b = m == -INFINITY ? 0.0f : m;
-              float s = t.s * ex2((t.m - b) * kLog2e);
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                s += ex2((v[j] - b) * kLog2e);
-              t = {m, s};
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[16];
+            float(&sum)[16] = acc[2 * ci + h];
+            ptx::tmem_ld_32x16(lanes + (uint32_t)(buf * BN + c0 + 16 * h), r);
+            ptx::tmem_ld_wait();
+            if (row_base >= p.M)
               continue;
-            } else {
+            if (!last) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                v[j] = ex2(fmaf(v[j] - top, kLog2e, -log2_sum));
-              if (mine >= 0 && mine < 32)
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  v[j] -= j == (int)mine ? 1.0f : 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                v[j] = label < 0 ? 0.0f : v[j] * factor;
+              for (int j = 0; j < 16; ++j)
+                sum[j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
+              continue;
             }
-          }
-          if constexpr (kOut != Out::kSums) {
-            __syncwarp(); // (the chunk before has been read)
+            float v[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              stg[lane * 33 + j] = v[j];
+            for (int j = 0; j < 16; ++j)
+              v[j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
+            if constexpr (kOut == Out::kStore) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                v[j] *= undo;
+            } else {
+              if (prob.bias)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  v[j] += __shfl_sync(0xffffffffu, b_lane, 16 * h + j);
+              const int here = mine >= 16 * h && mine < 16 * h + 16 ? (int)mine - 16 * h : -1;
+              if constexpr (kOut == Out::kSums) {
+                if (col0 + 16 * h + 16 > p.N)
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    if (col0 + 16 * h + j >= p.N)
+                      v[j] = -INFINITY;
+                if (here >= 0) {
+                  float l = 0.0f;
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    l = j == here ? v[j] : l;
+                  rows.target[row] = l;
+                }
+                float m = t.m;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  m = fmaxf(m, v[j]);
+                const float b = m == -INFINITY ? 0.0f : m;
+                float s = t.s * ex2((t.m - b) * kLog2e);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  s += ex2((v[j] - b) * kLog2e);
+                t = {m, s};
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  v[j] = ex2(fmaf(v[j] - top, kLog2e, -log2_sum));
+                if (here >= 0)
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    v[j] -= j == here ? 1.0f : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  v[j] = label < 0 ? 0.0f : v[j] * factor;
+              }
+            }
+            if constexpr (kOut != Out::kSums)
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                stg[lane * 33 + 16 * h + j] = v[j];
+          }
+          if (row_base >= p.M || !last)
+            continue;
+          if constexpr (kOut != Out::kSums) {
             __syncwarp();
             const int rows_here = p.M - row_base < 32 ? p.M - row_base : 32, cols_here = p.N - col0 < 32 ? p.N - col0 : 32;
             if constexpr (kOut == Out::kGrad && kF32) {
@@ -479,9 +489,9 @@ inline int launch_loss_gemm(const Products &in, const Operand *a, const Operand 
     configured[dev & 63] = true;
   }
   Products prob = in;
-  prob.chunk = k_chunk_blocks((PL == 3 ? 6 : 1) * 4);
-  if (prob.chunk <= 0)
-    prob.chunk = 1 << 29;
+  // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
+  // last four steps are the only ones on a large accumulator
+  prob.chunk = PL == 3 ? 1 : 24;
   CUtensorMap ma[2], mb[2];
   int tiles = 0;
   for (int i = 0; i < prob.count; ++i) {
