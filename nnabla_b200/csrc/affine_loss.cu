@@ -153,12 +153,17 @@ __global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ 
   }
 }
 
+// to (+)= the sum of `parts` tensors of n values, in order.
 template <typename T>
-__global__ void __launch_bounds__(256) round_kernel(const float *__restrict__ from, T *to, int64_t n, bool accum) {
+__global__ void __launch_bounds__(256) round_kernel(const float *__restrict__ from, int parts, T *to, int64_t n, bool accum) {
   pdl_wait();
   pdl_trigger();
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    to[i] = from_f32<T>(accum ? from[i] + to_f32(to[i]) : from[i]);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int p = 0; p < parts; ++p)
+      s += from[p * n + i];
+    to[i] = from_f32<T>(accum ? s + to_f32(to[i]) : s);
+  }
 }
 
 // [rows][cols] -> [rows][pitch] of 16-bit values, for rows that a TMA copy cannot read where they lie; eight values a thread.
@@ -214,7 +219,7 @@ template <typename T> size_t operand_bytes(const T *p, int64_t rows, int64_t col
   return cols % 8 == 0 && aligned16(p) ? 0 : (size_t)rows * up(cols, 8) * 2;
 }
 template <typename T> int make_operand(const T *p, int64_t rows, int64_t cols, void *scratch, Operand &o, cudaStream_t st) {
-  o = {scratch, rows, cols, up(cols, std::is_same<T, float>::value ? 64 : 8), rows, 1};
+  o = {scratch, rows, cols, up(cols, std::is_same<T, float>::value ? 64 : 8), 1};
   if constexpr (std::is_same<T, float>::value) {
     o.planes = 3;
     return split_rows_bf16(SplitRows{p, nullptr, scratch, rows, (int)cols, 3}, SplitRows{}, o.pitch, st);
@@ -228,9 +233,25 @@ template <typename T> int make_operand(const T *p, int64_t rows, int64_t cols, v
   return NB200_OK;
 }
 Operand columns(Operand o, int64_t c0, int64_t n) {
-  o.p = o.at(c0);
+  o.p = static_cast<const char *>(o.p) + 2 * c0;
   o.cols = n;
   return o;
+}
+
+// Time of a launch's tiles, in MMA cycles of an SM: rounds of 256 x 256 tiles on pairs of SMs, 512 cycles a K block, or of
+// 128 x 64 ones, 204 (51 an instruction, for its operands' reads; 32 by its products).
+struct TileCount {
+  int64_t M, N, kblocks;
+};
+bool pays_pairs(std::initializer_list<TileCount> products) {
+  int64_t pair_tiles = 0, single_tiles = 0, blocks = 1;
+  for (const TileCount &p : products) {
+    pair_tiles += ((p.M + 255) / 256) * ((p.N + 255) / 256);
+    single_tiles += ((p.M + 127) / 128) * ((p.N + 63) / 64);
+    blocks = std::max(blocks, p.kblocks);
+  }
+  auto rounds = [](int64_t tiles, int64_t units) { return (tiles + units - 1) / units; };
+  return rounds(pair_tiles, sm_count() / 2) * 512 <= rounds(single_tiles, sm_count()) * 204;
 }
 
 // Scratch for a call, in parts that begin at 256-byte boundaries.
@@ -243,13 +264,14 @@ struct Parts {
   }
 };
 
-constexpr int kTileN = 256;
 constexpr int64_t kFewRows = 16;
 
 template <typename T>
 int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *loss, float2 *stat, int64_t rows, int64_t size,
                    int64_t classes, cudaStream_t st) {
-  r.tiles = (int)(2 * ((classes + kTileN - 1) / kTileN));
+  const int kblocks = (int)((size + 63) / 64);
+  const bool pair = pays_pairs({{rows, classes, kblocks}});
+  r.tiles = (int)(2 * ((classes + (pair ? 255 : 63)) / (pair ? 256 : 64)));
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
   const size_t at_partial = parts.take((size_t)rows * r.tiles * 8), at_target = parts.take((size_t)rows * 4);
@@ -265,8 +287,8 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
   prob.count = 1;
   prob.bias = bias;
   prob.rows = r;
-  prob.p[0].M = (int)rows, prob.p[0].N = (int)classes, prob.p[0].kblocks = (int)((size + 63) / 64), prob.p[0].b_mn = 1;
-  NB_TRY((launch_loss_gemm<T, kTileN, Out::kSums>(prob, &ox, &ow, st)));
+  prob.p[0].M = (int)rows, prob.p[0].N = (int)classes, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
+  NB_TRY((pair ? launch_loss_gemm<T, true, Out::kSums> : launch_loss_gemm<T, false, Out::kSums>)(prob, &ox, &ow, st));
   NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, r, rows, loss, stat));
   return NB200_OK;
 }
@@ -280,12 +302,27 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   // A piece's G is 2^26 values, 128 MB in 16 bits: large enough that the tiles of its products end in one round of few
   // idle SMs, and read from L2 for the most part.
   int64_t piece = std::max<int64_t>(1024, (int64_t)(1 << 26) / kPlanes / rows);
-  piece = up((classes + (classes + piece - 1) / piece - 1) / ((classes + piece - 1) / piece), kTileN);
+  const int64_t count = (classes + piece - 1) / piece;
+  piece = up((classes + count - 1) / count, 256);
   const bool pieces = piece < classes;
+  // Few tiles of dx with a long K: its classes in up to 16 parts, each with sums of its own that round_kernel adds up.
+  const int64_t size_blocks = (size + 63) / 64, row_blocks = (rows + 63) / 64, piece_blocks = (std::min(piece, classes) + 63) / 64;
+  const bool pair_grad = pays_pairs({{rows, piece, size_blocks}});
+  const bool pair = pays_pairs({{dw ? size : 0, piece, row_blocks}, {dx ? rows : 0, size, piece_blocks}});
+  int splits = 1;
+  if (dx) {
+    const int64_t tiles = ((rows + (pair ? 255 : 127)) / (pair ? 256 : 128)) * ((size + (pair ? 255 : 63)) / (pair ? 256 : 64));
+    const int64_t units = pair ? sm_count() / 2 : sm_count();
+    while (splits < 16 && tiles * splits * 2 <= units && piece_blocks >= 8 * splits)
+      splits *= 2;
+  }
+  const int split_blocks = (int)((piece_blocks + splits - 1) / splits);
+  splits = (int)((piece_blocks + split_blocks - 1) / split_blocks); // no empty part (a last, smaller piece may leave some)
+  const bool direct = splits == 1 && (!pieces || (kF32 && !accum[0])); // dx without sums of its own
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
   const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(12);
-  const size_t at_dx = parts.take(pieces && dx && !kF32 ? (size_t)rows * size * 4 : 0);
+  const size_t at_dx = parts.take(dx && !direct ? (size_t)splits * rows * size * 4 : 0);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc(parts.bytes));
   char *base = static_cast<char *>(scratch.p);
@@ -299,47 +336,45 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   r.scale = scale;
   for (int64_t c0 = 0; c0 < classes; c0 += piece) {
     const int64_t n = std::min(piece, classes - c0);
-    const Operand og{base + at_g, rows, n, piece, rows, kPlanes}, owc = columns(ow, c0, n);
+    const Operand og{base + at_g, rows, n, piece, kPlanes}, owc = columns(ow, c0, n);
     Products prob{};
     prob.count = 1;
     prob.bias = bias;
     prob.class0 = (int)c0;
     prob.rows = r;
     Product &l = prob.p[0];
-    l.M = (int)rows, l.N = (int)n, l.kblocks = (int)((size + 63) / 64), l.b_mn = 1;
-    l.out = base + at_g, l.ldo = piece, l.plane = rows * piece;
-    NB_TRY((launch_loss_gemm<T, kTileN, Out::kGrad>(prob, &ox, &owc, st)));
+    l.M = (int)rows, l.N = (int)n, l.kblocks = (int)size_blocks, l.b_mn = 1;
+    l.out = base + at_g, l.ldo = piece, l.stride = rows * piece;
+    NB_TRY((pair_grad ? launch_loss_gemm<T, true, Out::kGrad> : launch_loss_gemm<T, false, Out::kGrad>)(prob, &ox, &owc, st));
     Operand a[2], b[2];
     prob.count = 0;
     if (dw) {
       Product &p = prob.p[prob.count];
       p = Product{};
-      p.M = (int)size, p.N = (int)n, p.kblocks = (int)((rows + 63) / 64), p.a_mn = p.b_mn = 1;
+      p.M = (int)size, p.N = (int)n, p.kblocks = (int)row_blocks, p.a_mn = p.b_mn = 1;
       p.out = dw + c0, p.ldo = classes, p.accum = accum[1];
+      p.vec = classes * sizeof(T) % 16 == 0 && aligned16(dw);
       a[prob.count] = ox, b[prob.count++] = og;
     }
     if (dx) {
-      const bool first = c0 == 0, last = c0 + n == classes;
       Product &p = prob.p[prob.count];
       p = Product{};
-      p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64);
-      p.ldo = size;
-      if (kF32) {
-        p.out = dx, p.accum = first ? accum[0] : true;
-      } else {
-        p.base = first ? nullptr : dx32;
-        p.out_f32 = !last;
-        p.out = last ? static_cast<void *>(dx) : dx32;
-        p.accum = last && accum[0];
-      }
+      p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64), p.ldo = size;
+      p.splits = (p.kblocks + split_blocks - 1) / split_blocks, p.split_blocks = split_blocks, p.stride = rows * size;
+      p.out = direct ? static_cast<void *>(dx) : dx32, p.out_f32 = !direct;
+      p.accum = c0 > 0 || (direct && accum[0]);
+      p.vec = size * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
       a[prob.count] = og, b[prob.count++] = owc;
     }
     if (prob.count)
-      NB_TRY((launch_loss_gemm<T, kTileN, Out::kStore>(prob, a, b, st)));
+      NB_TRY((pair ? launch_loss_gemm<T, true, Out::kStore> : launch_loss_gemm<T, false, Out::kStore>)(prob, a, b, st));
     if (db)
       NB_CUDA(launch_dependent(column_sums_kernel<G, T>, dim3((unsigned)((n + 31) / 32)), dim3(512), 0, st,
                                reinterpret_cast<const G *>(base + at_g), kPlanes, rows, n, piece, r.scale, db + c0, accum[2]));
   }
+  if (dx && !direct)
+    NB_CUDA(launch_dependent(round_kernel<T>, dim3((unsigned)std::min<int64_t>((rows * size + 255) / 256, 8 * sm_count())),
+                             dim3(256), 0, st, (const float *)dx32, splits, dx, rows * size, accum[0]));
   return NB200_OK;
 }
 
@@ -404,7 +439,7 @@ int backward(const T *x, const T *w, const T *bias, const void *label, int label
   }
   if (dx && pieces)
     NB_CUDA(launch_dependent(round_kernel<T>, dim3((unsigned)std::min<int64_t>((rows * size + 255) / 256, 8 * sm_count())),
-                             dim3(256), 0, st, (const float *)dx32, dx, rows * size, accum[0]));
+                             dim3(256), 0, st, (const float *)dx32, 1, dx, rows * size, accum[0]));
   return NB200_OK;
 }
 

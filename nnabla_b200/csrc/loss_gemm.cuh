@@ -1,16 +1,18 @@
 // The products of a classifying head on tcgen05: l = x W, dx = G W^T, dW = x^T G, each from the operands as they lie.
 //
-// Clusters of two CTAs make a 256 x BN tile (cta_group::2): each loads its own 128 rows of A and its own BN / 2 columns of B
-// by TMA, the leader issues the MMAs, both drain their 128 accumulator rows. W [inputs, classes] has its classes in
-// neighbouring memory, so in l = x W, and for both operands of dW, the rows of memory run along K: those operands are read as
-// MN-major ones, stored as chunks of 64 rows (K) x 128 bytes (bit 15 / 16 of the instruction descriptor; the leading byte
-// offset leads from one chunk of 64 columns to the next). Nothing is transposed.
+// W [inputs, classes] has its classes in neighbouring memory, so in l = x W, and for both operands of dW, the rows of memory
+// run along K: those operands are read as MN-major ones, stored as chunks of 64 rows (K) x 128 bytes (bit 15 / 16 of the
+// instruction descriptor; the leading byte offset leads from one chunk of 64 columns to the next). Nothing is transposed.
+//
+// Two shapes (kPair): clusters of two CTAs that make 256 x 256 tiles (cta_group::2: each loads its own 128 rows of A and 128
+// columns of B by TMA, the leader issues the MMAs, both drain their 128 accumulator rows), and single CTAs with 128 x 64 tiles
+// for products whose large tiles would leave most SMs idle.
 //
 // PL planes an operand: 1 (bf16 or fp16 as it is) or 3 (the bf16 pieces of an fp32 tensor; the six products that matter at
-// fp32 resolution). The tensor core's additions truncate: every 96 MMA steps the accumulator is added up in fp32 registers
+// fp32 resolution). The tensor core's additions truncate: every few MMA steps the accumulator is added up in fp32 registers
 // (gemm.cuh).
 //
-// What becomes of a tile, by the epilogue:
+// What becomes of a tile, by the epilogue, in which a thread owns a row:
 //   kSums   of each row and half of a tile's column chunks, the maximum and the sum of the exponentials; the label's logit
 //   kGrad   G, in 16 bits (fp32: three bf16 planes)
 //   kStore  the product itself, two products (dx and dW of a piece of the classes) in one launch: with one after the other,
@@ -42,56 +44,80 @@ enum class Out { kSums, kGrad, kStore };
 constexpr int kMaxProducts = 2;
 struct Product {
   int M, N, kblocks, m_tiles, n_tiles;
-  int a_mn, b_mn; // memory rows run along K
-  // kStore: out [M][ldo] (+)= scale[2] * D (+ base, fp32); kGrad: out is G [planes][M][ldo]
+  int splits, split_blocks; // kStore: K in `splits` tiles of split_blocks K blocks, each with a result of its own
+  int a_mn, b_mn;           // memory rows run along K
+  // kStore: out [splits][M][ldo] (+)= scale[2] * D; kGrad: out is G [planes][M][ldo]. stride: between splits or planes
   void *out;
-  const float *base;
-  int64_t ldo, plane;
+  int64_t ldo, stride;
   int out_f32, accum;
+  int vec; // rows of out begin at 16-byte boundaries
 };
 struct Products {
   Product p[kMaxProducts];
   int count;
-  int chunk; // K blocks accumulated in tensor memory
+  int chunk;  // K blocks accumulated in tensor memory
   int class0; // kSums, kGrad: the class of the first column
   const void *bias;
   LossRows rows;
 };
 
-// stages of the operands' ring
-template <int PL, int BN> constexpr int loss_stages() { return PL == 1 ? (BN == 256 ? 6 : 8) : 2; }
-template <int PL, int BN> constexpr size_t loss_smem_bytes() {
-  return (size_t)loss_stages<PL, BN>() * PL * (kTileM + BN / 2) * kRowBytes + kEpilogueStageBytes +
-         (2 * loss_stages<PL, BN>() + 4) * 8 + 16 + 1024;
+template <int PL, bool kPair> struct LossShape {
+  static constexpr int kTileRows = kPair ? 256 : 128, kTileCols = kPair ? 256 : 64; // of a cluster
+  static constexpr int kCtaCols = kPair ? 128 : 64;                                 // columns of B that a CTA loads
+  static constexpr uint32_t kABytes = kTileM * kRowBytes, kBBytes = kCtaCols * kRowBytes;
+  static constexpr uint32_t kStageBytes = PL * (kABytes + kBBytes);
+  static constexpr int kStages = PL == 3 ? 2 : 6;
+  static constexpr int kWarpStage = 32 * 32 * 4; // bytes of an epilogue warp's transpose buffer
+  static constexpr size_t kSmem =
+      (size_t)kStages * kStageBytes + kPairEpilogueWarps * kWarpStage + (2 * kStages + 4) * 8 + 16 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory budget");
+};
+
+__device__ __forceinline__ void add_f32x4(float *p, const float *v) { // (one writer an element and launch: no order to vary)
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+}
+template <typename T> __device__ __forceinline__ void store16(T *p, const float (&v)[16]) {
+  constexpr int V = kPackOf<T>;
+#pragma unroll
+  for (int q = 0; q < 16 / V; ++q) {
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      o[j] = v[q * V + j];
+    store_pack<T, V>(p + q * V, o);
+  }
 }
 
 // T: the operands' type; float means three bf16 planes.
-template <typename T, int BN, Out kOut>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+template <typename T, bool kPair, Out kOut>
+__global__ void __launch_bounds__(kPairThreads, 1)
     loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
                      const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
                      const __grid_constant__ Products prob, int *status) {
   constexpr bool kF32 = std::is_same<T, float>::value;
-  constexpr int PL = kF32 ? 3 : 1, STAGES = loss_stages<PL, BN>();
-  constexpr uint32_t kABytes = kTileM * kRowBytes, kBBytes = (BN / 2) * kRowBytes;
-  constexpr uint32_t kStageBytes = PL * (kABytes + kBBytes);
+  constexpr int PL = kF32 ? 3 : 1;
+  using S = LossShape<PL, kPair>;
+  constexpr int STAGES = S::kStages, BN = S::kTileCols;
+  constexpr uint32_t kABytes = S::kABytes, kBBytes = S::kBBytes, kStageBytes = S::kStageBytes;
   constexpr uint32_t kChunkBytes = 64 * kRowBytes; // 64 columns x 64 of K of an MN-major operand
   constexpr int kMyChunks = BN / 64;               // column chunks of 32 that an epilogue warp drains
   constexpr uint32_t kTmemCols = 2 * BN;
+  constexpr uint32_t kCtas = kPair ? 2 : 1;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float *stage_out = reinterpret_cast<float *>(smem + STAGES * kStageBytes);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * kStageBytes + kEpilogueStageBytes);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * kStageBytes + kPairEpilogueWarps * S::kWarpStage);
   uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tmem_full = bars + 2 * STAGES, *tmem_empty = tmem_full + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_ctarank(); // 0 = leader
-  const int pair_id = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-  const int tiles0 = prob.p[0].m_tiles * prob.p[0].n_tiles;
-  const int num_tiles = tiles0 + (kOut == Out::kStore && prob.count > 1 ? prob.p[1].m_tiles * prob.p[1].n_tiles : 0);
+  const uint32_t rank = kPair ? ptx::cluster_ctarank() : 0; // 0 = leader
+  const int unit = kPair ? blockIdx.x >> 1 : blockIdx.x, units = kPair ? gridDim.x >> 1 : gridDim.x;
+  const int tiles0 = prob.p[0].m_tiles * prob.p[0].n_tiles * prob.p[0].splits;
+  const int num_tiles =
+      tiles0 + (kOut == Out::kStore && prob.count > 1 ? prob.p[1].m_tiles * prob.p[1].n_tiles * prob.p[1].splits : 0);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -100,7 +126,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(tmem_full + b, 1);
-      ptx::mbar_init(tmem_empty + b, 2 * kPairEpilogueWarps);
+      ptx::mbar_init(tmem_empty + b, kCtas * kPairEpilogueWarps);
     }
     *abort_flag = 0;
     ptx::mbar_fence_init();
@@ -108,71 +134,92 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     ptx::prefetch_tensormap(&map_b0);
   }
   if (warp == 1) {
-    ptx::tmem_alloc_pair(tmem_slot, kTmemCols);
-    ptx::tmem_relinquish_pair();
+    if (kPair) {
+      ptx::tmem_alloc_pair(tmem_slot, kTmemCols);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, kTmemCols);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
-  ptx::cluster_sync(); // the peer's barriers are initialised before anything is signalled remotely
+  if (kPair)
+    ptx::cluster_sync(); // the peer's barriers are initialised before anything is signalled remotely
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
+  if (num_tiles <= units) // one round of tiles (early_trigger's reason)
+    pdl_trigger();
 
   auto gave_up = [&](int code) {
     if (*abort_flag == 0)
       atomicCAS(status, 0, code);
     *abort_flag = 1;
   };
-  // the product, first row and first column of a tile; rows vary fastest, so that the tiles in flight share columns of B
-  auto decode = [&](int tile, int &m0, int &n0) -> int {
-    const int which = kOut == Out::kStore && tile >= tiles0 ? 1 : 0;
-    tile -= which ? tiles0 : 0;
-    const int mt = prob.p[which].m_tiles;
-    n0 = tile / mt * BN;
-    m0 = tile % mt * kPairTileM;
-    return which;
+  // A tile's product, first row and column, split and K blocks [kb0, kb1). Rows vary fastest, so that the tiles in flight
+  // share columns of B.
+  struct At {
+    int which, m0, n0, split, kb0, kb1;
+  };
+  auto decode = [&](int tile) {
+    At t;
+    t.which = kOut == Out::kStore && tile >= tiles0 ? 1 : 0;
+    const Product &p = prob.p[t.which];
+    tile -= t.which ? tiles0 : 0;
+    t.m0 = tile % p.m_tiles * S::kTileRows;
+    tile /= p.m_tiles;
+    t.n0 = tile % p.n_tiles * BN;
+    t.split = tile / p.n_tiles;
+    t.kb0 = t.split * p.split_blocks;
+    t.kb1 = t.kb0 + p.split_blocks < p.kblocks ? t.kb0 + p.split_blocks : p.kblocks;
+    return t;
   };
 
   if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer (both CTAs)
+    // ------------------------------------------------------------ TMA producer (every CTA)
     if (ptx::elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t keep = ptx::l2_policy_evict_last();
-      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
-        int m0, n0;
-        const int which = decode(tile, m0, n0);
-        const Product &p = prob.p[which];
-        const CUtensorMap *ma = which ? &map_a1 : &map_a0, *mb = which ? &map_b1 : &map_b0;
-        m0 += (int)rank * kTileM;
-        n0 += (int)rank * (BN / 2);
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+      for (int tile = unit; tile < num_tiles && ok; tile += units) {
+        const At t = decode(tile);
+        const bool a_mn = prob.p[t.which].a_mn != 0, b_mn = prob.p[t.which].b_mn != 0;
+        const CUtensorMap *ma = t.which ? &map_a1 : &map_a0, *mb = t.which ? &map_b1 : &map_b0;
+        const int m0 = t.m0 + (int)rank * kTileM, n0 = t.n0 + (int)rank * S::kCtaCols;
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
           if (!ptx::mbar_wait(empty_bar + stage, phase ^ 1u, abort_flag)) {
             gave_up(kStatusProducerTimeout);
             ok = false;
             break;
           }
           uint8_t *st = smem + stage * kStageBytes;
-          const uint32_t full = ptx::map_to_cta(ptx::smem_u32(full_bar + stage), 0);
+          const uint32_t full = kPair ? ptx::map_to_cta(ptx::smem_u32(full_bar + stage), 0) : 0;
           if (rank == 0)
-            ptx::mbar_expect_tx(full_bar + stage, 2 * kStageBytes); // bytes of both CTAs
+            ptx::mbar_expect_tx(full_bar + stage, kCtas * kStageBytes); // bytes of both CTAs
+          auto load = [&](uint8_t *dst, const CUtensorMap *map, int c0, int c1, int pl) {
+            if constexpr (kPair)
+              ptx::tma_load_3d_pair(dst, map, full, c0, c1, pl, keep);
+            else
+              ptx::tma_load_3d(dst, map, full_bar + stage, c0, c1, pl);
+          };
 #pragma unroll
           for (int pl = 0; pl < PL; ++pl) {
             uint8_t *a = st + pl * kABytes, *b = st + PL * kABytes + pl * kBBytes;
-            if (p.a_mn) {
+            if (a_mn) {
 #pragma unroll
               for (int j = 0; j < kTileM / 64; ++j)
-                ptx::tma_load_3d_pair(a + j * kChunkBytes, ma, full, m0 + 64 * j, kb * 64, pl, keep);
+                load(a + j * kChunkBytes, ma, m0 + 64 * j, kb * 64, pl);
             } else {
-              ptx::tma_load_3d_pair(a, ma, full, kb * 64, m0, pl, keep);
+              load(a, ma, kb * 64, m0, pl);
             }
-            if (p.b_mn) {
+            if (b_mn) {
 #pragma unroll
-              for (int j = 0; j < BN / 128; ++j)
-                ptx::tma_load_3d_pair(b + j * kChunkBytes, mb, full, n0 + 64 * j, kb * 64, pl, keep);
+              for (int j = 0; j < S::kCtaCols / 64; ++j)
+                load(b + j * kChunkBytes, mb, n0 + 64 * j, kb * 64, pl);
             } else {
-              ptx::tma_load_3d_pair(b, mb, full, kb * 64, n0, pl, keep);
+              load(b, mb, kb * 64, n0, pl);
             }
           }
           if (++stage == STAGES) {
@@ -189,16 +236,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
-      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
-        int m0, n0;
-        const Product &p = prob.p[decode(tile, m0, n0)];
-        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0;
-        const uint32_t idesc = ptx::make_idesc(1u, std::is_same<T, __half>::value ? 0u : 1u, kPairTileM, BN) |
+      auto commit = [&](uint64_t *bar) { // on every CTA's barrier, when the MMAs so far have finished
+        if constexpr (kPair) {
+          ptx::mma_commit_pair(ptx::smem_u32(bar));
+          ptx::mma_commit_pair(ptx::map_to_cta(ptx::smem_u32(bar), 1));
+        } else {
+          ptx::mma_commit(bar);
+        }
+      };
+      for (int tile = unit; tile < num_tiles && ok; tile += units) {
+        const At t = decode(tile);
+        const bool a_mn = prob.p[t.which].a_mn != 0, b_mn = prob.p[t.which].b_mn != 0;
+        const uint32_t idesc = ptx::make_idesc(1u, std::is_same<T, __half>::value ? 0u : 1u, S::kTileRows, BN) |
                                (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
         // leading byte offset of an MN-major operand; 16 of K are 16 rows there, 32 bytes of a row otherwise
         const uint64_t a_lbo = a_mn ? (uint64_t)(kChunkBytes >> 4) << 16 : 0, b_lbo = b_mn ? (uint64_t)(kChunkBytes >> 4) << 16 : 0;
         const uint32_t a_step = a_mn ? (16 * kRowBytes) >> 4 : 2, b_step = b_mn ? (16 * kRowBytes) >> 4 : 2;
-        for (int kb0 = 0; kb0 < p.kblocks && ok; kb0 += prob.chunk, ++local) {
+        for (int kb0 = t.kb0; kb0 < t.kb1 && ok; kb0 += prob.chunk, ++local) {
           const int buf = local & 1;
           if (!ptx::mbar_wait(tmem_empty + buf, ((uint32_t)(local >> 1) & 1u) ^ 1u, abort_flag)) {
             gave_up(kStatusMmaTimeout);
@@ -208,7 +262,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           ptx::tc_fence_after_sync();
           const uint32_t d = tmem_base + (uint32_t)(buf * BN);
           uint32_t accumulate = 0;
-          const int kb1 = kb0 + prob.chunk < p.kblocks ? kb0 + prob.chunk : p.kblocks;
+          const int kb1 = kb0 + prob.chunk < t.kb1 ? kb0 + prob.chunk : t.kb1;
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!ptx::mbar_wait(full_bar + stage, phase, abort_flag)) {
               gave_up(kStatusMmaTimeout);
@@ -227,38 +281,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const uint64_t bd = ptx::smem_desc_k_sw128(st + PL * kABytes + (sum - pa) * kBBytes) | b_lbo;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                  ptx::mma_pair_bf16(d, ad + k * a_step, bd + k * b_step, idesc, accumulate);
+                  if constexpr (kPair)
+                    ptx::mma_pair_bf16(d, ad + k * a_step, bd + k * b_step, idesc, accumulate);
+                  else
+                    ptx::mma_bf16(d, ad + k * a_step, bd + k * b_step, idesc, accumulate);
                   accumulate = 1;
                 }
               }
-            ptx::mma_commit_pair(ptx::smem_u32(empty_bar + stage)); // frees the stage in both CTAs
-            ptx::mma_commit_pair(ptx::map_to_cta(ptx::smem_u32(empty_bar + stage), 1));
+            commit(empty_bar + stage); // frees the stage
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
             }
           }
-          if (ok) {
-            ptx::mma_commit_pair(ptx::smem_u32(tmem_full + buf));
-            ptx::mma_commit_pair(ptx::map_to_cta(ptx::smem_u32(tmem_full + buf), 1));
-          }
+          if (ok)
+            commit(tmem_full + buf);
         }
       }
     }
   } else {
-    // ---------------------------------------------------------------- epilogue (both CTAs): a thread a row
+    // ---------------------------------------------------------------- epilogue (every CTA): a thread a row
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const LossRows &rows = prob.rows;
-    float *stg = stage_out + (warp - 2) * (32 * 33);
+    float *stg = stage_out + (warp - 2) * (S::kWarpStage / 4);
     int local = 0;
     bool ok = true;
     float acc[2 * kMyChunks][16]; // 16 columns at a time: with 32 the sums and a chunk do not fit in 168 registers
-    for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
-      int m0, n0;
-      const Product &p = prob.p[decode(tile, m0, n0)];
-      const int row_base = m0 + (int)rank * kTileM + quarter * 32, row = row_base + lane;
-      const bool row_ok = row < p.M;
+    for (int tile = unit; tile < num_tiles && ok; tile += units) {
+      const At at = decode(tile);
+      const Product &p = prob.p[at.which];
+      const int M = p.M, N = p.N, n0 = at.n0;
+      const int row_base = at.m0 + (int)rank * kTileM + quarter * 32, row = row_base + lane;
+      const bool row_ok = row < M;
       int64_t label = -1;
       float top = 0.0f, log2_sum = 0.0f, factor = 0.0f, undo = 1.0f;
       if constexpr (kOut == Out::kStore) {
@@ -273,8 +328,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           }
         }
       }
-      // K in chunks: all but the last go to registers
-      const int chunks = (p.kblocks + prob.chunk - 1) / prob.chunk;
+      // kStore: this thread's row of the result, and whether its 16-byte accesses are aligned
+      const int64_t ldo = p.ldo;
+      const bool vec = p.vec != 0, accum = p.accum != 0, out_f32 = kF32 || p.out_f32 != 0;
+      const int64_t out0 = at.split * p.stride;
+      const int chunks = (at.kb1 - at.kb0 + prob.chunk - 1) / prob.chunk; // all but the last go to registers
       MaxSum t{-INFINITY, 0.0f};
       for (int kc = 0; kc < chunks && ok; ++kc, ++local) {
         const int buf = local & 1;
@@ -290,22 +348,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
         for (int ci = 0; ci < kMyChunks; ++ci) {
           const int c0 = 32 * half + 64 * ci, col0 = n0 + c0;
-          if (col0 >= p.N)
+          if (col0 >= N)
             break;
-          if (kOut != Out::kSums)
-            __syncwarp(); // (the staged chunk before has been read)
-          const int64_t mine = label - prob.class0 - col0; // the label's column in this chunk, if in [0, 32)
+          const int mine = (int)(label - prob.class0 - col0); // the label's column in this chunk, if in [0, 32)
           float b_lane = 0.0f;
           if constexpr (kOut != Out::kStore)
-            if (prob.bias && last && col0 + lane < p.N)
+            if (prob.bias && last && col0 + lane < N)
               b_lane = to_f32(static_cast<const T *>(prob.bias)[prob.class0 + col0 + lane]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            __syncwarp(); // (the staged chunk before has been read, and the load below is the whole warp's)
             uint32_t r[16];
             float(&sum)[16] = acc[2 * ci + h];
             ptx::tmem_ld_32x16(lanes + (uint32_t)(buf * BN + c0 + 16 * h), r);
             ptx::tmem_ld_wait();
-            if (row_base >= p.M)
+            if (row_base >= M)
               continue;
             if (!last) {
 #pragma unroll
@@ -317,21 +374,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j)
               v[j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
+            const int col = col0 + 16 * h;
             if constexpr (kOut == Out::kStore) {
 #pragma unroll
               for (int j = 0; j < 16; ++j)
                 v[j] *= undo;
+              if (!vec) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  stg[lane * 32 + ((16 * h + j) ^ lane)] = v[j];
+              } else if (row_ok && col < N) {
+                const int64_t off = out0 + (int64_t)row * ldo + col;
+                if (out_f32) {
+                  float *out = static_cast<float *>(p.out) + off;
+                  if (col + 16 > N) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                      if (col + j < N)
+                        out[j] = accum ? out[j] + v[j] : v[j];
+                  } else if (accum) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                      add_f32x4(out + j, v + j);
+                  } else {
+                    store16<float>(out, v);
+                  }
+                } else if constexpr (!kF32) {
+                  T *out = static_cast<T *>(p.out) + off;
+                  if (col + 16 > N) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                      if (col + j < N)
+                        out[j] = from_f32<T>(accum ? to_f32(out[j]) + v[j] : v[j]);
+                  } else {
+                    if (accum) {
+                      const Pack<T, 8> o0 = load_pack<T, 8>(out), o1 = load_pack<T, 8>(out + 8);
+#pragma unroll
+                      for (int j = 0; j < 8; ++j)
+                        v[j] += o0.f(j), v[8 + j] += o1.f(j);
+                    }
+                    store16<T>(out, v);
+                  }
+                }
+              }
             } else {
               if (prob.bias)
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                   v[j] += __shfl_sync(0xffffffffu, b_lane, 16 * h + j);
-              const int here = mine >= 16 * h && mine < 16 * h + 16 ? (int)mine - 16 * h : -1;
+              const int here = mine >= 16 * h && mine < 16 * h + 16 ? mine - 16 * h : -1;
               if constexpr (kOut == Out::kSums) {
-                if (col0 + 16 * h + 16 > p.N)
+                if (col + 16 > N)
 #pragma unroll
                   for (int j = 0; j < 16; ++j)
-                    if (col0 + 16 * h + j >= p.N)
+                    if (col + j >= N)
                       v[j] = -INFINITY;
                 if (here >= 0) {
                   float l = 0.0f;
@@ -361,82 +457,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                   v[j] = label < 0 ? 0.0f : v[j] * factor;
+                if (row_ok) { // (G's rows are as wide as whole tiles)
+                  if constexpr (kF32) {
+                    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)row * ldo + col;
+#pragma unroll
+                    for (int pl = 0; pl < 3; ++pl) {
+                      store16<__nv_bfloat16>(out + pl * p.stride, v);
+#pragma unroll
+                      for (int j = 0; j < 16; ++j)
+                        v[j] = __fsub_rn(v[j], __bfloat162float(__float2bfloat16_rn(v[j])));
+                    }
+                  } else {
+                    store16<T>(static_cast<T *>(p.out) + (int64_t)row * ldo + col, v);
+                  }
+                }
               }
             }
-            if constexpr (kOut != Out::kSums)
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                stg[lane * 33 + 16 * h + j] = v[j];
           }
-          if (row_base >= p.M || !last)
-            continue;
-          if constexpr (kOut != Out::kSums) {
+          if constexpr (kOut == Out::kStore) {
+            if (vec || !last || row_base >= M)
+              continue;
+            // rows that begin anywhere: through shared memory, so that a store writes 32 neighbouring columns of a row
             __syncwarp();
-            const int rows_here = p.M - row_base < 32 ? p.M - row_base : 32, cols_here = p.N - col0 < 32 ? p.N - col0 : 32;
-            if constexpr (kOut == Out::kGrad && kF32) {
-              __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)row_base * p.ldo + col0;
-#pragma unroll 4
-              for (int i = 0; i < rows_here; ++i) {
-                float f = stg[i * 33 + lane];
-                if (lane < cols_here)
-#pragma unroll
-                  for (int pl = 0; pl < 3; ++pl) {
-                    const __nv_bfloat16 h = __float2bfloat16_rn(f);
-                    out[pl * p.plane + i * p.ldo + lane] = h;
-                    f = __fsub_rn(f, __bfloat162float(h));
-                  }
-              }
-            } else if (kF32 || p.out_f32) {
-              float *out = static_cast<float *>(p.out) + (int64_t)row_base * p.ldo + col0 + lane;
-              const float *base = p.base ? p.base + (int64_t)row_base * p.ldo + col0 + lane : nullptr;
+            const int rows_here = M - row_base < 32 ? M - row_base : 32;
+            const int64_t off = out0 + (int64_t)row_base * ldo + col0 + lane;
+            if (col0 + lane >= N)
+              continue;
+            auto write = [&](auto *out) {
+              using O = std::remove_pointer_t<decltype(out)>;
+              if (accum) {
 #pragma unroll 8
-              for (int i = 0; i < rows_here; ++i) {
-                if (lane >= cols_here)
-                  continue;
-                float f = stg[i * 33 + lane];
-                if (base)
-                  f += base[i * p.ldo];
-                if (p.accum)
-                  f += out[i * p.ldo];
-                out[i * p.ldo] = f;
-              }
-            } else if constexpr (!kF32) {
-              // two columns a lane, two rows an instruction, where the pairs are aligned
-              T *out = static_cast<T *>(p.out) + (int64_t)row_base * p.ldo + col0;
-              const float *base = p.base ? p.base + (int64_t)row_base * p.ldo + col0 : nullptr;
-              if (cols_here == 32 && (p.ldo & 1) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0) {
-                const int c = 2 * (lane & 15);
-#pragma unroll 8
-                for (int i = lane >> 4; i < rows_here; i += 2) {
-                  float f[2] = {stg[i * 33 + c], stg[i * 33 + c + 1]};
-                  if (base)
-                    f[0] += base[i * p.ldo + c], f[1] += base[i * p.ldo + c + 1];
-                  if (p.accum) {
-                    const Pack<T, 2> old = load_pack<T, 2>(out + i * p.ldo + c);
-                    f[0] += old.f(0), f[1] += old.f(1);
-                  }
-                  store_pack<T, 2>(out + i * p.ldo + c, f);
-                }
+                for (int i = 0; i < rows_here; ++i, out += ldo)
+                  *out = from_f32<O>(to_f32(*out) + stg[i * 32 + (lane ^ i)]);
               } else {
-#pragma unroll 4
-                for (int i = 0; i < rows_here; ++i) {
-                  if (lane >= cols_here)
-                    continue;
-                  float f = stg[i * 33 + lane];
-                  if (base)
-                    f += base[i * p.ldo + lane];
-                  if (p.accum)
-                    f += to_f32(out[i * p.ldo + lane]);
-                  out[i * p.ldo + lane] = from_f32<T>(f);
-                }
+#pragma unroll 8
+                for (int i = 0; i < rows_here; ++i, out += ldo)
+                  *out = from_f32<O>(stg[i * 32 + (lane ^ i)]);
               }
-            }
+            };
+            if (out_f32)
+              write(static_cast<float *>(p.out) + off);
+            else
+              write(static_cast<T *>(p.out) + off);
           }
         }
         ptx::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0)
-          ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(tmem_empty + buf), 0));
+        if (lane == 0) {
+          if (kPair)
+            ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(tmem_empty + buf), 0));
+          else
+            ptx::mbar_arrive(tmem_empty + buf);
+        }
       }
       if constexpr (kOut == Out::kSums)
         if (ok && row_ok)
@@ -453,61 +525,78 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       __nanosleep(1000);
     __syncthreads();
   }
-  ptx::cluster_sync(); // neither CTA leaves while its peer may still signal its barriers
+  if (kPair)
+    ptx::cluster_sync(); // neither CTA leaves while its peer may still signal its barriers
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    if (kPair)
+      ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    else
+      ptx::tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
 // An operand in memory: [planes][rows][pitch] of 16-bit values, 16-byte aligned, pitch a multiple of 8.
 struct Operand {
   const void *p;
-  int64_t rows, cols, pitch, plane_rows;
+  int64_t rows, cols, pitch;
   int planes;
-  const void *at(int64_t col) const { return static_cast<const char *>(p) + 2 * col; }
 };
 inline int loss_operand_map(CUtensorMap *map, const Operand &o, bool mn, int box_rows) {
   const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.planes};
-  const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)(o.pitch * o.plane_rows) * 2};
+  const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)(o.pitch * o.rows) * 2};
   const uint32_t box[3] = {64, mn ? 64u : (uint32_t)box_rows, 1};
   return encode_tiled(map, 0, 3, o.p, dims, strides, box, nullptr, 128);
 }
 
-// The launch of up to two products: operands a[i] (M side) and b[i] (N side).
-template <typename T, int BN, Out kOut>
-inline int launch_loss_gemm(const Products &in, const Operand *a, const Operand *b, cudaStream_t st) {
+template <typename T, bool kPair, Out kOut>
+inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, cudaStream_t st) {
   constexpr int PL = std::is_same<T, float>::value ? 3 : 1;
-  auto kernel = loss_gemm_kernel<T, BN, kOut>;
-  constexpr size_t smem = loss_smem_bytes<PL, BN>();
-  static_assert(smem <= 227 * 1024, "shared memory budget");
+  using S = LossShape<PL, kPair>;
+  auto kernel = loss_gemm_kernel<T, kPair, kOut>;
   static std::atomic<bool> configured[64]{};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
     configured[dev & 63] = true;
   }
-  Products prob = in;
+  CUtensorMap ma[2], mb[2];
+  int64_t tiles = 0;
+  for (int i = 0; i < prob.count; ++i) {
+    Product &p = prob.p[i];
+    p.m_tiles = (p.M + S::kTileRows - 1) / S::kTileRows;
+    p.n_tiles = (p.N + S::kTileCols - 1) / S::kTileCols;
+    if (p.splits <= 1)
+      p.splits = 1, p.split_blocks = p.kblocks;
+    tiles += (int64_t)p.m_tiles * p.n_tiles * p.splits;
+    NB_TRY(loss_operand_map(&ma[i], a[i], p.a_mn, kTileM));
+    NB_TRY(loss_operand_map(&mb[i], b[i], p.b_mn, S::kCtaCols));
+  }
+  NB_CHECK(tiles < (1ll << 31), NB200_EVALUE, "too many rows and classes");
+  if (prob.count == 1)
+    ma[1] = ma[0], mb[1] = mb[0];
   // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
   // last four steps are the only ones on a large accumulator
   prob.chunk = PL == 3 ? 1 : 24;
-  CUtensorMap ma[2], mb[2];
-  int tiles = 0;
-  for (int i = 0; i < prob.count; ++i) {
-    Product &p = prob.p[i];
-    p.m_tiles = (p.M + kPairTileM - 1) / kPairTileM;
-    p.n_tiles = (p.N + BN - 1) / BN;
-    tiles += p.m_tiles * p.n_tiles;
-    NB_TRY(loss_operand_map(&ma[i], a[i], p.a_mn, kTileM));
-    NB_TRY(loss_operand_map(&mb[i], b[i], p.b_mn, BN / 2));
-  }
-  if (prob.count == 1)
-    ma[1] = ma[0], mb[1] = mb[0];
   int *status = nullptr;
   NB_TRY(device_status_word(&status));
-  const int pairs = std::min(sm_count() / 2, tiles);
-  NB_CUDA(launch_dependent(kernel, dim3(2 * pairs), dim3(kPairThreads), smem, st, ma[0], mb[0], ma[1], mb[1], prob, status));
+  constexpr int kCtas = kPair ? 2 : 1;
+  const int units = (int)std::min<int64_t>(sm_count() / kCtas, tiles);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kCtas * units);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  NB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma[0], mb[0], ma[1], mb[1], prob, status));
   return NB200_OK;
 }
 
