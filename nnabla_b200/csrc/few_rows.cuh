@@ -1,0 +1,227 @@
+// The classifying head for up to eight rows: W decides, 2 or 4 bytes for every two to sixteen operations a row, so that the
+// CUDA cores in fp32 keep up with HBM and nothing is laid out first.
+#pragma once
+#include "loss_gemm.cuh"
+
+namespace nb200 {
+
+constexpr int kFewRows = 8;
+constexpr int kFewThreads = 256, kFewK = 1024; // K of x held in shared memory at a time
+
+// l = x W + b for 8 * VEC classes a block: eight lanes side by side along a row of W, four rows of W a warp. Of those sums
+// kSums leaves the maximum and the sum of the exponentials, kGrad G in fp32.
+template <typename T, int R, int VEC, Out kOut>
+__global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__restrict__ x, const T *__restrict__ w,
+                                                                 const T *__restrict__ bias, LossRows rows, int count,
+                                                                 int64_t size, float *__restrict__ g, int64_t ldg) {
+  constexpr int kCols = 8 * VEC, kStep = kFewThreads / 8; // rows of W a pass
+  __shared__ alignas(16) float xs[kFewK * R];
+  __shared__ float sums[kFewThreads / 32][R][kCols];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t classes = rows.classes, c0 = (int64_t)blockIdx.x * kCols, c = c0 + (threadIdx.x & 7) * VEC;
+  const bool here = c < classes; // (VEC divides classes, or is 1)
+  float acc[R][VEC];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      acc[r][j] = 0.0f;
+  for (int64_t k0 = 0; k0 < size; k0 += kFewK) {
+    const int n = (int)(size - k0 < kFewK ? size - k0 : kFewK);
+    if (k0)
+      __syncthreads();
+    for (int i = threadIdx.x; i < R * kFewK; i += kFewThreads) { // neighbouring threads along K
+      const int r = i / kFewK, k = i % kFewK;
+      if (k < n)
+        xs[k * R + r] = r < count ? to_f32(x[r * size + k0 + k]) : 0.0f;
+    }
+    __syncthreads();
+    if (here) {
+      const T *p = w + (k0 + (threadIdx.x >> 3)) * classes + c;
+      auto add = [&](const Pack<T, VEC> &v, int k) {
+        float xv[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          xv[r] = xs[k * R + r];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            acc[r][j] = fmaf(xv[r], v.f(j), acc[r][j]);
+      };
+      int k = threadIdx.x >> 3;
+      for (; k + 7 * kStep < n; k += 8 * kStep) {
+        Pack<T, VEC> v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          v[u] = load_pack_stream<T, VEC>(p + (int64_t)u * kStep * classes);
+        p += 8 * kStep * classes;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          add(v[u], k + u * kStep);
+      }
+      for (; k < n; k += kStep, p += kStep * classes)
+        add(load_pack_stream<T, VEC>(p), k);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float s = acc[r][j];
+      s += __shfl_xor_sync(0xffffffffu, s, 8);
+      s += __shfl_xor_sync(0xffffffffu, s, 16);
+      if (lane < 8)
+        sums[warp][r][lane * VEC + j] = s;
+    }
+  __syncthreads();
+  for (int r = warp; r < count; r += kFewThreads / 32) { // a warp a row
+    const int64_t label = rows.label_of(r);
+    MaxSum t{-INFINITY, 0.0f};
+    for (int i = lane; i < kCols; i += 32) {
+      if (c0 + i >= classes)
+        continue;
+      float l = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kFewThreads / 32; ++u)
+        l += sums[u][r][i];
+      if (bias)
+        l += to_f32(bias[c0 + i]);
+      if constexpr (kOut == Out::kSums) {
+        t = join(t, MaxSum{l, l == -INFINITY ? 0.0f : l != l ? l : 1.0f}, kLog2e);
+        if (c0 + i == label)
+          rows.target[r] = l;
+      } else {
+        const float2 st = rows.stat[r];
+        const float v = ex2(fmaf(l - st.x, kLog2e, -st.y * kLog2e)) - (c0 + i == label ? 1.0f : 0.0f);
+        g[r * ldg + c0 + i] = label < 0 ? 0.0f : label >= classes ? NAN : v * rows.dloss[r];
+      }
+    }
+    if constexpr (kOut == Out::kSums) {
+      t = warp_join(t, kLog2e);
+      if (lane == 0)
+        rows.partial[(int64_t)r * rows.tiles + blockIdx.x] = make_float2(t.m, t.s);
+    }
+  }
+}
+
+// dx = G W^T and dW = x^T G in one pass over W: a block has kFewH rows of W, its threads walk along the classes. A pack of
+// G, [R][VEC] in fp32 from L2, serves all of the block's rows.
+constexpr int kFewH = 4;
+template <typename T, int R, int VEC>
+__global__ void __launch_bounds__(kFewThreads) few_grads_kernel(const T *__restrict__ x, const T *__restrict__ w,
+                                                                const float *__restrict__ g, int64_t ldg, T *dx, T *dw,
+                                                                int count, int64_t size, int64_t classes, bool accum_dx,
+                                                                bool accum_dw, bool keep) {
+  __shared__ float sums[kFewThreads / 32][kFewH * R];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t h0 = (int64_t)blockIdx.x * kFewH;
+  const int hs = (int)(size - h0 < kFewH ? size - h0 : kFewH);
+  float xv[kFewH][R], acc[kFewH][R];
+#pragma unroll
+  for (int h = 0; h < kFewH; ++h)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      xv[h][r] = h < hs && r < count ? to_f32(x[r * size + h0 + h]) : 0.0f;
+      acc[h][r] = 0.0f;
+    }
+  for (int64_t c = (int64_t)threadIdx.x * VEC; c < classes; c += kFewThreads * VEC) {
+    Pack<float, VEC> gv[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r < count)
+        gv[r] = load_pack<float, VEC>(g + r * ldg + c);
+      else
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          gv[r].v[j] = 0.0f;
+    Pack<T, VEC> wv[kFewH];
+    if (dx)
+#pragma unroll
+      for (int h = 0; h < kFewH; ++h)
+        if (h < hs)
+          wv[h] = load_pack_stream<T, VEC>(w + (h0 + h) * classes + c);
+#pragma unroll
+    for (int h = 0; h < kFewH; ++h) {
+      if (h >= hs)
+        continue;
+      if (dx)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            acc[h][r] = fmaf(gv[r].v[j], wv[h].f(j), acc[h][r]);
+      if (dw) {
+        T *to = dw + (h0 + h) * classes + c;
+        float o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          o[j] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            o[j] = fmaf(xv[h][r], gv[r].v[j], o[j]);
+        if (accum_dw) {
+          const Pack<T, VEC> old = load_pack<T, VEC>(to);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            o[j] += old.f(j);
+        }
+        store_pack<T, VEC>(to, o, keep);
+      }
+    }
+  }
+  if (!dx)
+    return;
+#pragma unroll
+  for (int h = 0; h < kFewH; ++h)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float s = warp_sum(acc[h][r]);
+      if (lane == 0)
+        sums[warp][h * R + r] = s;
+    }
+  __syncthreads();
+  if ((int)threadIdx.x < kFewH * R) {
+    const int h = threadIdx.x / R, r = threadIdx.x % R;
+    if (h < hs && r < count) {
+      float s = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kFewThreads / 32; ++u)
+        s += sums[u][threadIdx.x];
+      T *to = dx + r * size + h0 + h;
+      *to = from_f32<T>(accum_dx ? s + to_f32(*to) : s);
+    }
+  }
+}
+
+template <typename T, int R, int VEC>
+int few_logits(const T *x, const T *w, const T *bias, const LossRows &r, int count, int64_t size, float *g, int64_t ldg,
+               cudaStream_t st) {
+  const dim3 grid((unsigned)((r.classes + 8 * VEC - 1) / (8 * VEC)));
+  if (g)
+    NB_CUDA(launch_dependent(few_logits_kernel<T, R, VEC, Out::kGrad>, grid, dim3(kFewThreads), 0, st, x, w, bias, r, count,
+                             size, g, ldg));
+  else
+    NB_CUDA(launch_dependent(few_logits_kernel<T, R, VEC, Out::kSums>, grid, dim3(kFewThreads), 0, st, x, w, bias, r, count,
+                             size, g, ldg));
+  return NB200_OK;
+}
+
+// f(rows rounded up to 1, 2, 4 or 8; values an access) as compile-time constants
+template <typename T, typename F> int few_variant(int64_t rows, bool vec, F f) {
+  auto with_vec = [&](auto r) -> int {
+    return vec ? f(r, std::integral_constant<int, kPackOf<T>>{}) : f(r, std::integral_constant<int, 1>{});
+  };
+  return rows <= 1   ? with_vec(std::integral_constant<int, 1>{})
+         : rows <= 2 ? with_vec(std::integral_constant<int, 2>{})
+         : rows <= 4 ? with_vec(std::integral_constant<int, 4>{})
+                     : with_vec(std::integral_constant<int, 8>{});
+}
+
+} // namespace nb200
