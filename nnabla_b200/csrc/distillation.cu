@@ -57,9 +57,11 @@ template <typename T> struct Run {
   }
 };
 
+constexpr int kSumThreads = 256;
+
 // One row a cluster of blocks (one block where the rows are many). stat: the row's maximum, and log sum exp((x - maximum) / tau).
 template <typename T, typename I>
-__global__ void __launch_bounds__(512) distill_forward_kernel(const T *__restrict__ x, const I *__restrict__ index,
+__global__ void __launch_bounds__(kSumThreads, 4) distill_forward_kernel(const T *__restrict__ x, const I *__restrict__ index,
                                                               const T *__restrict__ teacher, float *__restrict__ loss,
                                                               float2 *__restrict__ stat, int64_t classes, int best,
                                                               float tau, int parts) {
@@ -178,36 +180,31 @@ __global__ void __launch_bounds__(512) distill_forward_kernel(const T *__restric
 
 constexpr int kGradThreads = 256, kGradPacks = 4;
 
-// dx (+)= gradient, a piece of a row a block: kGradThreads * kGradPacks packs of 16 bytes and the values around them. The
-// loads are on their way while warp 0 takes the teacher's sums and lists the entries whose class lies in the piece; those
-// classes are stored a second time, with their correction, by the first of the entries that name them.
+// dx (+)= gradient, a part of a row a block. Warp 0 takes the teacher's sums and lists the entries whose class lies in the
+// part; those classes' gradients are made first, from x as it is before anything is written (dx may be x), and stored last, by
+// the first of the entries that name them. The rest is one stream.
 template <typename T, typename I>
-__global__ void __launch_bounds__(kGradThreads) distill_backward_kernel(
+__global__ void __launch_bounds__(kGradThreads, 4) distill_backward_kernel(
     const T *x, const I *__restrict__ index, const T *__restrict__ teacher, const float2 *__restrict__ stat,
-    const float *__restrict__ dloss, T *dx, int64_t classes, int best, float tau, int pieces, bool accum, bool keep) {
+    const float *__restrict__ dloss, T *dx, int64_t classes, int best, float tau, int parts, bool accum, bool keep) {
   constexpr int V = kPackOf<T>;
-  constexpr int64_t kPiece = (int64_t)kGradThreads * kGradPacks * V;
   __shared__ int at[kMaxEntries];
   __shared__ float share[kMaxEntries];
   __shared__ int entries;
   __shared__ float weight; // 1 where the row has an entry, 0 where it has none, NaN where an entry's class does not exist
   pdl_wait();
   pdl_trigger();
-  const int64_t row = blockIdx.x / pieces;
-  const int piece = blockIdx.x - (int)row * pieces;
+  const int64_t row = blockIdx.x / parts;
+  const int part = blockIdx.x - (int)row * parts;
   const T *xr = x + row * classes;
   T *out = dx + row * classes;
-  // pieces begin at 16-byte boundaries of x but for the row's first
+  // parts begin at 16-byte boundaries of x but for the row's first
   const int64_t lead = (int64_t)(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / sizeof(T));
-  int64_t c0 = piece == 0 ? 0 : lead + piece * kPiece, c1 = lead + (piece + 1) * kPiece;
-  c1 = c1 < classes && piece + 1 < pieces ? c1 : classes;
+  const int64_t each = ((classes + parts - 1) / parts + V - 1) / V * V;
+  int64_t c0 = part == 0 ? 0 : lead + part * each, c1 = lead + (part + 1) * each;
+  c1 = c1 < classes && part + 1 < parts ? c1 : classes;
   c0 = c0 < c1 ? c0 : c1;
   const Run<T> run(xr + c0, c1 - c0);
-  Pack<T, V> p[kGradPacks];
-#pragma unroll
-  for (int u = 0; u < kGradPacks; ++u)
-    if (threadIdx.x + u * kGradThreads < run.packs)
-      p[u] = load_pack_stream<T, V>(run.body + (threadIdx.x + u * kGradThreads) * V);
   const float scale = kLog2e / tau, d = dloss[row] * tau, top = stat[row].x, log2_sum = stat[row].y * kLog2e;
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
@@ -239,42 +236,39 @@ __global__ void __launch_bounds__(kGradThreads) distill_backward_kernel(
     }
   }
   __syncthreads();
+  const int n = entries;
   const float factor = d * weight;
+  const bool dead = weight == 0.0f;
   auto q = [&](float v) { return ex2(fmaf(v - top, scale, -log2_sum)); };
-  auto value = [&](float v) { return weight == 0.0f ? 0.0f : q(v) * factor; };
-  // the corrected classes, read before anything is written: dx may be x
+  auto value = [&](float v) { return dead ? 0.0f : q(v) * factor; };
   float fixed[kMaxEntries / kGradThreads];
-  bool first[kMaxEntries / kGradThreads];
+  unsigned first = 0; // bit u: entry threadIdx.x + u * kGradThreads is the first that names its class
 #pragma unroll
   for (int u = 0; u < kMaxEntries / kGradThreads; ++u) {
     const int i = threadIdx.x + u * kGradThreads;
-    first[u] = i < entries;
-    if (!first[u])
+    if (i >= n)
       continue;
     float sum = 0.0f;
-    for (int j = 0; j < entries; ++j)
+    bool only = true;
+    for (int j = 0; j < n; ++j)
       if (at[j] == at[i]) {
-        first[u] &= j >= i;
+        only &= j >= i;
         sum += share[j];
       }
-    if (first[u]) {
+    if (only) {
+      first |= 1u << u;
       fixed[u] = (q(to_f32(xr[c0 + at[i]])) - sum) * factor;
       if (accum)
         fixed[u] += to_f32(out[c0 + at[i]]);
     }
   }
-  if (entries > 0)
+  if (n > 0)
     __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kGradPacks; ++u) {
-    const int64_t i = threadIdx.x + u * kGradThreads;
-    if (i >= run.packs)
-      continue;
-    T *to = out + (run.body - xr) + i * V;
+  auto store = [&](T *to, const Pack<T, V> &p) {
     float o[V];
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      o[j] = value(p[u].f(j));
+      o[j] = value(p.f(j));
     if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) {
       if (accum) {
         const Pack<T, V> old = load_pack<T, V>(to);
@@ -288,19 +282,32 @@ __global__ void __launch_bounds__(kGradThreads) distill_backward_kernel(
       for (int j = 0; j < V; ++j)
         to[j] = from_f32<T>(accum ? o[j] + to_f32(to[j]) : o[j]);
     }
+  };
+  T *body = out + (run.body - xr);
+  int64_t i = threadIdx.x;
+  for (; i + (kGradPacks - 1) * kGradThreads < run.packs; i += kGradPacks * kGradThreads) {
+    Pack<T, V> p[kGradPacks];
+#pragma unroll
+    for (int u = 0; u < kGradPacks; ++u)
+      p[u] = load_pack_stream<T, V>(run.body + (i + u * kGradThreads) * V);
+#pragma unroll
+    for (int u = 0; u < kGradPacks; ++u)
+      store(body + (i + u * kGradThreads) * V, p[u]);
   }
+  for (; i < run.packs; i += kGradThreads)
+    store(body + i * V, load_pack_stream<T, V>(run.body + i * V));
   if ((int)threadIdx.x < run.heads + run.tails) {
     const T *from = (int)threadIdx.x < run.heads ? run.head + threadIdx.x : run.tail + (threadIdx.x - run.heads);
     T *to = out + (from - xr);
     const float o = value(to_f32(*from));
     *to = from_f32<T>(accum ? o + to_f32(*to) : o);
   }
-  if (entries == 0)
+  if (n == 0)
     return;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kMaxEntries / kGradThreads; ++u)
-    if (first[u])
+    if (first >> u & 1)
       out[c0 + at[threadIdx.x + u * kGradThreads]] = from_f32<T>(fixed[u]);
 }
 
@@ -316,14 +323,12 @@ int check(int64_t rows, int64_t classes, int best, float temperature, int index_
 template <typename T, typename I>
 int forward(const T *x, const I *index, const T *teacher, float *loss, float *stat, int64_t rows, int64_t classes,
             int best, float tau, cudaStream_t st) {
-  // blocks of up to 512 threads with four packs each; few long rows go to clusters
+  // few long rows go to clusters
   const int64_t packs = (classes + kPackOf<T> - 1) / kPackOf<T>;
   int parts = 1;
-  while (parts < 8 && rows * parts < sm_count() && packs >= 1024 * parts)
+  while (parts < 8 && rows * parts < 2 * sm_count() && packs >= 512 * parts)
     parts *= 2;
-  int threads = 128;
-  while (threads < 512 && threads * 4 * parts < packs)
-    threads *= 2;
+  const int threads = packs <= 256 ? 128 : kSumThreads;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * parts));
   cfg.blockDim = dim3(threads);
@@ -343,12 +348,13 @@ int forward(const T *x, const I *index, const T *teacher, float *loss, float *st
 template <typename T, typename I>
 int backward(const T *x, const I *index, const T *teacher, const float *stat, const float *dloss, T *dx, int64_t rows,
              int64_t classes, int best, float tau, bool accum, cudaStream_t st) {
-  constexpr int64_t kPiece = (int64_t)kGradThreads * kGradPacks * kPackOf<T>;
-  const int64_t pieces = (classes + kPiece - 1) / kPiece;
-  NB_CHECK(rows * pieces < (1ll << 31), NB200_EVALUE, "too many rows and classes");
+  // a row a block, or in parts, of one round of its loads at least, until the blocks fill the SMs
+  const int64_t packs = (classes + kPackOf<T> - 1) / kPackOf<T>, most = (packs + kGradThreads * kGradPacks - 1) / (kGradThreads * kGradPacks);
+  const int64_t parts = std::min<int64_t>(most, (8 * sm_count() + rows - 1) / rows);
   const bool keep = (size_t)rows * classes * sizeof(T) <= kKeepBytes;
-  NB_CUDA(launch_dependent(distill_backward_kernel<T, I>, dim3((unsigned)(rows * pieces)), dim3(kGradThreads), 0, st, x,
-                           index, teacher, reinterpret_cast<const float2 *>(stat), dloss, dx, classes, best, tau, (int)pieces, accum, keep));
+  NB_CUDA(launch_dependent(distill_backward_kernel<T, I>, dim3((unsigned)(rows * parts)), dim3(kGradThreads), 0, st, x,
+                           index, teacher, reinterpret_cast<const float2 *>(stat), dloss, dx, classes, best, tau, (int)parts,
+                           accum, keep));
   return NB200_OK;
 }
 

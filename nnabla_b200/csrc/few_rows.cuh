@@ -6,7 +6,15 @@
 namespace nb200 {
 
 constexpr int kFewRows = 8;
-constexpr int kFewThreads = 256, kFewK = 1024; // K of x held in shared memory at a time
+constexpr int kFewThreads = 256, kFewValues = 8192; // of x held in shared memory at a time
+
+constexpr int kFewBatch = 4, kFewBatches = 3;                         // packs a group of copies, groups on the way
+constexpr int kFewRing = kFewBatch * kFewBatches * kFewThreads * 16; // bytes
+
+__device__ __forceinline__ void cp_async16(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to)), "l"(from) : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // l = x W + b for 8 * VEC classes a block: eight lanes side by side along a row of W, four rows of W a warp. Of those sums
 // kSums leaves the maximum and the sum of the exponentials, kGrad G in fp32.
@@ -15,8 +23,12 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
                                                                  const T *__restrict__ bias, LossRows rows, int count,
                                                                  int64_t size, float *__restrict__ g, int64_t ldg) {
   constexpr int kCols = 8 * VEC, kStep = kFewThreads / 8; // rows of W a pass
-  __shared__ alignas(16) float xs[kFewK * R];
-  __shared__ float sums[kFewThreads / 32][R][kCols];
+  constexpr int kFewK = kFewValues / R;
+  constexpr bool kAsync = VEC * sizeof(T) == 16;
+  extern __shared__ __align__(16) uint8_t few_smem[];
+  uint4(*ring)[kFewThreads] = reinterpret_cast<uint4(*)[kFewThreads]>(few_smem); // [kFewBatches * kFewBatch]
+  float *xs = reinterpret_cast<float *>(few_smem + (kAsync ? kFewRing : 0));
+  float(*sums)[R][kCols] = reinterpret_cast<float(*)[R][kCols]>(few_smem); // in the same place, behind the last use of both
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -28,44 +40,67 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
 #pragma unroll
     for (int j = 0; j < VEC; ++j)
       acc[r][j] = 0.0f;
+  // W by asynchronous copies, each thread for itself: kFewBatches groups of kFewBatch packs on the way, whatever the compiler
+  // makes of the registers (with eight ordinary loads a step it kept few in flight: 3.4 TB/s). A thread's rows of W are
+  // (threadIdx.x >> 3) + kStep * i through all pieces of K, kFewK being a multiple of kFewBatch * kStep.
+  static_assert(!kAsync || kFewK % (kFewBatch * kStep) == 0, "a piece of K is whole groups");
+  int64_t next = threadIdx.x >> 3;
+  int fetched = 0, batch = 0;
+  auto fetch = [&]() {
+    if constexpr (kAsync) {
+      const int at = fetched++ % kFewBatches * kFewBatch;
+#pragma unroll
+      for (int u = 0; u < kFewBatch; ++u, next += kStep)
+        if (here && next < size)
+          cp_async16(&ring[at + u][threadIdx.x], w + next * classes + c);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  if constexpr (kAsync)
+    for (int i = 0; i < kFewBatches; ++i)
+      fetch();
   for (int64_t k0 = 0; k0 < size; k0 += kFewK) {
     const int n = (int)(size - k0 < kFewK ? size - k0 : kFewK);
     if (k0)
       __syncthreads();
-    for (int i = threadIdx.x; i < R * kFewK; i += kFewThreads) { // neighbouring threads along K
-      const int r = i / kFewK, k = i % kFewK;
-      if (k < n)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll 4
+      for (int k = threadIdx.x; k < n; k += kFewThreads)
         xs[k * R + r] = r < count ? to_f32(x[r * size + k0 + k]) : 0.0f;
-    }
     __syncthreads();
-    if (here) {
-      const T *p = w + (k0 + (threadIdx.x >> 3)) * classes + c;
-      auto add = [&](const Pack<T, VEC> &v, int k) {
-        float xv[R];
+    if (!here)
+      continue;
+    auto add = [&](const Pack<T, VEC> &v, int k) {
+      float xv[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          xv[r] = xs[k * R + r];
+      for (int r = 0; r < R; ++r)
+        xv[r] = xs[k * R + r];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            acc[r][j] = fmaf(xv[r], v.f(j), acc[r][j]);
-      };
-      int k = threadIdx.x >> 3;
-      for (; k + 7 * kStep < n; k += 8 * kStep) {
-        Pack<T, VEC> v[8];
+        for (int j = 0; j < VEC; ++j)
+          acc[r][j] = fmaf(xv[r], v.f(j), acc[r][j]);
+    };
+    if constexpr (kAsync) {
+      for (int k = threadIdx.x >> 3; k < n; k += kFewBatch * kStep) {
+        const int at = batch % kFewBatches * kFewBatch;
+        cp_async_wait<kFewBatches - 1>();
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          v[u] = load_pack_stream<T, VEC>(p + (int64_t)u * kStep * classes);
-        p += 8 * kStep * classes;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          add(v[u], k + u * kStep);
+        for (int u = 0; u < kFewBatch; ++u)
+          if (k + u * kStep < n)
+            add(*reinterpret_cast<const Pack<T, VEC> *>(&ring[at + u][threadIdx.x]), k + u * kStep);
+        fetch();
+        ++batch;
       }
-      for (; k < n; k += kStep, p += kStep * classes)
-        add(load_pack_stream<T, VEC>(p), k);
+    } else {
+      for (int k = threadIdx.x >> 3; k < n; k += kStep)
+        add(load_pack<T, VEC>(w + (k0 + k) * classes + c), k);
     }
   }
+  if constexpr (kAsync)
+    cp_async_wait<0>();
+  __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -204,12 +239,23 @@ template <typename T, int R, int VEC>
 int few_logits(const T *x, const T *w, const T *bias, const LossRows &r, int count, int64_t size, float *g, int64_t ldg,
                cudaStream_t st) {
   const dim3 grid((unsigned)((r.classes + 8 * VEC - 1) / (8 * VEC)));
+  constexpr int kXs = kFewValues * 4, kSums = kFewThreads / 32 * R * 8 * VEC * 4, kRing = VEC * sizeof(T) == 16 ? kFewRing : 0;
+  constexpr int kMost = kRing + kXs > kSums ? kRing + kXs : kSums;
+  const int smem = std::max(kRing + (int)std::min<int64_t>(kXs, size * R * 4), kSums);
+  static std::atomic<bool> configured[64]{};
+  int dev = 0;
+  NB_CUDA(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    NB_CUDA(cudaFuncSetAttribute(few_logits_kernel<T, R, VEC, Out::kGrad>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    NB_CUDA(cudaFuncSetAttribute(few_logits_kernel<T, R, VEC, Out::kSums>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    configured[dev & 63] = true;
+  }
   if (g)
-    NB_CUDA(launch_dependent(few_logits_kernel<T, R, VEC, Out::kGrad>, grid, dim3(kFewThreads), 0, st, x, w, bias, r, count,
-                             size, g, ldg));
+    NB_CUDA(launch_dependent(few_logits_kernel<T, R, VEC, Out::kGrad>, grid, dim3(kFewThreads), smem, st, x, w, bias, r,
+                             count, size, g, ldg));
   else
-    NB_CUDA(launch_dependent(few_logits_kernel<T, R, VEC, Out::kSums>, grid, dim3(kFewThreads), 0, st, x, w, bias, r, count,
-                             size, g, ldg));
+    NB_CUDA(launch_dependent(few_logits_kernel<T, R, VEC, Out::kSums>, grid, dim3(kFewThreads), smem, st, x, w, bias, r,
+                             count, size, g, ldg));
   return NB200_OK;
 }
 

@@ -16,99 +16,144 @@ namespace {
 
 constexpr int kNormMaxWarps = 32;
 
-// Sums of N values over the threads of a row: a warp's, or (row_warps > 1) the block's. Every thread gets them.
-// `turn` alternates the shared slots, so that one barrier a sum is enough.
+// Sums of N (1 or 2) values over the threads of a row: a warp's, or (row_warps > 1, a multiple of 4) the block's. Every thread
+// gets them. Two values share their shuffles: after the first step each half of the warp goes on with one of them. `turn`
+// alternates the shared slots, so that one barrier a sum is enough.
 template <int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int row_warps, float (*slots)[N][kNormMaxWarps], int &turn) {
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    v[i] = warp_sum(v[i]);
-  if (row_warps == 1)
-    return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float(*s)[kNormMaxWarps] = slots[turn];
-  turn ^= 1;
-  if (lane == 0)
+  if (row_warps == 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      s[i][warp] = v[i];
+      v[i] = warp_sum(v[i]);
+    return;
+  }
+  float s;
+  if constexpr (N == 2) {
+    const bool upper = lane >= 16;
+    s = (upper ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[1], 16);
+  } else {
+    s = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+  }
+#pragma unroll
+  for (int d = 8; d; d >>= 1)
+    s += __shfl_xor_sync(0xffffffffu, s, d);
+  float(*to)[kNormMaxWarps] = slots[turn];
+  turn ^= 1;
+  if (lane == 0)
+    to[0][warp] = s;
+  if (N == 2 && lane == 16)
+    to[N - 1][warp] = s;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    v[i] = warp_sum(lane < row_warps ? s[i][lane] : 0.0f);
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.0f;
+    for (int w = 0; w < row_warps; w += 4) {
+      const float4 f = *reinterpret_cast<const float4 *>(&to[i][w]);
+      v[i] += (f.x + f.y) + (f.z + f.w);
+    }
+  }
 }
 
 // VEC values an access, NV accesses a thread; a row belongs to row_warps warps, and a block holds one row or (row_warps == 1)
-// a row a warp.
-template <typename T, typename P, int VEC, int NV>
+// a row a warp; ROWS such rows at once, for which one barrier serves and one look at the parameters.
+template <typename T, typename P, int VEC, int NV, int ROWS>
 __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ x, const P *__restrict__ beta,
-                                                          const P *__restrict__ gamma, T *__restrict__ y,
-                                                          float *__restrict__ mean_out, float *__restrict__ var_out,
-                                                          int64_t rows, int size, float inv_size, float eps, int row_warps,
-                                                          bool keep) {
-  __shared__ float slots[2][1][kNormMaxWarps];
+                                                          const P *__restrict__ gamma, T *y, float *__restrict__ mean_out,
+                                                          float *__restrict__ var_out, int64_t rows, int size,
+                                                          float inv_size, float eps, int row_warps, bool keep) {
+  __shared__ alignas(16) float slots[2][ROWS][kNormMaxWarps];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
+  const int64_t row = ((row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x)) * ROWS;
   if (row >= rows) // (whole warps, and never where the block shares a row)
     return;
   const int at = (row_warps == 1 ? lane : (int)threadIdx.x) * VEC, step = row_warps * 32 * VEC;
-  const T *xr = x + row * size;
-  Pack<T, VEC> v[NV];
+  const int here = rows - row < ROWS ? (int)(rows - row) : ROWS;
+  float v[ROWS][NV][VEC];
+  {
+    Pack<T, VEC> p[ROWS][NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (at + i * step < size)
-      v[i] = load_pack_stream<T, VEC>(xr + at + i * step);
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (q < here && at + i * step < size)
+          p[q][i] = load_pack_stream<T, VEC>(x + (row + q) * size + at + i * step);
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          v[q][i][j] = q < here && at + i * step < size ? p[q][i].f(j) : 0.0f;
+  }
   int turn = 0;
-  float sum[1] = {0.0f};
+  float mean[ROWS], r[ROWS];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (at + i * step < size)
+  for (int q = 0; q < ROWS; ++q) {
+    mean[q] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        sum[0] += v[i].f(j);
-  row_sums<1>(sum, row_warps, slots, turn);
-  const float mean = sum[0] * inv_size;
-  float sq[1] = {0.0f};
+        mean[q] += v[q][i][j];
+  }
+  row_sums<ROWS>(mean, row_warps, slots, turn);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (at + i * step < size)
+  for (int q = 0; q < ROWS; ++q) {
+    mean[q] *= inv_size;
+    r[q] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float m = at + i * step < size ? mean[q] : 0.0f;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float d = v[i].f(j) - mean;
-        sq[0] = fmaf(d, d, sq[0]);
+        v[q][i][j] -= m;
+        r[q] = fmaf(v[q][i][j], v[q][i][j], r[q]);
       }
-  row_sums<1>(sq, row_warps, slots, turn);
-  const float var = sq[0] * inv_size;
-  const float r = 1.0f / sqrtf(var + eps);
-  if (at == 0) {
-    if (mean_out)
-      mean_out[row] = mean;
-    if (var_out)
-      var_out[row] = var;
+    }
   }
-  T *yr = y + row * size;
+  row_sums<ROWS>(r, row_warps, slots, turn);
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q) {
+    const float var = r[q] * inv_size;
+    r[q] = rsqrtf(var + eps);
+    if (at == 0 && q < here) {
+      if (mean_out)
+        mean_out[row + q] = mean[q];
+      if (var_out)
+        var_out[row + q] = var;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = at + i * step;
     if (c >= size)
       continue;
-    Pack<P, VEC> g, b;
-    if (gamma)
-      g = load_pack<P, VEC>(gamma + c);
-    if (beta)
-      b = load_pack<P, VEC>(beta + c);
-    float o[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      o[j] = (v[i].f(j) - mean) * r;
+    float g[VEC], b[VEC];
+    {
+      Pack<P, VEC> gp, bp;
       if (gamma)
-        o[j] *= g.f(j);
+        gp = load_pack<P, VEC>(gamma + c);
       if (beta)
-        o[j] += b.f(j);
+        bp = load_pack<P, VEC>(beta + c);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        g[j] = gamma ? gp.f(j) : 1.0f;
+        b[j] = beta ? bp.f(j) : 0.0f;
+      }
     }
-    store_pack<T, VEC>(yr + c, o, keep);
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      if (q >= here)
+        continue;
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        o[j] = fmaf(v[q][i][j] * r[q], g[j], b[j]);
+      store_pack<T, VEC>(y + (row + q) * size + c, o, keep);
+    }
   }
 }
 
@@ -145,7 +190,7 @@ __global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThrea
     layer_norm_long_kernel(const T *__restrict__ x, const T *__restrict__ dy, const P *__restrict__ beta,
                            const P *__restrict__ gamma, T *y, float *mean_io, float *var_io, int64_t size, float eps,
                            bool accum) {
-  __shared__ float slots[2][kBackward ? 2 : 1][kNormMaxWarps];
+  __shared__ alignas(16) float slots[2][kBackward ? 2 : 1][kNormMaxWarps];
   __shared__ float shared_sums[2][2];
   pdl_wait();
   pdl_trigger();
@@ -189,7 +234,7 @@ __global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThrea
     });
     row_sums<1>(s, kLongThreads / 32, slots, turn);
     cluster_sums<1>(s, shared_sums[1], kLongBlocks);
-    const float var = (float)(s[0] * inv), r = 1.0f / sqrtf(var + eps);
+    const float var = (float)(s[0] * inv), r = rsqrtf(var + eps);
     if (part == 0 && threadIdx.x == 0) {
       if (mean_io)
         mean_io[row] = mean;
@@ -207,7 +252,7 @@ __global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThrea
     }
   } else {
     const T *dr = dy + row * size;
-    const float mean = mean_io[row], r = 1.0f / sqrtf(var_io[row] + eps);
+    const float mean = mean_io[row], r = rsqrtf(var_io[row] + eps);
     float s[2];
     sum_up(s, [&](int64_t c) {
       const float g = gamma ? to_f32(dr[c]) * to_f32(gamma[c]) : to_f32(dr[c]);
@@ -238,7 +283,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
     const T *__restrict__ x, const T *__restrict__ dy, const P *__restrict__ gamma, const float *__restrict__ mean,
     const float *__restrict__ var, T *dx, float *__restrict__ partial, int64_t rows, int size, float inv_size, float eps,
     int row_warps, bool accum, bool keep) {
-  __shared__ float slots[2][2][kNormMaxWarps];
+  __shared__ alignas(16) float slots[2][2][kNormMaxWarps];
   extern __shared__ float combine[]; // [warps][2][size], where a row is a warp's
   pdl_wait();
   pdl_trigger();
@@ -250,29 +295,43 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i)
     sum_dy[i] = sum_dyu[i] = 0.0f;
-  int turn = 0;
-  for (int64_t row = first; row < rows; row += stride) {
-    const T *xr = x + row * size, *dr = dy + row * size;
-    Pack<T, VEC> xv[NV], dv[NV];
+  Pack<P, VEC> g[NV];
+  if (gamma)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (at + i * step < size)
+        g[i] = load_pack<P, VEC>(gamma + at + i * step);
+  // the next row is on its way while this one is summed up and stored
+  Pack<T, VEC> next_x[NV], next_dy[NV];
+  float next_mean = 0.0f, next_var = 0.0f;
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (at + i * step < size) {
-        xv[i] = load_pack_stream<T, VEC>(xr + at + i * step);
-        dv[i] = load_pack_stream<T, VEC>(dr + at + i * step);
+        next_x[i] = load_pack_stream<T, VEC>(x + row * size + at + i * step);
+        next_dy[i] = load_pack_stream<T, VEC>(dy + row * size + at + i * step);
       }
-    const float mu = mean[row], r = 1.0f / sqrtf(var[row] + eps);
+    next_mean = mean[row], next_var = var[row];
+  };
+  if (first < rows)
+    fetch(first);
+  int turn = 0;
+  for (int64_t row = first; row < rows; row += stride) {
+    Pack<T, VEC> xv[NV], dv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      xv[i] = next_x[i], dv[i] = next_dy[i];
+    const float mu = next_mean, r = rsqrtf(next_var + eps);
+    if (row + stride < rows)
+      fetch(row + stride);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = at + i * step;
-      if (c >= size)
+      if (at + i * step >= size)
         continue;
-      Pack<P, VEC> g;
-      if (gamma)
-        g = load_pack<P, VEC>(gamma + c);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g.f(j) : d;
+        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g[i].f(j) : d;
         s[0] += gd;
         s[1] = fmaf(gd, u, s[1]);
         if (kParams) {
@@ -291,18 +350,16 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
       const int c = at + i * step;
       if (c >= size)
         continue;
-      Pack<P, VEC> g;
-      if (gamma)
-        g = load_pack<P, VEC>(gamma + c);
-      Pack<T, VEC> old;
-      if (accum)
-        old = load_pack<T, VEC>(out + c);
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g.f(j) : d;
-        o[j] = r * (gd - m1 - u * m2);
-        if (accum)
+        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g[i].f(j) : d;
+        o[j] = r * fmaf(-u, m2, gd - m1);
+      }
+      if (accum) {
+        const Pack<T, VEC> old = load_pack<T, VEC>(out + c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
           o[j] += old.f(j);
       }
       store_pack<T, VEC>(out + c, o, keep);
@@ -359,7 +416,7 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const T *__rest
   for (int64_t row = r0; row < r1; ++row) {
     const float d = to_f32(dy[row * size + c]);
     a += d;
-    b = fmaf(d, (to_f32(x[row * size + c]) - mean[row]) * (1.0f / sqrtf(var[row] + eps)), b);
+    b = fmaf(d, (to_f32(x[row * size + c]) - mean[row]) * (rsqrtf(var[row] + eps)), b);
   }
   partial[(int64_t)blockIdx.y * 2 * size + c] = a;
   partial[(int64_t)blockIdx.y * 2 * size + size + c] = b;
@@ -400,20 +457,20 @@ __global__ void __launch_bounds__(512) layer_norm_param_kernel(const float *__re
 }
 
 // Threads of a row and accesses of a thread. Rows of up to four accesses a lane are a warp's (no barrier); longer ones a
-// block's, two accesses a thread where that is enough threads to fill the SMs, one where the rows are fewer than them.
+// block's, with `want` accesses a thread where the rows are enough to fill the SMs and one where they are few.
 struct RowShape {
   int row_warps, nv;
   bool fits;
 };
-RowShape row_shape(int64_t size, int vec, int64_t rows, int max_threads, int max_nv) {
+RowShape row_shape(int64_t size, int vec, int64_t rows, int max_threads, int max_nv, int want) {
   const int64_t packs = (size + vec - 1) / vec;
   if (packs <= 32)
     return {1, 1, true};
   const bool few = rows < 2 * sm_count();
   if (packs <= 128 && !few)
     return {1, packs <= 64 ? 2 : 4, true};
-  int threads = 64;
-  while (threads < max_threads && (int64_t)threads * (few ? 1 : 2) < packs)
+  int threads = 128;
+  while (threads < max_threads && (int64_t)threads * (few ? 1 : want) < packs)
     threads *= 2;
   int nv = 1;
   while (nv < max_nv && (int64_t)threads * nv < packs)
@@ -441,20 +498,30 @@ int forward(const T *x, const P *beta, const P *gamma, T *y, float *mean, float 
   const bool keep = (size_t)rows * size * sizeof(T) <= kKeepBytes;
   auto run = [&](auto vec) -> int {
     constexpr int kVec = decltype(vec)::value;
-    const RowShape s = row_shape(size, kVec, rows, 1024, kVec == 1 ? 32 : 8);
+    const RowShape s = row_shape(size, kVec, rows, 1024, kVec == 1 ? 32 : 8, kVec == 1 ? 8 : 4);
     if (!s.fits || (rows <= sm_count() / kLongBlocks && size >= 32768)) {
       NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, false>, dim3((unsigned)(rows * kLongBlocks)), dim3(kLongThreads),
                                0, st, x, (const T *)nullptr, beta, gamma, y, mean, var, size, eps, false));
       return NB200_OK;
     }
     const int per_block = s.row_warps == 1 ? 4 : 1;
+    // two rows at once where that leaves enough blocks
     return with_count(s.nv, Counts{}, [&](auto nv) -> int {
       constexpr int kNv = decltype(nv)::value;
-      if constexpr (kVec == 1 || kNv <= 8)
-        NB_CUDA(launch_dependent(layer_norm_kernel<T, P, kVec, kNv>, dim3((unsigned)((rows + per_block - 1) / per_block)),
+      auto launch = [&](auto count) -> int {
+        constexpr int kRows = decltype(count)::value;
+        const int64_t blocks = (rows + per_block * kRows - 1) / (per_block * kRows);
+        NB_CUDA(launch_dependent(layer_norm_kernel<T, P, kVec, kNv, kRows>, dim3((unsigned)blocks),
                                  dim3(32 * s.row_warps * per_block), 0, st, x, beta, gamma, y, mean, var, rows, (int)size,
                                  1.0f / (float)size, eps, s.row_warps, keep));
-      return NB200_OK;
+        return NB200_OK;
+      };
+      if constexpr (kVec * kNv <= 16)
+        if (rows / per_block >= 16 * sm_count())
+          return launch(std::integral_constant<int, 2>{});
+      if constexpr (kVec == 1 || kNv <= 8)
+        return launch(std::integral_constant<int, 1>{});
+      return NB200_EVALUE;
     });
   };
   const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(beta);
@@ -469,7 +536,7 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
   int parts = 0;
   auto run = [&](auto vec) -> int {
     constexpr int kVec = decltype(vec)::value;
-    const RowShape s = row_shape(size, kVec, rows, 512, kVec == 1 ? 16 : 4);
+    const RowShape s = row_shape(size, kVec, rows, 512, kVec == 1 ? 16 : 4, kVec == 1 ? 8 : 2);
     if (!s.fits) {
       if (params) {
         const int64_t columns = (size + 255) / 256;
@@ -487,7 +554,7 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
       return NB200_OK;
     }
     const int per_block = s.row_warps == 1 ? 8 : 1, threads = 32 * s.row_warps * per_block;
-    const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, (int64_t)sm_count() * (1024 / threads));
+    const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, (int64_t)sm_count() * std::max(1, 512 / threads));
     if (params) {
       parts = (int)blocks;
       NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));

@@ -878,6 +878,268 @@ PyObject *min_max_quantize_backward(PyObject *, PyObject *const *a, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
+// ---- normalization over features, losses: operands in float32, bfloat16 or float16 ---------------------------------
+int type_code(at::ScalarType t) {
+  return t == at::kFloat ? NB200_F32 : t == at::kBFloat16 ? NB200_BF16 : t == at::kHalf ? NB200_F16 : -1;
+}
+// a contiguous tensor of one of the three types
+const at::Tensor *typed(Plain &p, PyObject *o) {
+  p.require(THPVariable_Check(o));
+  if (!p.ok)
+    return nullptr;
+  const at::ScalarType t = THPVariable_Unpack(o).scalar_type();
+  p.require(type_code(t) >= 0);
+  return p.tensor(o, t);
+}
+const at::Tensor *integers(Plain &p, PyObject *o) {
+  p.require(THPVariable_Check(o));
+  if (!p.ok)
+    return nullptr;
+  const at::ScalarType t = THPVariable_Unpack(o).scalar_type();
+  p.require(t == at::kLong || t == at::kInt);
+  return p.tensor(o, t);
+}
+bool is_integer(PyObject *o, long v) {
+  if (!PyLong_Check(o))
+    return false;
+  const long n = PyLong_AsLong(o);
+  if (n == -1 && PyErr_Occurred())
+    PyErr_Clear();
+  return n == v;
+}
+// (None, None, ...) and (False, False, ...)
+bool all_are(PyObject *o, PyObject *what, Py_ssize_t n) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != n)
+    return false;
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (PyTuple_GET_ITEM(o, i) != what)
+      return false;
+  return true;
+}
+PyObject *gradients(const at::Tensor (&grad)[3]) {
+  PyObject *r = PyTuple_New(3);
+  for (int i = 0; r && i < 3; ++i)
+    PyTuple_SET_ITEM(r, i, grad[i].defined() ? THPVariable_Wrap(grad[i]) : Py_NewRef(Py_None));
+  return r;
+}
+// Whether t is a parameter of x's normalized axes, all but the first.
+bool is_parameter(const at::Tensor &t, const at::Tensor &x, at::ScalarType type) {
+  const at::IntArrayRef s = t.sizes(), xs = x.sizes();
+  return t.scalar_type() == type && (type == x.scalar_type() || type == at::kFloat) &&
+         (s == xs.slice(1) || (s.size() == xs.size() && s[0] == 1 && s.slice(1) == xs.slice(1)));
+}
+
+// layer_normalization(x, beta, gamma, batch_axis, eps, output_stat): functions.layer_normalization
+PyObject *layer_normalization(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6)
+    return PyErr_Format(PyExc_TypeError, "expected 6 arguments, got %zd", nargs);
+  Plain p;
+  const at::Tensor *x = typed(p, a[0]), *beta = a[1] == Py_None ? nullptr : typed(p, a[1]),
+                   *gamma = a[2] == Py_None ? nullptr : typed(p, a[2]);
+  const float eps = p.number(a[4]);
+  const bool stats = p.truth(a[5]);
+  p.require(is_integer(a[3], 0) && p.ok && x->dim() >= 2 && x->numel() > 0);
+  if (!p.ok)
+    return not_plain();
+  const at::ScalarType params = gamma ? gamma->scalar_type() : beta ? beta->scalar_type() : x->scalar_type();
+  for (const at::Tensor *t : {beta, gamma})
+    p.require(!t || is_parameter(*t, *x, params));
+  if (!p.ok)
+    return not_plain();
+  const int64_t rows = x->size(0), size = x->numel() / rows;
+  const at::Tensor y = empty_like_of(*x, x->sizes(), x->scalar_type());
+  at::Tensor mean, var;
+  if (stats) {
+    c10::SmallVector<int64_t, 8> shape(x->dim(), 1);
+    shape[0] = rows;
+    mean = empty_like_of(*x, shape, at::kFloat);
+    var = empty_like_of(*x, shape, at::kFloat);
+  }
+  if (!run_on(*x, [&](void *stream) {
+        return nb200_layer_normalization(x->data_ptr(), beta ? beta->data_ptr() : nullptr, gamma ? gamma->data_ptr() : nullptr,
+                                         y.data_ptr(), stats ? data<float>(&mean) : nullptr, stats ? data<float>(&var) : nullptr,
+                                         rows, size, eps, type_code(x->scalar_type()), type_code(params), stream);
+      }))
+    return nullptr;
+  if (stats)
+    return Py_BuildValue("NNN", THPVariable_Wrap(y), THPVariable_Wrap(mean), THPVariable_Wrap(var));
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_normalization_backward(x, dy, gamma, mean, variance, batch_axis, eps, propagate_down, accum, grads, beta)
+PyObject *layer_normalization_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11)
+    return PyErr_Format(PyExc_TypeError, "expected 11 arguments, got %zd", nargs);
+  Plain p;
+  const at::Tensor *x = typed(p, a[0]), *dy = typed(p, a[1]), *gamma = typed(p, a[2]), *mean = p.f32(a[3]), *var = p.f32(a[4]);
+  const float eps = p.number(a[6]);
+  bool down[3];
+  read_flags(p, a[7], down);
+  p.require(is_integer(a[5], 0) && all_are(a[8], Py_False, 3) && all_are(a[9], Py_None, 3) && a[10] == Py_None && p.ok &&
+            x->dim() >= 2 && x->numel() > 0 && dy->sizes() == x->sizes() && dy->scalar_type() == x->scalar_type() &&
+            mean->numel() == x->size(0) && var->numel() == x->size(0) && is_parameter(*gamma, *x, gamma->scalar_type()));
+  if (!p.ok)
+    return not_plain();
+  const int64_t rows = x->size(0), size = x->numel() / rows;
+  at::Tensor grad[3];
+  for (int i = 0; i < 3; ++i)
+    if (down[i])
+      grad[i] = empty_like_of(*x, i == 0 ? x->sizes() : gamma->sizes(), i == 0 ? x->scalar_type() : gamma->scalar_type());
+  auto at = [&](int i) { return down[i] ? grad[i].data_ptr() : nullptr; };
+  if (!run_on(*x, [&](void *stream) {
+        return nb200_layer_normalization_backward(x->data_ptr(), dy->data_ptr(), gamma->data_ptr(), data<float>(mean),
+                                                  data<float>(var), at(0), at(1), at(2), rows, size, eps,
+                                                  type_code(x->scalar_type()), type_code(gamma->scalar_type()), 0, 0, 0, stream);
+      }))
+    return nullptr;
+  return gradients(grad);
+  END_HANDLE_TH_ERRORS
+}
+
+// Operands of the affine layer's loss, a matrix each: rows, inputs, classes.
+struct Head {
+  const at::Tensor *x, *w, *label, *bias;
+  int64_t rows, size, classes;
+  Head(Plain &p, PyObject *xo, PyObject *wo, PyObject *lo, PyObject *bo, PyObject *base_axis) {
+    x = typed(p, xo), w = typed(p, wo), label = integers(p, lo), bias = bo == Py_None ? nullptr : typed(p, bo);
+    p.require(is_integer(base_axis, 1) && p.ok && x->dim() == 2 && w->dim() == 2 && x->size(1) == w->size(0) &&
+              w->scalar_type() == x->scalar_type() && x->numel() > 0 && w->numel() > 0);
+    if (!p.ok)
+      return;
+    rows = x->size(0), size = x->size(1), classes = w->size(1);
+    p.require(label->size(0) == rows && label->numel() == rows && label->dim() <= 2 &&
+              (!bias || (bias->dim() == 1 && bias->size(0) == classes && bias->scalar_type() == x->scalar_type())));
+  }
+  const void *b() const { return bias ? bias->data_ptr() : nullptr; }
+  int type() const { return type_code(x->scalar_type()); }
+  int label_bytes() const { return (int)label->element_size(); }
+};
+
+// affine_softmax_cross_entropy(x, weight, label, bias, base_axis, output_stat)
+PyObject *affine_softmax_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6)
+    return PyErr_Format(PyExc_TypeError, "expected 6 arguments, got %zd", nargs);
+  Plain p;
+  const Head h(p, a[0], a[1], a[2], a[3], a[4]);
+  const bool stats = p.truth(a[5]);
+  if (!p.ok)
+    return not_plain();
+  const at::Tensor loss = empty_like_of(*h.x, {h.rows, 1}, at::kFloat), stat = empty_like_of(*h.x, {h.rows, 2}, at::kFloat);
+  if (!run_on(*h.x, [&](void *stream) {
+        return nb200_affine_softmax_cross_entropy(h.x->data_ptr(), h.w->data_ptr(), h.b(), h.label->data_ptr(),
+                                                  data<float>(&loss), data<float>(&stat), h.rows, h.size, h.classes, h.type(),
+                                                  h.label_bytes(), stream);
+      }))
+    return nullptr;
+  if (stats)
+    return Py_BuildValue("NN", THPVariable_Wrap(loss), THPVariable_Wrap(stat));
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
+// affine_softmax_cross_entropy_backward(x, weight, label, stat, dloss, bias, base_axis, propagate_down, accum, grads)
+PyObject *affine_softmax_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10)
+    return PyErr_Format(PyExc_TypeError, "expected 10 arguments, got %zd", nargs);
+  Plain p;
+  const Head h(p, a[0], a[1], a[2], a[5], a[6]);
+  const at::Tensor *stat = p.f32(a[3]), *dloss = p.f32(a[4]);
+  bool down[3];
+  read_flags(p, a[7], down);
+  p.require(all_are(a[8], Py_False, 3) && all_are(a[9], Py_None, 3) && p.ok && stat->numel() == 2 * h.rows &&
+            dloss->numel() == h.rows);
+  if (!p.ok)
+    return not_plain();
+  down[2] = down[2] && h.bias;
+  const at::Tensor *like[3] = {h.x, h.w, h.bias};
+  at::Tensor grad[3];
+  for (int i = 0; i < 3; ++i)
+    if (down[i])
+      grad[i] = empty_like_of(*h.x, like[i]->sizes(), h.x->scalar_type());
+  auto at = [&](int i) { return down[i] ? grad[i].data_ptr() : nullptr; };
+  if (!run_on(*h.x, [&](void *stream) {
+        return nb200_affine_softmax_cross_entropy_backward(h.x->data_ptr(), h.w->data_ptr(), h.b(), h.label->data_ptr(),
+                                                           data<float>(stat), data<float>(dloss), at(0), at(1), at(2), h.rows,
+                                                           h.size, h.classes, h.type(), h.label_bytes(), 0, 0, 0, stream);
+      }))
+    return nullptr;
+  return gradients(grad);
+  END_HANDLE_TH_ERRORS
+}
+
+// Operands of the distillation: the student's logits, the teacher's entries.
+struct Distilled {
+  const at::Tensor *x, *index, *teacher;
+  int64_t rows, classes;
+  int best;
+  float temperature;
+  Distilled(Plain &p, PyObject *xo, PyObject *io, PyObject *to, PyObject *temp) {
+    x = typed(p, xo), index = integers(p, io), teacher = typed(p, to);
+    temperature = p.number(temp);
+    p.require(p.ok && temperature > 0.0f && temperature < INFINITY && x->dim() >= 1 && x->numel() > 0 &&
+              index->sizes() == teacher->sizes() && index->dim() == x->dim() && teacher->scalar_type() == x->scalar_type());
+    if (!p.ok)
+      return;
+    classes = x->size(-1), rows = x->numel() / classes, best = (int)std::min<int64_t>(index->size(-1), 1 << 30);
+    p.require(index->sizes().slice(0, x->dim() - 1) == x->sizes().slice(0, x->dim() - 1));
+  }
+  c10::SmallVector<int64_t, 8> shape(int64_t last) const {
+    c10::SmallVector<int64_t, 8> s(x->sizes().begin(), x->sizes().end());
+    s.back() = last;
+    return s;
+  }
+};
+
+// top_k_distillation(x, index, teacher, temperature, output_stat)
+PyObject *top_k_distillation(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5)
+    return PyErr_Format(PyExc_TypeError, "expected 5 arguments, got %zd", nargs);
+  Plain p;
+  const Distilled d(p, a[0], a[1], a[2], a[3]);
+  const bool stats = p.truth(a[4]);
+  if (!p.ok)
+    return not_plain();
+  const at::Tensor loss = empty_like_of(*d.x, d.shape(1), at::kFloat), stat = empty_like_of(*d.x, d.shape(2), at::kFloat);
+  if (!run_on(*d.x, [&](void *stream) {
+        return nb200_top_k_distillation(d.x->data_ptr(), d.index->data_ptr(), d.teacher->data_ptr(), data<float>(&loss),
+                                        data<float>(&stat), d.rows, d.classes, d.best, d.temperature,
+                                        type_code(d.x->scalar_type()), (int)d.index->element_size(), stream);
+      }))
+    return nullptr;
+  if (stats)
+    return Py_BuildValue("NN", THPVariable_Wrap(loss), THPVariable_Wrap(stat));
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
+// top_k_distillation_backward(x, index, teacher, stat, dloss, temperature, accum, dx)
+PyObject *top_k_distillation_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8)
+    return PyErr_Format(PyExc_TypeError, "expected 8 arguments, got %zd", nargs);
+  Plain p;
+  const Distilled d(p, a[0], a[1], a[2], a[5]);
+  const at::Tensor *stat = p.f32(a[3]), *dloss = p.f32(a[4]);
+  p.require(a[6] == Py_False && a[7] == Py_None && p.ok && stat->numel() == 2 * d.rows && dloss->numel() == d.rows);
+  if (!p.ok)
+    return not_plain();
+  const at::Tensor dx = empty_like_of(*d.x, d.x->sizes(), d.x->scalar_type());
+  if (!run_on(*d.x, [&](void *stream) {
+        return nb200_top_k_distillation_backward(d.x->data_ptr(), d.index->data_ptr(), d.teacher->data_ptr(), data<float>(stat),
+                                                 data<float>(dloss), dx.data_ptr(), d.rows, d.classes, d.best, d.temperature,
+                                                 type_code(d.x->scalar_type()), (int)d.index->element_size(), 0, stream);
+      }))
+    return nullptr;
+  return THPVariable_Wrap(dx);
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))Entry<name>::call, METH_FASTCALL, nullptr}
 #define HELPER(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 
@@ -962,6 +1224,12 @@ PyMethodDef methods[] = {
     HELPER("min_max_quantize_backward", min_max_quantize_backward),
     HELPER("batch_normalization_backward", batch_normalization_backward),
     HELPER("codes_nhwc_slots", codes_nhwc_slots),
+    HELPER("layer_normalization", layer_normalization),
+    HELPER("layer_normalization_backward", layer_normalization_backward),
+    HELPER("affine_softmax_cross_entropy", affine_softmax_cross_entropy),
+    HELPER("affine_softmax_cross_entropy_backward", affine_softmax_cross_entropy_backward),
+    HELPER("top_k_distillation", top_k_distillation),
+    HELPER("top_k_distillation_backward", top_k_distillation_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 

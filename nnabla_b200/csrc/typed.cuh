@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace nb200 {
@@ -24,20 +26,37 @@ template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) :
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
   return *reinterpret_cast<const Pack<T, N> *>(p);
 }
-// The same for data that this pass reads once (kStream) and for results: ordinary or streaming.
+// The same for data that this pass reads once. In program order (volatile): a run of them is in flight together, where the
+// compiler would otherwise put each next to its use to save registers.
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack_stream(const T *p) {
   if constexpr (N * sizeof(T) == 16) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
+    uint4 u;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
     return *reinterpret_cast<const Pack<T, N> *>(&u);
   } else {
     return load_pack<T, N>(p);
   }
 }
-template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const float (&v)[N], bool keep = true) {
+// Rounding of neighbouring values, two at a time where the type has it.
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> round_pack(const float (&v)[N]) {
   Pack<T, N> o;
+  if constexpr (N % 2 == 0 && std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    o.v[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < N; i += 2)
+      *reinterpret_cast<__nv_bfloat162 *>(&o.v[i]) = __floats2bfloat162_rn(v[i], v[i + 1]);
+  } else if constexpr (N % 2 == 0 && std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      *reinterpret_cast<__half2 *>(&o.v[i]) = __floats2half2_rn(v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      o.v[i] = from_f32<T>(v[i]);
+  }
+  return o;
+}
+template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const float (&v)[N], bool keep = true) {
+  const Pack<T, N> o = round_pack<T, N>(v);
   if constexpr (N * sizeof(T) == 16)
     st_result(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(&o), keep);
   else

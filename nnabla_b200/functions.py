@@ -1516,6 +1516,10 @@ def layer_normalization(x, beta, gamma, batch_axis=0, eps=1e-05, output_stat=Fal
     with 1 for the batch axes (or without those axes), in x's type or float32, or None. output_stat=True also returns the
     mean and the variance, float32, of x's shape with 1 for the normalized axes: what the backward pass needs.
     outputs: [y], a contiguous tensor like x, which may be x itself."""
+    if outputs is None:
+        fast = L.layer_normalization(x, beta, gamma, batch_axis, eps, output_stat)
+        if fast is not None:
+            return fast
     x, (beta, gamma), dtype, rows, size, lead = _norm_operands(x, ((beta, "beta"), (gamma, "gamma")), batch_axis)
     y = _buffer(None if outputs is None else outputs[0], "outputs[0]", x, False)
     if outputs is not None:
@@ -1536,6 +1540,9 @@ def layer_normalization_backward(x, dy, gamma, mean, variance, batch_axis=0, eps
     gradient arrives at them). Returns (dx, dbeta, dgamma), None where propagate_down is False. dbeta and dgamma have
     gamma's shape and type, or beta's where gamma is None; without both, (1, ..., size) and float32. The sums over the rows
     are added in a fixed order. grads[0] may be dy or x."""
+    fast = L.layer_normalization_backward(x, dy, gamma, mean, variance, batch_axis, eps, propagate_down, accum, grads, beta)
+    if fast is not None:
+        return fast
     x, (gamma, beta), dtype, rows, size, lead = _norm_operands(x, ((gamma, "gamma"), (beta, "beta")), batch_axis)
     dy = _typed(dy, "dy", x, (x.dtype,))
     if dy.shape != x.shape:
@@ -1586,6 +1593,10 @@ def affine_softmax_cross_entropy(x, weight, label, bias=None, base_axis=1, outpu
     a row. A row with a negative label does not count: its loss is 0. A label >= classes makes its row's loss NaN.
     Returns the loss, float32, x.shape[:base_axis] + (1,); with output_stat=True also x.shape[:base_axis] + (2,), float32,
     what the backward pass needs: the row's largest logit, and log sum exp(l - largest)."""
+    if outputs is None:
+        fast = L.affine_softmax_cross_entropy(x, weight, label, bias, base_axis, output_stat)
+        if fast is not None:
+            return fast
     x, weight, label, bias, rows, size, classes, lead = _loss_operands(x, weight, label, bias, base_axis)
     loss = L.empty(lead + (1,), x)
     if outputs is not None:
@@ -1604,6 +1615,10 @@ def affine_softmax_cross_entropy_backward(x, weight, label, stat, dloss, bias=No
     dloss: float32, one value a row. Returns (dx, dweight, dbias) in the operands' type, None where propagate_down is False
     or there is no bias. In float16 the gradient at a logit is kept relative to the largest dloss, so that small ones are
     not lost before the products; scale the loss if the results themselves are too small for the type."""
+    fast = L.affine_softmax_cross_entropy_backward(x, weight, label, stat, dloss, bias, base_axis, propagate_down, accum,
+                                                   grads)
+    if fast is not None:
+        return fast
     x, weight, label, bias, rows, size, classes, _ = _loss_operands(x, weight, label, bias, base_axis)
     stat, dloss = _typed(stat, "stat", x, (torch.float32,)), _typed(dloss, "dloss", x, (torch.float32,))
     if stat.numel() != 2 * rows or dloss.numel() != rows:
@@ -1644,6 +1659,10 @@ def top_k_distillation(x, index, teacher, temperature=1.0, output_stat=False, n_
     K, and one without any has the loss 0 and no gradient. A class that is named twice counts twice; one that does not exist
     makes its row's loss and gradient NaN. Returns the loss (..., 1), float32; with output_stat=True also
     (..., 2), float32, what the backward pass needs: the row's maximum, and log sum exp((x - maximum) / temperature)."""
+    if outputs is None:
+        fast = L.top_k_distillation(x, index, teacher, temperature, output_stat)
+        if fast is not None:
+            return fast
     x, index, teacher, rows, classes, best = _distillation_operands(x, index, teacher, temperature)
     shape = tuple(x.shape[:-1]) + (1,)
     like = L.empty(shape, x)
@@ -1659,6 +1678,9 @@ def top_k_distillation(x, index, teacher, temperature=1.0, output_stat=False, n_
 def top_k_distillation_backward(x, index, teacher, stat, dloss, temperature=1.0, accum=False, dx=None):
     """The gradient of top_k_distillation for x: temperature * (q - p) * dloss. stat: the forward pass's; dloss: float32,
     one value a row. dx receives it, or (accum=True) has it added; it may be x itself."""
+    fast = L.top_k_distillation_backward(x, index, teacher, stat, dloss, temperature, accum, dx)
+    if fast is not None:
+        return fast
     x, index, teacher, rows, classes, best = _distillation_operands(x, index, teacher, temperature)
     stat, dloss = _typed(stat, "stat", x, (torch.float32,)), _typed(dloss, "dloss", x, (torch.float32,))
     if stat.numel() != 2 * rows or dloss.numel() != rows:
