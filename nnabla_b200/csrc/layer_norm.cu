@@ -69,24 +69,29 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
   const int64_t row = ((row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x)) * ROWS;
   if (row >= rows) // (whole warps, and never where the block shares a row)
     return;
-  const int at = (row_warps == 1 ? lane : (int)threadIdx.x) * VEC, step = row_warps * 32 * VEC;
+  // a warp's accesses lie side by side: constant offsets from one address
+  constexpr int step = 32 * VEC;
+  const int at = (row_warps == 1 ? 0 : warp) * (NV * step) + lane * VEC;
   const int here = rows - row < ROWS ? (int)(rows - row) : ROWS;
   float v[ROWS][NV][VEC];
   {
     Pack<T, VEC> p[ROWS][NV];
+    const T *xr = x + row * size + at;
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (q < here && at + i * step < size)
-          p[q][i] = load_pack_stream<T, VEC>(x + (row + q) * size + at + i * step);
+          p[q][i] = load_pack_stream<T, VEC>(xr + (int64_t)q * size + i * step);
+        else
+          p[q][i].clear();
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          v[q][i][j] = q < here && at + i * step < size ? p[q][i].f(j) : 0.0f;
+          v[q][i][j] = p[q][i].f(j);
   }
   int turn = 0;
   float mean[ROWS], r[ROWS];
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
         o[j] = fmaf(v[q][i][j] * r[q], g[j], b[j]);
-      store_pack<T, VEC>(y + (row + q) * size + c, o, keep);
+      store_pack<T, VEC>(y + (row + q) * size + at + i * step, o, keep);
     }
   }
 }
@@ -288,7 +293,8 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int at = (row_warps == 1 ? lane : (int)threadIdx.x) * VEC, step = row_warps * 32 * VEC;
+  constexpr int step = 32 * VEC; // (as in the forward kernel)
+  const int at = (row_warps == 1 ? 0 : warp) * (NV * step) + lane * VEC;
   const int64_t first = row_warps == 1 ? (int64_t)blockIdx.x * warps + warp : (int64_t)blockIdx.x;
   const int64_t stride = row_warps == 1 ? (int64_t)gridDim.x * warps : (int64_t)gridDim.x;
   float sum_dy[NV * VEC], sum_dyu[NV * VEC];
@@ -498,7 +504,8 @@ int forward(const T *x, const P *beta, const P *gamma, T *y, float *mean, float 
   const bool keep = (size_t)rows * size * sizeof(T) <= kKeepBytes;
   auto run = [&](auto vec) -> int {
     constexpr int kVec = decltype(vec)::value;
-    const RowShape s = row_shape(size, kVec, rows, 1024, kVec == 1 ? 32 : 8, kVec == 1 ? 8 : 4);
+    constexpr int kMaxNv = kVec == 1 ? 32 : kVec == 2 ? 16 : 8;
+    const RowShape s = row_shape(size, kVec, rows, 1024, kMaxNv, kVec == 1 ? 8 : 4);
     if (!s.fits || (rows <= sm_count() / kLongBlocks && size >= 32768)) {
       NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, false>, dim3((unsigned)(rows * kLongBlocks)), dim3(kLongThreads),
                                0, st, x, (const T *)nullptr, beta, gamma, y, mean, var, size, eps, false));
@@ -519,13 +526,16 @@ int forward(const T *x, const P *beta, const P *gamma, T *y, float *mean, float 
       if constexpr (kVec * kNv <= 16)
         if (rows / per_block >= 16 * sm_count())
           return launch(std::integral_constant<int, 2>{});
-      if constexpr (kVec == 1 || kNv <= 8)
+      if constexpr (kNv <= kMaxNv)
         return launch(std::integral_constant<int, 1>{});
       return NB200_EVALUE;
     });
   };
   const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(beta);
-  return vec ? run(std::integral_constant<int, kPackOf<T>>{}) : run(std::integral_constant<int, 1>{});
+  const bool pairs = size % 2 == 0 && aligned8(x) && aligned8(y) && aligned8(gamma) && aligned8(beta);
+  return vec     ? run(std::integral_constant<int, kPackOf<T>>{})
+         : pairs ? run(std::integral_constant<int, 2>{})
+                 : run(std::integral_constant<int, 1>{});
 }
 
 template <typename T, typename P>
@@ -536,7 +546,8 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
   int parts = 0;
   auto run = [&](auto vec) -> int {
     constexpr int kVec = decltype(vec)::value;
-    const RowShape s = row_shape(size, kVec, rows, 512, kVec == 1 ? 16 : 4, kVec == 1 ? 8 : 2);
+    constexpr int kMaxNv = kVec == 1 ? 16 : kVec == 2 ? 8 : 4;
+    const RowShape s = row_shape(size, kVec, rows, 512, kMaxNv, kVec == 1 ? 8 : kVec == 2 ? 4 : 2);
     if (!s.fits) {
       if (params) {
         const int64_t columns = (size + 255) / 256;
@@ -562,7 +573,7 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
     const size_t smem = params && s.row_warps == 1 ? (size_t)per_block * 2 * size * 4 : 0;
     return with_count(s.nv, Counts{}, [&](auto nv) -> int {
       constexpr int kNv = decltype(nv)::value;
-      if constexpr (kNv <= (kVec == 1 ? 16 : 4)) {
+      if constexpr (kNv <= kMaxNv) {
         auto kernel = params ? layer_norm_backward_kernel<T, P, kVec, kNv, true>
                              : layer_norm_backward_kernel<T, P, kVec, kNv, false>;
         if (smem > 48 * 1024)
@@ -576,7 +587,10 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
   };
   if (rows > 0) {
     const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gamma);
-    NB_TRY(vec ? run(std::integral_constant<int, kPackOf<T>>{}) : run(std::integral_constant<int, 1>{}));
+    const bool pairs = size % 2 == 0 && aligned8(x) && aligned8(dy) && aligned8(dx) && aligned8(gamma);
+    NB_TRY(vec     ? run(std::integral_constant<int, kPackOf<T>>{})
+           : pairs ? run(std::integral_constant<int, 2>{})
+                   : run(std::integral_constant<int, 1>{}));
   }
   if (params)
     NB_CUDA(launch_dependent(layer_norm_param_kernel<P>, dim3((unsigned)((size + 31) / 32), 2), dim3(512), 0, st,

@@ -21,7 +21,29 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 // N neighbouring values as they lie in memory (16-byte accesses where N values are 16 bytes or a multiple of it)
 template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
   T v[N];
-  __device__ __forceinline__ float f(int i) const { return to_f32(v[i]); }
+  // Value i in fp32. Of 16-bit pairs by words: taken one by one they cost an instruction more each to pick them out.
+  __device__ __forceinline__ float f(int i) const {
+    if constexpr (N % 2 == 0 && std::is_same<T, __nv_bfloat16>::value) {
+      const uint32_t w = reinterpret_cast<const uint32_t *>(v)[i / 2];
+      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    } else if constexpr (N % 2 == 0 && std::is_same<T, __half>::value) {
+      const __half2 h = reinterpret_cast<const __half2 *>(v)[i / 2];
+      return i & 1 ? __high2float(h) : __low2float(h);
+    } else {
+      return to_f32(v[i]);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+    if constexpr (N * sizeof(T) % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < (int)(N * sizeof(T) / 4); ++i)
+        reinterpret_cast<uint32_t *>(v)[i] = 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = from_f32<T>(0.0f);
+    }
+  }
 };
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
   return *reinterpret_cast<const Pack<T, N> *>(p);
@@ -88,6 +110,7 @@ template <typename F> int with_type(int code, F f) {
   return fail(NB200_EVALUE, "unknown type code %d", code);
 }
 inline size_t type_bytes(int code) { return code == NB200_F32 ? 4 : 2; }
+inline bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 } // namespace nb200
