@@ -295,7 +295,7 @@ int forward(const T *x, const T *w, const T *bias, LossRows r, float *loss, floa
   if (rows > kFewRows)
     return forward_tensor<T>(x, w, bias, r, loss, stat, rows, size, r.classes, st);
   const bool vec = r.classes % kPackOf<T> == 0 && aligned16(w);
-  const int64_t columns = 8 * (vec ? kPackOf<T> : 1);
+  const int64_t columns = vec ? few_lanes<T, kPackOf<T>>() * kPackOf<T> : few_lanes<T, 1>();
   r.tiles = (int)((r.classes + columns - 1) / columns);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc((size_t)rows * r.tiles * 8 + (size_t)rows * 4));

@@ -11,20 +11,24 @@ constexpr int kFewThreads = 256, kFewValues = 8192; // of x held in shared memor
 constexpr int kFewBatch = 4, kFewBatches = 3;                         // packs a group of copies, groups on the way
 constexpr int kFewRing = kFewBatch * kFewBatches * kFewThreads * 16; // bytes
 
+template <typename T, int VEC> constexpr int few_lanes() { return VEC * sizeof(T) == 16 ? 4 : 32; }
+
 __device__ __forceinline__ void cp_async16(void *to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to)), "l"(from) : "memory");
 }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// l = x W + b for 8 * VEC classes a block: eight lanes side by side along a row of W, four rows of W a warp. Of those sums
+// l = x W + b for a few classes a block: 64 bytes of a row of W, four lanes, eight rows a warp, so that the blocks are many and
+// their rounds even (with 128 bytes 500 blocks for 32000 classes, 4 on some SMs and 3 on others: 28 us); 32 lanes of one value
+// where rows do not begin at 16-byte boundaries. Of those sums
 // kSums leaves the maximum and the sum of the exponentials, kGrad G in fp32.
 template <typename T, int R, int VEC, Out kOut>
 __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__restrict__ x, const T *__restrict__ w,
                                                                  const T *__restrict__ bias, LossRows rows, int count,
                                                                  int64_t size, float *__restrict__ g, int64_t ldg) {
-  constexpr int kCols = 8 * VEC, kStep = kFewThreads / 8; // rows of W a pass
-  constexpr int kFewK = kFewValues / R;
   constexpr bool kAsync = VEC * sizeof(T) == 16;
+  constexpr int kLanes = few_lanes<T, VEC>(), kCols = kLanes * VEC, kStep = kFewThreads / kLanes; // kStep: rows of W a pass
+  constexpr int kFewK = kFewValues / R;
   extern __shared__ __align__(16) uint8_t few_smem[];
   uint4(*ring)[kFewThreads] = reinterpret_cast<uint4(*)[kFewThreads]>(few_smem); // [kFewBatches * kFewBatch]
   float *xs = reinterpret_cast<float *>(few_smem + (kAsync ? kFewRing : 0));
@@ -32,7 +36,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t classes = rows.classes, c0 = (int64_t)blockIdx.x * kCols, c = c0 + (threadIdx.x & 7) * VEC;
+  const int64_t classes = rows.classes, c0 = (int64_t)blockIdx.x * kCols, c = c0 + (threadIdx.x % kLanes) * VEC;
   const bool here = c < classes; // (VEC divides classes, or is 1)
   float acc[R][VEC];
 #pragma unroll
@@ -42,9 +46,9 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
       acc[r][j] = 0.0f;
   // W by asynchronous copies, each thread for itself: kFewBatches groups of kFewBatch packs on the way, whatever the compiler
   // makes of the registers (with eight ordinary loads a step it kept few in flight: 3.4 TB/s). A thread's rows of W are
-  // (threadIdx.x >> 3) + kStep * i through all pieces of K, kFewK being a multiple of kFewBatch * kStep.
+  // (threadIdx.x / kLanes) + kStep * i through all pieces of K, kFewK being a multiple of kFewBatch * kStep.
   static_assert(!kAsync || kFewK % (kFewBatch * kStep) == 0, "a piece of K is whole groups");
-  int64_t next = threadIdx.x >> 3;
+  int64_t next = threadIdx.x / kLanes;
   int fetched = 0, batch = 0;
   auto fetch = [&]() {
     if constexpr (kAsync) {
@@ -83,7 +87,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
           acc[r][j] = fmaf(xv[r], v.f(j), acc[r][j]);
     };
     if constexpr (kAsync) {
-      for (int k = threadIdx.x >> 3; k < n; k += kFewBatch * kStep) {
+      for (int k = threadIdx.x / kLanes; k < n; k += kFewBatch * kStep) {
         const int at = batch % kFewBatches * kFewBatch;
         cp_async_wait<kFewBatches - 1>();
 #pragma unroll
@@ -94,7 +98,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
         ++batch;
       }
     } else {
-      for (int k = threadIdx.x >> 3; k < n; k += kStep)
+      for (int k = threadIdx.x / kLanes; k < n; k += kStep)
         add(load_pack<T, VEC>(w + (k0 + k) * classes + c), k);
     }
   }
@@ -106,9 +110,10 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       float s = acc[r][j];
-      s += __shfl_xor_sync(0xffffffffu, s, 8);
-      s += __shfl_xor_sync(0xffffffffu, s, 16);
-      if (lane < 8)
+#pragma unroll
+      for (int d = 16; d >= kLanes; d >>= 1)
+        s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (lane < kLanes)
         sums[warp][r][lane * VEC + j] = s;
     }
   __syncthreads();
@@ -238,8 +243,9 @@ __global__ void __launch_bounds__(kFewThreads) few_grads_kernel(const T *__restr
 template <typename T, int R, int VEC>
 int few_logits(const T *x, const T *w, const T *bias, const LossRows &r, int count, int64_t size, float *g, int64_t ldg,
                cudaStream_t st) {
-  const dim3 grid((unsigned)((r.classes + 8 * VEC - 1) / (8 * VEC)));
-  constexpr int kXs = kFewValues * 4, kSums = kFewThreads / 32 * R * 8 * VEC * 4, kRing = VEC * sizeof(T) == 16 ? kFewRing : 0;
+  constexpr int kCols = few_lanes<T, VEC>() * VEC;
+  const dim3 grid((unsigned)((r.classes + kCols - 1) / kCols));
+  constexpr int kXs = kFewValues * 4, kSums = kFewThreads / 32 * R * kCols * 4, kRing = VEC * sizeof(T) == 16 ? kFewRing : 0;
   constexpr int kMost = kRing + kXs > kSums ? kRing + kXs : kSums;
   const int smem = std::max(kRing + (int)std::min<int64_t>(kXs, size * R * 4), kSums);
   static std::atomic<bool> configured[64]{};

@@ -136,19 +136,15 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
     const int c = at + i * step;
     if (c >= size)
       continue;
-    float g[VEC], b[VEC];
-    {
-      Pack<P, VEC> gp, bp;
-      if (gamma)
-        gp = load_pack<P, VEC>(gamma + c);
-      if (beta)
-        bp = load_pack<P, VEC>(beta + c);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        g[j] = gamma ? gp.f(j) : 1.0f;
-        b[j] = beta ? bp.f(j) : 0.0f;
-      }
-    }
+    Pack<P, VEC> g, b; // (none: filled once, not chosen at every value)
+    if (gamma)
+      g = load_pack<P, VEC>(gamma + c);
+    else
+      g.fill(1.0f);
+    if (beta)
+      b = load_pack<P, VEC>(beta + c);
+    else
+      b.clear();
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       if (q >= here)
@@ -156,7 +152,7 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        o[j] = fmaf(v[q][i][j] * r[q], g[j], b[j]);
+        o[j] = fmaf(v[q][i][j] * r[q], g.f(j), b.f(j));
       store_pack<T, VEC>(y + (row + q) * size + at + i * step, o, keep);
     }
   }
@@ -302,20 +298,25 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
   for (int i = 0; i < NV * VEC; ++i)
     sum_dy[i] = sum_dyu[i] = 0.0f;
   Pack<P, VEC> g[NV];
-  if (gamma)
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (at + i * step < size)
-        g[i] = load_pack<P, VEC>(gamma + at + i * step);
+  for (int i = 0; i < NV; ++i)
+    if (gamma && at + i * step < size)
+      g[i] = load_pack<P, VEC>(gamma + at + i * step);
+    else
+      g[i].fill(1.0f);
   // the next row is on its way while this one is summed up and stored
   Pack<T, VEC> next_x[NV], next_dy[NV];
   float next_mean = 0.0f, next_var = 0.0f;
   auto fetch = [&](int64_t row) {
+    const T *xr = x + row * size + at, *dr = dy + row * size + at;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (at + i * step < size) {
-        next_x[i] = load_pack_stream<T, VEC>(x + row * size + at + i * step);
-        next_dy[i] = load_pack_stream<T, VEC>(dy + row * size + at + i * step);
+        next_x[i] = load_pack_stream<T, VEC>(xr + i * step);
+        next_dy[i] = load_pack_stream<T, VEC>(dr + i * step);
+      } else { // (a dy of 0 adds nothing to any sum)
+        next_x[i].clear();
+        next_dy[i].clear();
       }
     next_mean = mean[row], next_var = var[row];
   };
@@ -332,12 +333,10 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
       fetch(row + stride);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (at + i * step >= size)
-        continue;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g[i].f(j) : d;
+        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = d * g[i].f(j);
         s[0] += gd;
         s[1] = fmaf(gd, u, s[1]);
         if (kParams) {
@@ -345,23 +344,21 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
           sum_dyu[i * VEC + j] = fmaf(d, u, sum_dyu[i * VEC + j]);
         }
       }
-    }
     if (!dx)
       continue;
     row_sums<2>(s, row_warps, slots, turn);
-    const float m1 = s[0] * inv_size, m2 = s[1] * inv_size;
-    T *out = dx + row * size;
+    // r (gd - m1 - u m2) as r gd + (a x + b)
+    const float m1 = s[0] * inv_size, a = -r * r * (s[1] * inv_size), b = fmaf(-mu, a, -r * m1);
+    T *out = dx + row * size + at;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = at + i * step;
-      if (c >= size)
+      if (at + i * step >= size)
         continue;
+      const int c = i * step;
       float o[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float u = (xv[i].f(j) - mu) * r, d = dv[i].f(j), gd = gamma ? d * g[i].f(j) : d;
-        o[j] = r * fmaf(-u, m2, gd - m1);
-      }
+      for (int j = 0; j < VEC; ++j)
+        o[j] = fmaf(dv[i].f(j) * g[i].f(j), r, fmaf(xv[i].f(j), a, b));
       if (accum) {
         const Pack<T, VEC> old = load_pack<T, VEC>(out + c);
 #pragma unroll

@@ -33,15 +33,18 @@ template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) :
       return to_f32(v[i]);
     }
   }
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = from_f32<T>(f);
+  }
   __device__ __forceinline__ void clear() {
     if constexpr (N * sizeof(T) % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < (int)(N * sizeof(T) / 4); ++i)
         reinterpret_cast<uint32_t *>(v)[i] = 0u;
     } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[i] = from_f32<T>(0.0f);
+      fill(0.0f);
     }
   }
 };
