@@ -295,7 +295,7 @@ int forward(const T *x, const T *w, const T *bias, LossRows r, float *loss, floa
   if (rows > kFewRows)
     return forward_tensor<T>(x, w, bias, r, loss, stat, rows, size, r.classes, st);
   const bool vec = r.classes % kPackOf<T> == 0 && aligned16(w);
-  const int64_t columns = vec ? few_lanes<T, kPackOf<T>>() * kPackOf<T> : few_lanes<T, 1>();
+  const int64_t columns = vec ? few_lanes<T, kPackOf<T>>() * kPackOf<T> : 32;
   r.tiles = (int)((r.classes + columns - 1) / columns);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc((size_t)rows * r.tiles * 8 + (size_t)rows * 4));
@@ -325,7 +325,7 @@ int backward(const T *x, const T *w, const T *bias, LossRows r, T *dx, T *dw, T 
     const bool keep = (size_t)size * classes * sizeof(T) <= kKeepBytes;
     NB_TRY(few_variant<T>(rows, vec && aligned16(dw), [&](auto n, auto v) -> int {
       NB_CUDA(launch_dependent(few_grads_kernel<T, decltype(n)::value, decltype(v)::value>,
-                               dim3((unsigned)((size + kFewH - 1) / kFewH)), dim3(kFewThreads), 0, st, x, w,
+                               dim3((unsigned)((size + kFewH - 1) / kFewH)), dim3(kFewGradThreads), 0, st, x, w,
                                (const float *)g, ldg, dx, dw, (int)rows, size, classes, accum[0], accum[1], keep));
       return NB200_OK;
     }));

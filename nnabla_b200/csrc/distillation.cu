@@ -329,19 +329,8 @@ int forward(const T *x, const I *index, const T *teacher, float *loss, float *st
   while (parts < 8 && rows * parts < 2 * sm_count() && packs >= 512 * parts)
     parts *= 2;
   const int threads = packs <= 256 ? 128 : kSumThreads;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * parts));
-  cfg.blockDim = dim3(threads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  NB_CUDA(cudaLaunchKernelEx(&cfg, distill_forward_kernel<T, I>, x, index, teacher, loss, reinterpret_cast<float2 *>(stat), classes, best, tau, parts));
+  NB_CUDA(launch_clusters(distill_forward_kernel<T, I>, (unsigned)(rows * parts), parts, threads, 0, st, x, index, teacher, loss,
+                          reinterpret_cast<float2 *>(stat), classes, best, tau, parts));
   return NB200_OK;
 }
 

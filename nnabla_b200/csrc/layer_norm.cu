@@ -425,12 +425,12 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const T *__rest
   partial[(int64_t)blockIdx.y * 2 * size + size + c] = b;
 }
 
-// dbeta (+)= sum over the parts of [part][0][c], dgamma of [part][1][c], in a fixed order: a block takes 32 columns, its 16
+// dbeta (+)= sum over the parts of [part][0][c], dgamma of [part][1][c], in a fixed order: a block takes 32 columns, its 32
 // warps the parts in turn.
 template <typename P>
-__global__ void __launch_bounds__(512) layer_norm_param_kernel(const float *__restrict__ partial, int parts, int64_t size,
+__global__ void __launch_bounds__(1024) layer_norm_param_kernel(const float *__restrict__ partial, int parts, int64_t size,
                                                                P *dbeta, P *dgamma, bool accum_beta, bool accum_gamma) {
-  __shared__ float sums[16][33];
+  __shared__ float sums[32][33];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(512) layer_norm_param_kernel(const float *__re
   if (c < size) {
     const float *p = partial + (int64_t)blockIdx.y * size + c;
 #pragma unroll 8
-    for (int k = warp; k < parts; k += 16)
+    for (int k = warp; k < parts; k += 32)
       s += p[(int64_t)k * 2 * size];
   }
   sums[warp][lane] = s;
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(512) layer_norm_param_kernel(const float *__re
   if (warp == 0 && c < size) {
     s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w)
+    for (int w = 0; w < 32; ++w)
       s += sums[w][lane];
     if (accum)
       s += to_f32(out[c]);
@@ -521,7 +521,7 @@ int forward(const T *x, const P *beta, const P *gamma, T *y, float *mean, float 
         return NB200_OK;
       };
       if constexpr (kVec * kNv <= 16)
-        if (rows / per_block >= 16 * sm_count())
+        if (rows / per_block >= 64 * sm_count())
           return launch(std::integral_constant<int, 2>{});
       if constexpr (kNv <= kMaxNv)
         return launch(std::integral_constant<int, 1>{});
@@ -562,7 +562,9 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
       return NB200_OK;
     }
     const int per_block = s.row_warps == 1 ? 8 : 1, threads = 32 * s.row_warps * per_block;
-    const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, (int64_t)sm_count() * std::max(1, 512 / threads));
+    // as many blocks as are resident, and then no more than their rounds need: each leaves partial sums
+    const int64_t groups = (rows + per_block - 1) / per_block, most = (int64_t)sm_count() * std::max(1, 512 / threads);
+    const int64_t rounds = (groups + most - 1) / most, blocks = (groups + rounds - 1) / rounds;
     if (params) {
       parts = (int)blocks;
       NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));
@@ -590,7 +592,7 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
                    : run(std::integral_constant<int, 1>{}));
   }
   if (params)
-    NB_CUDA(launch_dependent(layer_norm_param_kernel<P>, dim3((unsigned)((size + 31) / 32), 2), dim3(512), 0, st,
+    NB_CUDA(launch_dependent(layer_norm_param_kernel<P>, dim3((unsigned)((size + 31) / 32), 2), dim3(1024), 0, st,
                              static_cast<const float *>(scratch.p), parts, size, dbeta, dgamma, accum_beta, accum_gamma));
   return NB200_OK;
 }

@@ -583,20 +583,7 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
   NB_TRY(device_status_word(&status));
   constexpr int kCtas = kPair ? 2 : 1;
   const int units = (int)std::min<int64_t>(sm_count() / kCtas, tiles);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kCtas * units);
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCtas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  NB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma[0], mb[0], ma[1], mb[1], prob, status));
+  NB_CUDA(launch_clusters(kernel, kCtas * units, kCtas, kPairThreads, S::kSmem, st, ma[0], mb[0], ma[1], mb[1], prob, status));
   return NB200_OK;
 }
 
