@@ -11,7 +11,6 @@
 
 #include "few_rows.cuh"
 #include "loss_gemm.cuh"
-#include "prepare.cuh"
 
 namespace nb200 {
 namespace {
@@ -39,110 +38,212 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(LossRows rows, int64_t c
   }
 }
 
-// db (+)= the column sums of G, [planes][rows][ld], a block 32 columns; scale[2] (scale NULL: 1) undoes G's scaling.
-template <typename G, typename TO>
-__global__ void __launch_bounds__(512) column_sums_kernel(const G *__restrict__ g, int planes, int64_t rows, int64_t columns,
-                                                          int64_t ld, const float *scale, TO *db, bool accum) {
-  __shared__ float sums[16][33];
+// Column sums of G, [planes][rows][ld]: a thread eight (fp32: four) neighbouring columns, a block's eight warps its slab of
+// rows in turn; part[slab][ldp].
+template <typename G>
+__global__ void __launch_bounds__(256) column_sums_kernel(const G *__restrict__ g, int64_t all_rows, int64_t slab,
+                                                          int64_t columns, int64_t ld, float *__restrict__ part, int64_t ldp) {
+  constexpr int V = kPackOf<G>;
+  __shared__ float sums[8][32 * V];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0.0f;
-  if (c < columns)
-#pragma unroll 8
-    for (int64_t r = warp; r < planes * rows; r += 16)
-      s += to_f32(g[r * ld + c]);
-  sums[warp][lane] = s;
+  const int64_t c0 = (int64_t)blockIdx.x * 32 * V, c = c0 + lane * V, r0 = blockIdx.y * slab;
+  const int64_t r1 = r0 + slab < all_rows ? r0 + slab : all_rows;
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    s[j] = 0.0f;
+  if (c < columns) // (ld is a multiple of V and G is as wide)
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      const Pack<G, V> p = load_pack<G, V>(g + r * ld + c);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        s[j] += p.f(j);
+    }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    sums[warp][lane * V + j] = s[j];
   __syncthreads();
-  if (warp == 0 && c < columns) {
-    s = 0.0f;
+  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+    float t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w)
-      s += sums[w][lane];
-    if (scale)
-      s *= scale[2];
-    db[c] = from_f32<TO>(accum ? s + to_f32(db[c]) : s);
+    for (int w = 0; w < 8; ++w)
+      t += sums[w][i];
+    if (c0 + i < ldp)
+      part[blockIdx.y * ldp + c0 + i] = t;
   }
 }
 
-// to (+)= the sum of `parts` tensors of n values, in order.
-template <typename T>
-__global__ void __launch_bounds__(256) round_kernel(const float *__restrict__ from, int parts, T *to, int64_t n, bool accum) {
+// to [rows][ldt] (+)= scale[2] (scale NULL: 1) * the sum, in order, of `parts` matrices [rows][ldf], `stride` apart.
+// V columns a thread.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float *__restrict__ from, int parts, int64_t stride, int64_t rows,
+                                                        int64_t cols, int64_t ldf, const float *scale, T *to, int64_t ldt,
+                                                        bool accum) {
   pdl_wait();
   pdl_trigger();
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float s = 0.0f;
-    for (int p = 0; p < parts; ++p)
-      s += from[p * n + i];
-    to[i] = from_f32<T>(accum ? s + to_f32(to[i]) : s);
-  }
-}
-
-// [rows][cols] -> [rows][pitch] of 16-bit values, for rows that a TMA copy cannot read where they lie; eight values a thread.
-__global__ void __launch_bounds__(256) repitch_kernel(const uint16_t *__restrict__ from, uint16_t *__restrict__ to,
-                                                      int64_t rows, int64_t cols, int64_t pitch) {
-  pdl_wait();
-  pdl_trigger();
-  const int64_t packs = pitch / 8;
+  const int64_t packs = (cols + V - 1) / V;
+  const float times = scale ? scale[2] : 1.0f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * packs; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / packs, c = (i - r * packs) * 8;
-    Pack<uint16_t, 8> v;
+    const int64_t r = i / packs, c = (i - r * packs) * V;
+    float s[V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v.v[j] = c + j < cols ? from[r * cols + c + j] : (uint16_t)0;
-    *reinterpret_cast<Pack<uint16_t, 8> *>(to + r * pitch + c) = v;
+    for (int j = 0; j < V; ++j)
+      s[j] = 0.0f;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) {
+      const Pack<float, V> f = load_pack<float, V>(from + p * stride + r * ldf + c);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        s[j] += f.v[j];
+    }
+    T *t = to + r * ldt + c;
+    Pack<T, V> old;
+    if (accum)
+      old = load_pack<T, V>(t);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s[j] *= times;
+      if (accum)
+        s[j] += old.f(j);
+    }
+    store_pack<T, V>(t, s);
   }
 }
+template <typename T>
+int add_parts(const float *from, int parts, int64_t stride, int64_t rows, int64_t cols, int64_t ldf, const float *scale, T *to,
+              int64_t ldt, bool accum, cudaStream_t st) {
+  const bool vec = cols % 4 == 0 && stride % 4 == 0 && ldf % 4 == 0 && ldt % 4 == 0 && aligned16(from) &&
+                   (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(T) - 1)) == 0;
+  const int64_t items = rows * ((cols + (vec ? 3 : 0)) / (vec ? 4 : 1));
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, 16 * sm_count())));
+  NB_CUDA(launch_dependent(vec ? add_parts_kernel<T, 4> : add_parts_kernel<T, 1>, grid, dim3(256), 0, st, from, parts, stride,
+                           rows, cols, ldf, scale, to, ldt, accum));
+  return NB200_OK;
+}
 
-// What G is kept relative to: scale = {the largest |dloss| of a row that counts, 2^e, their quotient}. With the largest taken
+// db (+)= the column sums of G [planes * rows][ld], of which `part` holds slabs() rows of ld sums.
+template <typename G> int64_t column_slabs(int64_t all_rows, int64_t columns) {
+  const int64_t wide = (columns + 32 * kPackOf<G> - 1) / (32 * kPackOf<G>);
+  return std::max<int64_t>(1, std::min<int64_t>((all_rows + 31) / 32, 4 * sm_count() / wide));
+}
+template <typename G, typename T>
+int column_sums(const G *g, int64_t all_rows, int64_t columns, int64_t ld, float *part, const float *scale, T *db, bool accum,
+                cudaStream_t st) {
+  const int64_t slabs = column_slabs<G>(all_rows, columns), slab = (all_rows + slabs - 1) / slabs;
+  const int64_t count = (all_rows + slab - 1) / slab, wide = (columns + 32 * kPackOf<G> - 1) / (32 * kPackOf<G>);
+  NB_CUDA(launch_dependent(column_sums_kernel<G>, dim3((unsigned)wide, (unsigned)count), dim3(256), 0, st, g, all_rows, slab,
+                           columns, ld, part, ld));
+  return add_parts<T>(part, (int)count, ld, 1, columns, ld, scale, db, 0, accum, st);
+}
+
+// What the tensor-core products need before they start, in one launch: up to two matrices laid out as operands (fp32: three
+// bf16 pieces; 16 bits: rows at a pitch that a TMA copy can read), and the scale of G.
+struct Layout {
+  const void *from; // NULL: the matrix is an operand as it lies
+  void *to;
+  int64_t rows, cols, pitch, packs; // packs: rows * pitch / 8
+};
+struct Preparation {
+  Layout m[2];
+  unsigned blocks[2]; // blocks of 256 threads for each, eight values a thread and step
+  LossRows rows;      // G's scale, by one more block where scale is not NULL
+  int64_t count;
+  float times;
+  float *scale;
+};
+
+// scale = {the largest |dloss| of a row that counts, 2^e, their quotient}: what G is kept relative to. With the largest taken
 // out, the gradient of a mean, the same in every row, is no rounded factor of G: at the label G is -1 + p. e is 14 for an fp16 G,
 // which so has eleven bits down to 2^-28 of the largest gradient, and 0 for the others.
-__global__ void __launch_bounds__(1024) gradient_scale_kernel(LossRows rows, int64_t count, float times, float *scale) {
-  __shared__ float tops[32];
-  pdl_wait();
-  pdl_trigger();
+__device__ void gradient_scale(const Preparation &p) {
+  __shared__ float tops[8];
   float top = 0.0f;
-  for (int64_t r = threadIdx.x; r < count; r += 1024)
-    if (rows.label_of(r) >= 0)
-      top = fmaxf(top, fabsf(rows.dloss[r]));
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < p.count; r += 256)
+    if (p.rows.label_of(r) >= 0)
+      top = fmaxf(top, fabsf(p.rows.dloss[r]));
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0)
     tops[threadIdx.x >> 5] = top;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    top = warp_max(tops[threadIdx.x]);
-    if (threadIdx.x == 0) {
-      // (none, or one that is not finite: G as it is)
-      const bool plain = !(top >= 1.17549435e-38f && top < INFINITY);
-      scale[0] = plain ? 1.0f : top;
-      scale[1] = times;
-      scale[2] = (plain ? 1.0f : top) / times;
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w)
+      top = fmaxf(top, tops[w]);
+    // (none, or one that is not finite: G as it is)
+    const bool plain = !(top >= 1.17549435e-38f && top < INFINITY);
+    p.scale[0] = plain ? 1.0f : top;
+    p.scale[1] = p.times;
+    p.scale[2] = (plain ? 1.0f : top) / p.times;
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) loss_prepare_kernel(const __grid_constant__ Preparation p) {
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == p.blocks[0] + p.blocks[1]) {
+    gradient_scale(p);
+    return;
+  }
+  const int which = blockIdx.x < p.blocks[0] ? 0 : 1;
+  const Layout &m = p.m[which];
+  const T *from = static_cast<const T *>(m.from);
+  const bool vec = std::is_same<T, float>::value && m.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+  const int64_t per_row = m.pitch / 8, step = (int64_t)p.blocks[which] * 256;
+  for (int64_t i = (int64_t)(blockIdx.x - (which ? p.blocks[0] : 0)) * 256 + threadIdx.x; i < m.packs; i += step) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    const T *src = from + r * m.cols + c;
+    Pack<T, 8> v;
+    if (vec && c + 8 <= m.cols) {
+      v = load_pack<T, 8>(src);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v.v[j] = c + j < m.cols ? src[j] : from_f32<T>(0.0f);
+    }
+    if constexpr (std::is_same<T, float>::value) {
+      __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(m.to) + r * m.pitch + c;
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl) {
+        const Pack<__nv_bfloat16, 8> h = round_pack<__nv_bfloat16, 8>(v.v);
+        *reinterpret_cast<Pack<__nv_bfloat16, 8> *>(to + pl * m.rows * m.pitch) = h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v.v[j] = __fsub_rn(v.v[j], h.f(j));
+      }
+    } else {
+      *reinterpret_cast<Pack<T, 8> *>(static_cast<T *>(m.to) + r * m.pitch + c) = v;
     }
   }
 }
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// A matrix as an operand of the tensor-core products: as it lies, or (rows that a TMA copy cannot read, fp32) laid out anew
-// in `scratch`, of operand_bytes().
+// A matrix as an operand of the tensor-core products: as it lies, or laid out anew in operand_bytes() of scratch.
 template <typename T> size_t operand_bytes(const T *p, int64_t rows, int64_t cols) {
   if (std::is_same<T, float>::value)
     return (size_t)3 * rows * up(cols, 64) * 2;
   return cols % 8 == 0 && aligned16(p) ? 0 : (size_t)rows * up(cols, 8) * 2;
 }
-template <typename T> int make_operand(const T *p, int64_t rows, int64_t cols, void *scratch, Operand &o, cudaStream_t st) {
-  o = {scratch, rows, cols, up(cols, std::is_same<T, float>::value ? 64 : 8), 1};
-  if constexpr (std::is_same<T, float>::value) {
-    o.planes = 3;
-    return split_rows_bf16(SplitRows{p, nullptr, scratch, rows, (int)cols, 3}, SplitRows{}, o.pitch, st);
-  } else if (operand_bytes(p, rows, cols) == 0) {
+template <typename T> Operand operand(const T *p, int64_t rows, int64_t cols, void *scratch, Layout &layout) {
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  Operand o{scratch, rows, cols, up(cols, kF32 ? 64 : 8), kF32 ? 3 : 1};
+  layout = Layout{};
+  if (operand_bytes(p, rows, cols) == 0)
     o.p = p;
-  } else {
-    const int64_t blocks = (rows * (o.pitch / 8) + 255) / 256;
-    NB_CUDA(launch_dependent(repitch_kernel, dim3((unsigned)std::min<int64_t>(blocks, 64 * sm_count())), dim3(256), 0, st,
-                             reinterpret_cast<const uint16_t *>(p), static_cast<uint16_t *>(scratch), rows, cols, o.pitch));
-  }
+  else
+    layout = Layout{p, scratch, rows, cols, o.pitch, rows * o.pitch / 8};
+  return o;
+}
+template <typename T> int prepare(Preparation &p, cudaStream_t st) {
+  for (int i = 0; i < 2; ++i)
+    p.blocks[i] = p.m[i].from ? (unsigned)std::min<int64_t>((p.m[i].packs + 255) / 256, 32 * sm_count()) : 0;
+  const unsigned blocks = p.blocks[0] + p.blocks[1] + (p.scale ? 1 : 0);
+  if (blocks)
+    NB_CUDA(launch_dependent(loss_prepare_kernel<T>, dim3(blocks), dim3(256), 0, st, p));
   return NB200_OK;
 }
 Operand columns(Operand o, int64_t c0, int64_t n) {
@@ -182,7 +283,7 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
                    int64_t classes, cudaStream_t st) {
   const int kblocks = (int)((size + 63) / 64);
   const bool pair = pays_pairs({{rows, classes, kblocks}});
-  r.tiles = (int)(2 * ((classes + (pair ? 255 : 63)) / (pair ? 256 : 64)));
+  r.tiles = loss_sum_tiles<T>(classes, kblocks, pair);
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
   const size_t at_partial = parts.take((size_t)rows * r.tiles * 8), at_target = parts.take((size_t)rows * 4);
@@ -191,15 +292,15 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
   char *base = static_cast<char *>(scratch.p);
   r.partial = reinterpret_cast<float2 *>(base + at_partial);
   r.target = reinterpret_cast<float *>(base + at_target);
-  Operand ox, ow;
-  NB_TRY(make_operand(x, rows, size, base + at_x, ox, st));
-  NB_TRY(make_operand(w, size, classes, base + at_w, ow, st));
+  Preparation pre{};
+  const Operand ox = operand(x, rows, size, base + at_x, pre.m[0]), ow = operand(w, size, classes, base + at_w, pre.m[1]);
+  NB_TRY(prepare<T>(pre, st));
   Products prob{};
   prob.count = 1;
   prob.bias = bias;
   prob.rows = r;
   prob.p[0].M = (int)rows, prob.p[0].N = (int)classes, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
-  NB_TRY((pair ? launch_loss_gemm<T, true, Out::kSums> : launch_loss_gemm<T, false, Out::kSums>)(prob, &ox, &ow, st));
+  NB_TRY((run_loss_gemm<T, Out::kSums>(pair, prob, &ox, &ow, st)));
   NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, r, rows, loss, stat));
   return NB200_OK;
 }
@@ -216,34 +317,41 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   const int64_t count = (classes + piece - 1) / piece;
   piece = up((classes + count - 1) / count, 256);
   const bool pieces = piece < classes;
-  // Few tiles of dx with a long K: its classes in up to 16 parts, each with sums of its own that round_kernel adds up.
   const int64_t size_blocks = (size + 63) / 64, row_blocks = (rows + 63) / 64, piece_blocks = (std::min(piece, classes) + 63) / 64;
   const bool pair_grad = pays_pairs({{rows, piece, size_blocks}});
   const bool pair = pays_pairs({{dw ? size : 0, piece, row_blocks}, {dx ? rows : 0, size, piece_blocks}});
-  int splits = 1;
-  if (dx) {
-    const int64_t tiles = ((rows + (pair ? 255 : 127)) / (pair ? 256 : 128)) * ((size + (pair ? 255 : 63)) / (pair ? 256 : 64));
-    const int64_t units = pair ? sm_count() / 2 : sm_count();
-    while (splits < 16 && tiles * splits * 2 <= units && piece_blocks >= 8 * splits)
+  // A product with few tiles and a long K (dx of few rows, dW of many) has it in up to 16 parts, each with sums of its own that
+  // add_parts joins, until a tile is a third of an SM's share at most.
+  const int64_t tile_m = pair ? 256 : 128, tile_n = pair ? 256 : 64, units = pair ? sm_count() / 2 : sm_count();
+  const int64_t dw_tiles = dw ? (size + tile_m - 1) / tile_m * ((piece + tile_n - 1) / tile_n) : 0;
+  const int64_t dx_tiles = dx ? (rows + tile_m - 1) / tile_m * ((size + tile_n - 1) / tile_n) : 0;
+  const int64_t share = std::max<int64_t>(8, (dw_tiles * row_blocks + dx_tiles * piece_blocks) / (3 * units));
+  auto split = [&](int64_t tiles, int64_t blocks, int &splits, int &split_blocks) {
+    splits = 1;
+    while (splits < 16 && tiles * splits < 4 * units && blocks > share * splits)
       splits *= 2;
-  }
-  const int split_blocks = (int)((piece_blocks + splits - 1) / splits);
-  splits = (int)((piece_blocks + split_blocks - 1) / split_blocks); // no empty part (a last, smaller piece may leave some)
-  const bool direct = splits == 1 && (!pieces || (kF32 && !accum[0])); // dx without sums of its own
+    split_blocks = (int)((blocks + splits - 1) / splits);
+    splits = (int)((blocks + split_blocks - 1) / split_blocks); // no empty part (a last, smaller piece may leave some)
+  };
+  int dx_splits, dx_blocks, dw_splits, dw_blocks;
+  split(dx_tiles, piece_blocks, dx_splits, dx_blocks);
+  split(dw_tiles, row_blocks, dw_splits, dw_blocks);
+  const bool direct = dx_splits == 1 && (!pieces || (kF32 && !accum[0])); // dx without sums of its own
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
   const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(12);
-  const size_t at_dx = parts.take(dx && !direct ? (size_t)splits * rows * size * 4 : 0);
+  const size_t at_dx = parts.take(dx && !direct ? (size_t)dx_splits * rows * size * 4 : 0);
+  const size_t at_dw = parts.take(dw && dw_splits > 1 ? (size_t)dw_splits * size * piece * 4 : 0);
+  const size_t at_db = parts.take(db ? (size_t)column_slabs<G>(kPlanes * rows, piece) * piece * 4 : 0);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc(parts.bytes));
   char *base = static_cast<char *>(scratch.p);
-  float *dx32 = reinterpret_cast<float *>(base + at_dx);
-  Operand ox, ow;
-  NB_TRY(make_operand(x, rows, size, base + at_x, ox, st));
-  NB_TRY(make_operand(w, size, classes, base + at_w, ow, st));
+  float *dx32 = reinterpret_cast<float *>(base + at_dx), *dw32 = reinterpret_cast<float *>(base + at_dw);
   float *scale = reinterpret_cast<float *>(base + at_scale);
-  NB_CUDA(launch_dependent(gradient_scale_kernel, dim3(1), dim3(1024), 0, st, r, rows,
-                           std::is_same<T, __half>::value ? 16384.0f : 1.0f, scale));
+  Preparation pre{};
+  const Operand ox = operand(x, rows, size, base + at_x, pre.m[0]), ow = operand(w, size, classes, base + at_w, pre.m[1]);
+  pre.rows = r, pre.count = rows, pre.scale = scale, pre.times = std::is_same<T, __half>::value ? 16384.0f : 1.0f;
+  NB_TRY(prepare<T>(pre, st));
   r.scale = scale;
   for (int64_t c0 = 0; c0 < classes; c0 += piece) {
     const int64_t n = std::min(piece, classes - c0);
@@ -256,36 +364,42 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
     Product &l = prob.p[0];
     l.M = (int)rows, l.N = (int)n, l.kblocks = (int)size_blocks, l.b_mn = 1;
     l.out = base + at_g, l.ldo = piece, l.stride = rows * piece;
-    NB_TRY((pair_grad ? launch_loss_gemm<T, true, Out::kGrad> : launch_loss_gemm<T, false, Out::kGrad>)(prob, &ox, &owc, st));
+    NB_TRY((run_loss_gemm<T, Out::kGrad>(pair_grad, prob, &ox, &owc, st)));
     Operand a[2], b[2];
     prob.count = 0;
     if (dw) {
       Product &p = prob.p[prob.count];
       p = Product{};
       p.M = (int)size, p.N = (int)n, p.kblocks = (int)row_blocks, p.a_mn = p.b_mn = 1;
-      p.out = dw + c0, p.ldo = classes, p.accum = accum[1];
-      p.vec = classes * sizeof(T) % 16 == 0 && aligned16(dw);
+      if (dw_splits > 1) {
+        p.splits = dw_splits, p.split_blocks = dw_blocks, p.stride = size * piece;
+        p.out = dw32, p.ldo = piece, p.out_f32 = 1, p.vec = 1;
+      } else {
+        p.out = dw + c0, p.ldo = classes, p.accum = accum[1];
+        p.vec = classes * sizeof(T) % 16 == 0 && aligned16(dw);
+      }
       a[prob.count] = ox, b[prob.count++] = og;
     }
     if (dx) {
       Product &p = prob.p[prob.count];
       p = Product{};
       p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64), p.ldo = size;
-      p.splits = (p.kblocks + split_blocks - 1) / split_blocks, p.split_blocks = split_blocks, p.stride = rows * size;
+      p.splits = (p.kblocks + dx_blocks - 1) / dx_blocks, p.split_blocks = dx_blocks, p.stride = rows * size;
       p.out = direct ? static_cast<void *>(dx) : dx32, p.out_f32 = !direct;
       p.accum = c0 > 0 || (direct && accum[0]);
       p.vec = size * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
       a[prob.count] = og, b[prob.count++] = owc;
     }
     if (prob.count)
-      NB_TRY((pair ? launch_loss_gemm<T, true, Out::kStore> : launch_loss_gemm<T, false, Out::kStore>)(prob, a, b, st));
+      NB_TRY((run_loss_gemm<T, Out::kStore>(pair, prob, a, b, st)));
+    if (dw && dw_splits > 1)
+      NB_TRY(add_parts<T>(dw32, dw_splits, size * piece, size, n, piece, nullptr, dw + c0, classes, accum[1], st));
     if (db)
-      NB_CUDA(launch_dependent(column_sums_kernel<G, T>, dim3((unsigned)((n + 31) / 32)), dim3(512), 0, st,
-                               reinterpret_cast<const G *>(base + at_g), kPlanes, rows, n, piece, r.scale, db + c0, accum[2]));
+      NB_TRY((column_sums<G, T>(reinterpret_cast<const G *>(base + at_g), kPlanes * rows, n, piece,
+                                reinterpret_cast<float *>(base + at_db), scale, db + c0, accum[2], st)));
   }
   if (dx && !direct)
-    NB_CUDA(launch_dependent(round_kernel<T>, dim3((unsigned)std::min<int64_t>((rows * size + 255) / 256, 8 * sm_count())),
-                             dim3(256), 0, st, (const float *)dx32, splits, dx, rows * size, accum[0]));
+    NB_TRY(add_parts<T>(dx32, dx_splits, rows * size, 1, rows * size, rows * size, nullptr, dx, rows * size, accum[0], st));
   return NB200_OK;
 }
 
@@ -331,8 +445,7 @@ int backward(const T *x, const T *w, const T *bias, LossRows r, T *dx, T *dw, T 
     }));
   }
   if (db)
-    NB_CUDA(launch_dependent(column_sums_kernel<float, T>, dim3((unsigned)((classes + 31) / 32)), dim3(512), 0, st,
-                             (const float *)g, 1, rows, classes, ldg, (const float *)nullptr, db, accum[2]));
+    NB_TRY(add_parts<T>(g, (int)rows, ldg, 1, classes, ldg, nullptr, db, classes, accum[2], st));
   return NB200_OK;
 }
 

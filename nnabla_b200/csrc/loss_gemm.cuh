@@ -55,21 +55,26 @@ struct Product {
 struct Products {
   Product p[kMaxProducts];
   int count;
+  int extra_tiles; // see the kernel's tile_at
   int chunk;  // K blocks accumulated in tensor memory
   int class0; // kSums, kGrad: the class of the first column
   const void *bias;
   LossRows rows;
 };
 
-template <int PL, bool kPair> struct LossShape {
+// kLong: K goes through tensor memory in more than one chunk, and the chunks' sums take an epilogue thread 128 registers; eight
+// epilogue warps. Without them there is room for sixteen, which a short K needs: its tiles are bound by the epilogue's latencies
+// (K = 302: 1900 cycles a 16-column step with two warps a scheduler, 2560 cycles of MMAs a tile of 256 columns).
+template <int PL, bool kPair, bool kLong> struct LossShape {
+  static constexpr int kWarps = kPair && !kLong ? 16 : 8, kThreads = 32 * (2 + kWarps); // epilogue warps; threads
   static constexpr int kTileRows = kPair ? 256 : 128, kTileCols = kPair ? 256 : 64; // of a cluster
   static constexpr int kCtaCols = kPair ? 128 : 64;                                 // columns of B that a CTA loads
   static constexpr uint32_t kABytes = kTileM * kRowBytes, kBBytes = kCtaCols * kRowBytes;
   static constexpr uint32_t kStageBytes = PL * (kABytes + kBBytes);
-  static constexpr int kStages = PL == 3 ? 2 : 6;
+  static constexpr int kStages = PL == 3 ? 2 : kWarps == 16 ? 5 : 6;
   static constexpr int kWarpStage = 32 * 32 * 4; // bytes of an epilogue warp's transpose buffer
   static constexpr size_t kSmem =
-      (size_t)kStages * kStageBytes + kPairEpilogueWarps * kWarpStage + (2 * kStages + 4) * 8 + 16 + 1024;
+      (size_t)kStages * kStageBytes + kWarps * kWarpStage + (2 * kStages + 4) * 8 + 16 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
 };
 
@@ -89,25 +94,26 @@ template <typename T> __device__ __forceinline__ void store16(T *p, const float 
 }
 
 // T: the operands' type; float means three bf16 planes.
-template <typename T, bool kPair, Out kOut>
-__global__ void __launch_bounds__(kPairThreads, 1)
+template <typename T, bool kPair, bool kLong, Out kOut>
+__global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 1, kPair, kLong>::kThreads, 1)
     loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
                      const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
                      const __grid_constant__ Products prob, int *status) {
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int PL = kF32 ? 3 : 1;
-  using S = LossShape<PL, kPair>;
+  using S = LossShape<PL, kPair, kLong>;
   constexpr int STAGES = S::kStages, BN = S::kTileCols;
   constexpr uint32_t kABytes = S::kABytes, kBBytes = S::kBBytes, kStageBytes = S::kStageBytes;
   constexpr uint32_t kChunkBytes = 64 * kRowBytes; // 64 columns x 64 of K of an MN-major operand
-  constexpr int kMyChunks = BN / 64;               // column chunks of 32 that an epilogue warp drains
+  constexpr int kParts = S::kWarps / 4;            // epilogue warps that share the rows of a quarter
+  constexpr int kMyChunks = BN / (32 * kParts);    // column chunks of 32 that each drains
   constexpr uint32_t kTmemCols = 2 * BN;
   constexpr uint32_t kCtas = kPair ? 2 : 1;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float *stage_out = reinterpret_cast<float *>(smem + STAGES * kStageBytes);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * kStageBytes + kPairEpilogueWarps * S::kWarpStage);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * kStageBytes + S::kWarps * S::kWarpStage);
   uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tmem_full = bars + 2 * STAGES, *tmem_empty = tmem_full + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -126,7 +132,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(tmem_full + b, 1);
-      ptx::mbar_init(tmem_empty + b, kCtas * kPairEpilogueWarps);
+      ptx::mbar_init(tmem_empty + b, kCtas * S::kWarps);
     }
     *abort_flag = 0;
     ptx::mbar_fence_init();
@@ -175,6 +181,22 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     t.kb1 = t.kb0 + p.split_blocks < p.kblocks ? t.kb0 + p.split_blocks : p.kblocks;
     return t;
   };
+  // This unit's i-th tile, or -1: the first product's dealt out one by one; of the second's, `extra_tiles` to each of the units
+  // that got one more of the first, the rest to the others.
+  const int more = tiles0 % units, own0 = tiles0 / units + (unit < more ? 1 : 0);
+  auto tile_at = [&](int i) -> int {
+    if (i < own0)
+      return unit + i * units;
+    if (kOut != Out::kStore || num_tiles == tiles0)
+      return -1;
+    i -= own0;
+    int t;
+    if (unit < more)
+      t = i < prob.extra_tiles ? unit + i * more : num_tiles;
+    else
+      t = more * prob.extra_tiles + (unit - more) + i * (units - more);
+    return t < num_tiles - tiles0 ? tiles0 + t : -1;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (every CTA)
@@ -183,7 +205,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t keep = ptx::l2_policy_evict_last();
-      for (int tile = unit; tile < num_tiles && ok; tile += units) {
+      for (int i = 0, tile; ok && (tile = tile_at(i)) >= 0; ++i) {
         const At t = decode(tile);
         const bool a_mn = prob.p[t.which].a_mn != 0, b_mn = prob.p[t.which].b_mn != 0;
         const CUtensorMap *ma = t.which ? &map_a1 : &map_a0, *mb = t.which ? &map_b1 : &map_b0;
@@ -244,7 +266,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           ptx::mma_commit(bar);
         }
       };
-      for (int tile = unit; tile < num_tiles && ok; tile += units) {
+      for (int i = 0, tile; ok && (tile = tile_at(i)) >= 0; ++i) {
         const At t = decode(tile);
         const bool a_mn = prob.p[t.which].a_mn != 0, b_mn = prob.p[t.which].b_mn != 0;
         const uint32_t idesc = ptx::make_idesc(1u, std::is_same<T, __half>::value ? 0u : 1u, S::kTileRows, BN) |
@@ -301,14 +323,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA): a thread a row
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
     const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const LossRows &rows = prob.rows;
     float *stg = stage_out + (warp - 2) * (S::kWarpStage / 4);
     int local = 0;
     bool ok = true;
-    float acc[2 * kMyChunks][16]; // 16 columns at a time: with 32 the sums and a chunk do not fit in 168 registers
-    for (int tile = unit; tile < num_tiles && ok; tile += units) {
+    float acc[kLong ? 2 * kMyChunks : 1][16]; // 16 columns at a time: with 32 the sums and a chunk do not fit in 168 registers
+    for (int i = 0, tile; ok && (tile = tile_at(i)) >= 0; ++i) {
       const At at = decode(tile);
       const Product &p = prob.p[at.which];
       const int M = p.M, N = p.N, n0 = at.n0;
@@ -334,6 +356,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int64_t out0 = at.split * p.stride;
       const int chunks = (at.kb1 - at.kb0 + prob.chunk - 1) / prob.chunk; // all but the last go to registers
       MaxSum t{-INFINITY, 0.0f};
+      if constexpr (kOut != Out::kStore)
+        if (prob.bias) { // this warp's columns of it, while the tile is being made
+          __syncwarp();
+#pragma unroll
+          for (int ci = 0; ci < kMyChunks; ++ci) {
+            const int c = n0 + 32 * part + 32 * kParts * ci + lane;
+            stg[32 * ci + lane] = c < N ? to_f32(static_cast<const T *>(prob.bias)[prob.class0 + c]) : 0.0f;
+          }
+          __syncwarp();
+        }
       for (int kc = 0; kc < chunks && ok; ++kc, ++local) {
         const int buf = local & 1;
         const bool got = ptx::mbar_wait(tmem_full + buf, (uint32_t)(local >> 1) & 1u, abort_flag);
@@ -347,24 +379,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const bool last = kc + 1 == chunks;
 #pragma unroll
         for (int ci = 0; ci < kMyChunks; ++ci) {
-          const int c0 = 32 * half + 64 * ci, col0 = n0 + c0;
+          const int c0 = 32 * part + 32 * kParts * ci, col0 = n0 + c0;
           if (col0 >= N)
             break;
           const int mine = (int)(label - prob.class0 - col0); // the label's column in this chunk, if in [0, 32)
-          float b_lane = 0.0f;
-          if constexpr (kOut != Out::kStore)
-            if (prob.bias && last && col0 + lane < N)
-              b_lane = to_f32(static_cast<const T *>(prob.bias)[prob.class0 + col0 + lane]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             __syncwarp(); // (the staged chunk before has been read, and the load below is the whole warp's)
             uint32_t r[16];
-            float(&sum)[16] = acc[2 * ci + h];
+            float(&sum)[16] = acc[kLong ? 2 * ci + h : 0];
             ptx::tmem_ld_32x16(lanes + (uint32_t)(buf * BN + c0 + 16 * h), r);
             ptx::tmem_ld_wait();
             if (row_base >= M)
               continue;
-            if (!last) {
+            if (kLong && !last) {
 #pragma unroll
               for (int j = 0; j < 16; ++j)
                 sum[j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
@@ -373,7 +401,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             float v[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              v[j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
+              v[j] = !kLong || kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
             const int col = col0 + 16 * h;
             if constexpr (kOut == Out::kStore) {
 #pragma unroll
@@ -420,8 +448,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             } else {
               if (prob.bias)
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  v[j] += __shfl_sync(0xffffffffu, b_lane, 16 * h + j);
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 b = *reinterpret_cast<const float4 *>(stg + 32 * ci + 16 * h + j);
+                  v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+                }
               const int here = mine >= 16 * h && mine < 16 * h + 16 ? mine - 16 * h : -1;
               if constexpr (kOut == Out::kSums) {
                 if (col + 16 > N)
@@ -436,16 +466,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     l = j == here ? v[j] : l;
                   rows.target[row] = l;
                 }
-                float m = t.m;
+                float m4[4] = {t.m, v[1], v[2], v[3]}; // four chains each, for their latency
+                m4[0] = fmaxf(m4[0], v[0]);
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  m = fmaxf(m, v[j]);
+                for (int j = 4; j < 16; ++j)
+                  m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 const float b = m == -INFINITY ? 0.0f : m;
-                float s = t.s * ex2((t.m - b) * kLog2e);
+                float s4[4] = {t.s * ex2((t.m - b) * kLog2e), 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                  s += ex2((v[j] - b) * kLog2e);
-                t = {m, s};
+                  s4[j & 3] += ex2((v[j] - b) * kLog2e);
+                t = {m, (s4[0] + s4[1]) + (s4[2] + s4[3])};
               } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
@@ -512,7 +544,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       if constexpr (kOut == Out::kSums)
         if (ok && row_ok)
-          rows.partial[(int64_t)row * rows.tiles + n0 / BN * 2 + half] = make_float2(t.m, t.s);
+          rows.partial[(int64_t)row * rows.tiles + n0 / BN * kParts + part] = make_float2(t.m, t.s);
     }
   }
 
@@ -549,11 +581,21 @@ inline int loss_operand_map(CUtensorMap *map, const Operand &o, bool mn, int box
   return encode_tiled(map, 0, 3, o.p, dims, strides, box, nullptr, 128);
 }
 
-template <typename T, bool kPair, Out kOut>
+// 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
+// last four steps are the only ones on a large accumulator
+template <typename T> constexpr int loss_chunk() { return std::is_same<T, float>::value ? 1 : 24; }
+template <typename T> bool loss_is_long(int64_t kblocks) { return kblocks > loss_chunk<T>(); }
+// The maxima and sums that kSums leaves of a row.
+template <typename T> int loss_sum_tiles(int64_t classes, int64_t kblocks, bool pair) {
+  return (int)(pair ? (classes + 255) / 256 * (loss_is_long<T>(kblocks) || std::is_same<T, float>::value ? 2 : 4)
+                    : (classes + 63) / 64 * 2);
+}
+
+template <typename T, bool kPair, bool kLong, Out kOut>
 inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, cudaStream_t st) {
   constexpr int PL = std::is_same<T, float>::value ? 3 : 1;
-  using S = LossShape<PL, kPair>;
-  auto kernel = loss_gemm_kernel<T, kPair, kOut>;
+  using S = LossShape<PL, kPair, kLong>;
+  auto kernel = loss_gemm_kernel<T, kPair, kLong, kOut>;
   static std::atomic<bool> configured[64]{};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
@@ -561,30 +603,61 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
     NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
     configured[dev & 63] = true;
   }
+  Operand oa[kMaxProducts], ob[kMaxProducts];
+  for (int i = 0; i < prob.count; ++i) {
+    oa[i] = a[i], ob[i] = b[i];
+    if (prob.p[i].splits <= 1)
+      prob.p[i].splits = 1, prob.p[i].split_blocks = prob.p[i].kblocks;
+  }
+  if (prob.count == 2 && prob.p[0].split_blocks < prob.p[1].split_blocks) { // the product with the longer tiles first
+    std::swap(prob.p[0], prob.p[1]);
+    std::swap(oa[0], oa[1]);
+    std::swap(ob[0], ob[1]);
+  }
   CUtensorMap ma[2], mb[2];
-  int64_t tiles = 0;
+  int64_t tiles[2] = {0, 0}, cost[2] = {1, 1};
   for (int i = 0; i < prob.count; ++i) {
     Product &p = prob.p[i];
     p.m_tiles = (p.M + S::kTileRows - 1) / S::kTileRows;
     p.n_tiles = (p.N + S::kTileCols - 1) / S::kTileCols;
-    if (p.splits <= 1)
-      p.splits = 1, p.split_blocks = p.kblocks;
-    tiles += (int64_t)p.m_tiles * p.n_tiles * p.splits;
-    NB_TRY(loss_operand_map(&ma[i], a[i], p.a_mn, kTileM));
-    NB_TRY(loss_operand_map(&mb[i], b[i], p.b_mn, S::kCtaCols));
+    tiles[i] = (int64_t)p.m_tiles * p.n_tiles * p.splits;
+    cost[i] = p.split_blocks;
+    NB_TRY(loss_operand_map(&ma[i], oa[i], p.a_mn, kTileM));
+    NB_TRY(loss_operand_map(&mb[i], ob[i], p.b_mn, S::kCtaCols));
   }
-  NB_CHECK(tiles < (1ll << 31), NB200_EVALUE, "too many rows and classes");
+  NB_CHECK(tiles[0] + tiles[1] < (1ll << 31), NB200_EVALUE, "too many rows and classes");
   if (prob.count == 1)
     ma[1] = ma[0], mb[1] = mb[0];
-  // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
-  // last four steps are the only ones on a large accumulator
-  prob.chunk = PL == 3 ? 1 : 24;
+  constexpr int kCtas = kPair ? 2 : 1;
+  const int64_t units = std::min<int64_t>(sm_count() / kCtas, tiles[0] + tiles[1]);
+  // How many of the second product's tiles the units with one more of the first's get, so that the last one ends first.
+  const int64_t more = tiles[0] % units;
+  prob.extra_tiles = 0;
+  if (more && tiles[1]) {
+    int64_t best = -1;
+    for (int64_t n = 0; n <= (tiles[1] + more - 1) / more; ++n) {
+      const int64_t rest = std::max<int64_t>(0, tiles[1] - more * n);
+      const int64_t time = std::max(cost[0] + n * cost[1], (rest + units - more - 1) / (units - more) * cost[1]);
+      if (best < 0 || time < best)
+        best = time, prob.extra_tiles = (int)n;
+    }
+  }
+  prob.chunk = loss_chunk<T>();
   int *status = nullptr;
   NB_TRY(device_status_word(&status));
-  constexpr int kCtas = kPair ? 2 : 1;
-  const int units = (int)std::min<int64_t>(sm_count() / kCtas, tiles);
-  NB_CUDA(launch_clusters(kernel, kCtas * units, kCtas, kPairThreads, S::kSmem, st, ma[0], mb[0], ma[1], mb[1], prob, status));
+  NB_CUDA(launch_clusters(kernel, (unsigned)(kCtas * units), kCtas, S::kThreads, S::kSmem, st, ma[0], mb[0], ma[1], mb[1], prob,
+                          status));
   return NB200_OK;
+}
+template <typename T, Out kOut>
+int run_loss_gemm(bool pair, const Products &prob, const Operand *a, const Operand *b, cudaStream_t st) {
+  bool is_long = std::is_same<T, float>::value; // (fp32 has the registers' sums at any length)
+  for (int i = 0; i < prob.count; ++i)
+    is_long = is_long || loss_is_long<T>(prob.p[i].splits > 1 ? prob.p[i].split_blocks : prob.p[i].kblocks);
+  if constexpr (!std::is_same<T, float>::value)
+    if (!is_long)
+      return (pair ? launch_loss_gemm<T, true, false, kOut> : launch_loss_gemm<T, false, false, kOut>)(prob, a, b, st);
+  return (pair ? launch_loss_gemm<T, true, true, kOut> : launch_loss_gemm<T, false, true, kOut>)(prob, a, b, st);
 }
 
 } // namespace nb200
