@@ -161,10 +161,12 @@ struct Preparation {
 __device__ void gradient_scale(const Preparation &p) {
   __shared__ float tops[8];
   float top = 0.0f;
-#pragma unroll 4
-  for (int64_t r = threadIdx.x; r < p.count; r += 256)
-    if (p.rows.label_of(r) >= 0)
-      top = fmaxf(top, fabsf(p.rows.dloss[r]));
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < p.count; r += 256) {
+    const int64_t label = p.rows.label_of(r);
+    const float d = fabsf(p.rows.dloss[r]);
+    top = fmaxf(top, label >= 0 ? d : 0.0f);
+  }
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0)
     tops[threadIdx.x >> 5] = top;
@@ -311,9 +313,8 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kPlanes = kF32 ? 3 : 1;
   using G = std::conditional_t<kF32, __nv_bfloat16, T>;
-  // A piece's G is 2^26 values, 128 MB in 16 bits: large enough that the tiles of its products end in one round of few
-  // idle SMs, and read from L2 for the most part.
-  int64_t piece = std::max<int64_t>(1024, (int64_t)(1 << 26) / kPlanes / rows);
+  // A piece's G is 64 MB: both products read it from L2, and their tiles are rounds enough to leave few SMs idle.
+  int64_t piece = std::max<int64_t>(1024, (int64_t)(1 << 25) / kPlanes / rows);
   const int64_t count = (classes + piece - 1) / piece;
   piece = up((classes + count - 1) / count, 256);
   const bool pieces = piece < classes;
@@ -340,7 +341,8 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
   const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(12);
-  const size_t at_dx = parts.take(dx && !direct ? (size_t)dx_splits * rows * size * 4 : 0);
+  const int64_t ld_dx = up(size, 4); // of dx's own sums
+  const size_t at_dx = parts.take(dx && !direct ? (size_t)dx_splits * rows * ld_dx * 4 : 0);
   const size_t at_dw = parts.take(dw && dw_splits > 1 ? (size_t)dw_splits * size * piece * 4 : 0);
   const size_t at_db = parts.take(db ? (size_t)column_slabs<G>(kPlanes * rows, piece) * piece * 4 : 0);
   AsyncScratch scratch(st);
@@ -383,11 +385,11 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
     if (dx) {
       Product &p = prob.p[prob.count];
       p = Product{};
-      p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64), p.ldo = size;
-      p.splits = (p.kblocks + dx_blocks - 1) / dx_blocks, p.split_blocks = dx_blocks, p.stride = rows * size;
+      p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64), p.ldo = direct ? size : ld_dx;
+      p.splits = (p.kblocks + dx_blocks - 1) / dx_blocks, p.split_blocks = dx_blocks, p.stride = rows * ld_dx;
       p.out = direct ? static_cast<void *>(dx) : dx32, p.out_f32 = !direct;
       p.accum = c0 > 0 || (direct && accum[0]);
-      p.vec = size * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
+      p.vec = p.ldo * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
       a[prob.count] = og, b[prob.count++] = owc;
     }
     if (prob.count)
@@ -399,7 +401,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
                                 reinterpret_cast<float *>(base + at_db), scale, db + c0, accum[2], st)));
   }
   if (dx && !direct)
-    NB_TRY(add_parts<T>(dx32, dx_splits, rows * size, 1, rows * size, rows * size, nullptr, dx, rows * size, accum[0], st));
+    NB_TRY(add_parts<T>(dx32, dx_splits, rows * ld_dx, rows, size, ld_dx, nullptr, dx, size, accum[0], st));
   return NB200_OK;
 }
 
@@ -427,22 +429,29 @@ int backward(const T *x, const T *w, const T *bias, LossRows r, T *dx, T *dw, T 
              const bool accum[3], cudaStream_t st) {
   if (rows > kFewRows)
     return backward_tensor<T>(x, w, bias, r, dx, dw, db, rows, size, r.classes, accum, st);
-  const int64_t classes = r.classes, ldg = up(classes, 4);
+  const int64_t classes = r.classes, ldg = up(classes, 4), columns = (classes + 8 * kFewGradThreads - 1) / (8 * kFewGradThreads);
+  Parts parts;
+  const size_t at_g = parts.take((size_t)rows * ldg * 4), at_dx = parts.take(dx ? (size_t)columns * rows * size * 4 : 0);
   AsyncScratch scratch(st);
-  NB_TRY(scratch.alloc((size_t)rows * ldg * 4));
-  float *g = static_cast<float *>(scratch.p);
+  NB_TRY(scratch.alloc(parts.bytes));
+  char *base = static_cast<char *>(scratch.p);
+  float *g = reinterpret_cast<float *>(base + at_g), *dx32 = reinterpret_cast<float *>(base + at_dx);
   const bool vec = classes % kPackOf<T> == 0 && aligned16(w);
   NB_TRY(few_variant<T>(rows, vec, [&](auto n, auto v) {
     return few_logits<T, decltype(n)::value, decltype(v)::value>(x, w, bias, r, (int)rows, size, g, ldg, st);
   }));
   if (dx || dw) {
     const bool keep = (size_t)size * classes * sizeof(T) <= kKeepBytes;
+    const int64_t walks = (size + kFewWalk - 1) / kFewWalk, slabs = std::min<int64_t>(walks, (4 * sm_count() + columns - 1) / columns);
+    const int64_t slab = (walks + slabs - 1) / slabs * kFewWalk;
     NB_TRY(few_variant<T>(rows, vec && aligned16(dw), [&](auto n, auto v) -> int {
       NB_CUDA(launch_dependent(few_grads_kernel<T, decltype(n)::value, decltype(v)::value>,
-                               dim3((unsigned)((size + kFewH - 1) / kFewH)), dim3(kFewGradThreads), 0, st, x, w,
-                               (const float *)g, ldg, dx, dw, (int)rows, size, classes, accum[0], accum[1], keep));
+                               dim3((unsigned)columns, (unsigned)((size + slab - 1) / slab)), dim3(kFewGradThreads), 0, st, x, w,
+                               (const float *)g, ldg, dx != nullptr, dw, dx32, (int)rows, size, slab, classes, accum[1], keep));
       return NB200_OK;
     }));
+    if (dx)
+      NB_TRY(add_parts<T>(dx32, (int)columns, rows * size, 1, rows * size, rows * size, nullptr, dx, rows * size, accum[0], st));
   }
   if (db)
     NB_TRY(add_parts<T>(g, (int)rows, ldg, 1, classes, ldg, nullptr, db, classes, accum[2], st));

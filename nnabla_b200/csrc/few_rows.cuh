@@ -7,6 +7,23 @@ namespace nb200 {
 
 constexpr int kFewRows = 8;
 constexpr int kFewThreads = 256, kFewGradThreads = 256, kFewValues = 8192; // values: of x held in shared memory at a time
+// Two fp32 multiply-adds in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 constexpr int kFewBatch = 4, kFewBatches = 3;                         // packs a batch of copies, batches on the way
 constexpr int kFewRing = kFewBatch * kFewBatches * kFewThreads * 16; // bytes
 
@@ -47,12 +64,13 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
   const int64_t classes = rows.classes, c0 = group * kCols, c = c0 + (threadIdx.x % kLanes) * VEC;
   const bool here = c < classes; // (VEC divides classes, or is 1)
   const int64_t each = (size + splits - 1) / splits, ka = split * each, kb = ka + each < size ? ka + each : size;
-  float acc[R][VEC];
+  constexpr int kPairs = (VEC + 1) / 2; // of neighbouring classes
+  uint64_t acc[R][kPairs];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      acc[r][j] = 0.0f;
+    for (int j = 0; j < kPairs; ++j)
+      acc[r][j] = 0;
   // W by asynchronous copies, each thread for itself: kFewBatches batches of kFewBatch packs on the way, whatever the compiler
   // makes of the registers (of eight ordinary loads a step it kept few in flight: 3.4 TB/s). The batches are those of the loop
   // below, a full piece of K being whole batches.
@@ -83,15 +101,18 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
         xs[k * R + r] = r < count ? to_f32(x[r * size + k0 + k]) : 0.0f;
     __syncthreads();
     auto add = [&](const Pack<T, VEC> &v, int k) {
-      float xv[R];
+      uint64_t wv[kPairs];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        xv[r] = xs[k * R + r];
+      for (int j = 0; j < kPairs; ++j)
+        wv[j] = pair_of(v.f(2 * j), 2 * j + 1 < VEC ? v.f(2 * j + 1) : 0.0f);
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        const float xv = xs[k * R + r];
+        const uint64_t xx = pair_of(xv, xv);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          acc[r][j] = fmaf(xv[r], v.f(j), acc[r][j]);
+        for (int j = 0; j < kPairs; ++j)
+          acc[r][j] = fma2(xx, wv[j], acc[r][j]);
+      }
     };
     if constexpr (kAsync) {
       for (int k = k_first; k < n; k += kFewBatch * kStep) {
@@ -117,7 +138,8 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      float s = acc[r][j];
+      const float2 both = unpair(acc[r][j / 2]);
+      float s = j & 1 ? both.y : both.x;
 #pragma unroll
       for (int d = 16; d >= kLanes; d >>= 1)
         s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -174,96 +196,145 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// dx = G W^T and dW = x^T G in one pass over W: a block has kFewH rows of W, its threads walk along the classes. A pack of
-// G, [R][VEC] in fp32 from L2, serves all of the block's rows.
-constexpr int kFewH = 4;
+// dx = G W^T and dW = x^T G in one pass over W. A thread has eight columns of G in registers, [R][8] in fp32, and walks along
+// the rows of W: of each it loads its columns, stores those of dW and has R products for dx, which its warp sums up (the first
+// steps exchange halves of the R values, so that eight values take nine shuffles). The sums of a block's columns, 256 * 8, go to
+// partial[block column][R][size]. (With the threads along a row and G read from L2 for every four rows of W [5, 1792] . [1792,
+// 109056] bf16 took 398 us.)
+constexpr int kFewWalk = 32; // rows of W between two exchanges of the warps' sums
 template <typename T, int R, int VEC>
 __global__ void __launch_bounds__(kFewGradThreads) few_grads_kernel(const T *__restrict__ x, const T *__restrict__ w,
-                                                                const float *__restrict__ g, int64_t ldg, T *dx, T *dw,
-                                                                int count, int64_t size, int64_t classes, bool accum_dx,
-                                                                bool accum_dw, bool keep) {
-  __shared__ float sums[kFewGradThreads / 32][kFewH * R];
+                                                                    const float *__restrict__ g, int64_t ldg, bool want_dx,
+                                                                    T *dw, float *__restrict__ partial, int count,
+                                                                    int64_t size, int64_t slab, int64_t classes,
+                                                                    bool accum_dw, bool keep) {
+  constexpr int kGroups = 8 / VEC, kWarps = kFewGradThreads / 32; // groups of VEC neighbouring columns
+  __shared__ float xs[kFewWalk][R], sums[kWarps][kFewWalk][R];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t h0 = (int64_t)blockIdx.x * kFewH;
-  const int hs = (int)(size - h0 < kFewH ? size - h0 : kFewH);
-  float xv[kFewH][R], acc[kFewH][R];
+  const int64_t c0 = (int64_t)blockIdx.x * kFewGradThreads * 8 + threadIdx.x * VEC;
+  const int64_t h0 = blockIdx.y * slab, h1 = h0 + slab < size ? h0 + slab : size;
+  auto column = [&](int i) { return c0 + (int64_t)i * kFewGradThreads * VEC; }; // of group i
+  uint64_t gv[R][4];
 #pragma unroll
-  for (int h = 0; h < kFewH; ++h)
+  for (int r = 0; r < R; ++r) {
+    float f[8];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      xv[h][r] = h < hs && r < count ? to_f32(x[r * size + h0 + h]) : 0.0f;
-      acc[h][r] = 0.0f;
-    }
-  for (int64_t c = (int64_t)threadIdx.x * VEC; c < classes; c += kFewGradThreads * VEC) {
-    Pack<float, VEC> gv[R];
+    for (int i = 0; i < kGroups; ++i)
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < count)
-        gv[r] = load_pack<float, VEC>(g + r * ldg + c);
-      else
+      for (int j = 0; j < VEC; ++j)
+        f[i * VEC + j] = r < count && column(i) < classes ? g[r * ldg + column(i) + j] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          gv[r].v[j] = 0.0f;
-    Pack<T, VEC> wv[kFewH];
-    if (dx)
-#pragma unroll
-      for (int h = 0; h < kFewH; ++h)
-        if (h < hs)
-          wv[h] = load_pack_stream<T, VEC>(w + (h0 + h) * classes + c);
-#pragma unroll
-    for (int h = 0; h < kFewH; ++h) {
-      if (h >= hs)
-        continue;
-      if (dx)
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            acc[h][r] = fmaf(gv[r].v[j], wv[h].f(j), acc[h][r]);
-      if (dw) {
-        T *to = dw + (h0 + h) * classes + c;
-        float o[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          o[j] = 0.0f;
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            o[j] = fmaf(xv[h][r], gv[r].v[j], o[j]);
-        if (accum_dw) {
-          const Pack<T, VEC> old = load_pack<T, VEC>(to);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            o[j] += old.f(j);
-        }
-        store_pack<T, VEC>(to, o, keep);
-      }
-    }
+    for (int j = 0; j < 4; ++j)
+      gv[r][j] = pair_of(f[2 * j], f[2 * j + 1]);
   }
-  if (!dx)
-    return;
+  Pack<T, VEC> next[2][kGroups]; // the next two rows of W
+  auto fetch = [&](int64_t h, int to) {
 #pragma unroll
-  for (int h = 0; h < kFewH; ++h)
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float s = warp_sum(acc[h][r]);
-      if (lane == 0)
-        sums[warp][h * R + r] = s;
+    for (int i = 0; i < kGroups; ++i)
+      if (want_dx && h < h1 && column(i) < classes)
+        next[to][i] = load_pack_stream<T, VEC>(w + h * classes + column(i));
+      else
+        next[to][i].clear();
+  };
+  fetch(h0, 0);
+  fetch(h0 + 1, 1);
+  for (int64_t h = h0; h < h1; h += kFewWalk) {
+    const int n = (int)(h1 - h < kFewWalk ? h1 - h : kFewWalk);
+    for (int i = threadIdx.x; i < kFewWalk * R; i += kFewGradThreads) {
+      const int r = i / kFewWalk, k = i % kFewWalk;
+      xs[k][r] = r < count && k < n ? to_f32(x[r * size + h + k]) : 0.0f;
     }
-  __syncthreads();
-  if ((int)threadIdx.x < kFewH * R) {
-    const int h = threadIdx.x / R, r = threadIdx.x % R;
-    if (h < hs && r < count) {
-      float s = 0.0f;
+    __syncthreads();
+    auto row = [&](int k, int from) {
+      uint64_t wv[4], xv[R];
+      {
+        float f[8];
 #pragma unroll
-      for (int u = 0; u < kFewGradThreads / 32; ++u)
-        s += sums[u][threadIdx.x];
-      T *to = dx + r * size + h0 + h;
-      *to = from_f32<T>(accum_dx ? s + to_f32(*to) : s);
+        for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            f[i * VEC + j] = next[from][i].f(j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          wv[j] = pair_of(f[2 * j], f[2 * j + 1]);
+      }
+      fetch(h + k + 2, from);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        xv[r] = pair_of(xs[k][r], xs[k][r]);
+      if (dw) {
+        float o[kGroups][VEC];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint64_t t = 0;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            t = fma2(xv[r], gv[r][j], t);
+          const float2 both = unpair(t);
+          o[2 * j / VEC][2 * j % VEC] = both.x;
+          o[(2 * j + 1) / VEC][(2 * j + 1) % VEC] = both.y;
+        }
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+          if (column(i) >= classes)
+            continue;
+          T *to = dw + (h + k) * classes + column(i);
+          if (accum_dw) {
+            const Pack<T, VEC> old = load_pack<T, VEC>(to);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+              o[i][j] += old.f(j);
+          }
+          store_pack<T, VEC>(to, o[i], keep);
+        }
+      }
+      if (want_dx) {
+        float s[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          uint64_t t = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            t = fma2(gv[r][j], wv[j], t);
+          const float2 both = unpair(t);
+          s[r] = both.x + both.y;
+        }
+        int d = 16;
+#pragma unroll
+        for (int m = R / 2; m >= 1; m /= 2, d /= 2) {
+          const bool upper = lane & d;
+#pragma unroll
+          for (int r = 0; r < m; ++r) {
+            const float away = upper ? s[r] : s[r + m];
+            s[r] = (upper ? s[r + m] : s[r]) + __shfl_xor_sync(0xffffffffu, away, d);
+          }
+        }
+#pragma unroll
+        for (; d >= 1; d /= 2)
+          s[0] += __shfl_xor_sync(0xffffffffu, s[0], d);
+        if (lane % (32 / R) == 0) // lane's leading bits are the row that it ended with
+          sums[warp][k][lane / (32 / R)] = s[0];
+      }
+    };
+    for (int k = 0; k < n; k += 2) {
+      row(k, 0);
+      if (k + 1 < n)
+        row(k + 1, 1);
     }
+    __syncthreads();
+    if (want_dx)
+      for (int i = threadIdx.x; i < kFewWalk * R; i += kFewGradThreads) {
+        const int r = i / kFewWalk, k = i % kFewWalk;
+        if (k >= n || r >= count)
+          continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kWarps; ++u)
+          s += sums[u][k][r];
+        partial[((int64_t)blockIdx.x * count + r) * size + h + k] = s;
+      }
   }
 }
 

@@ -277,22 +277,26 @@ __global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThrea
 }
 
 // dx, and where kParams the sums over this block's rows of dy and dy u, each thread for the columns that it holds: a block
-// (or a warp of it, for short rows) walks over the rows, and leaves partial sums [blocks][2][size] for
-// layer_norm_param_kernel.
-template <typename T, typename P, int VEC, int NV, bool kParams>
+// (or a warp of it, for short rows; kCluster, for rows that one block does not hold: a cluster of blocks, each with `slice`
+// columns) walks over the rows, and leaves partial sums [blocks or clusters][2][size] for layer_norm_param_kernel.
+template <typename T, typename P, int VEC, int NV, bool kParams, bool kCluster>
 __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
     const T *__restrict__ x, const T *__restrict__ dy, const P *__restrict__ gamma, const float *__restrict__ mean,
     const float *__restrict__ var, T *dx, float *__restrict__ partial, int64_t rows, int size, float inv_size, float eps,
-    int row_warps, bool accum, bool keep) {
+    int row_warps, int cluster, int slice, bool accum, bool keep) {
   __shared__ alignas(16) float slots[2][2][kNormMaxWarps];
+  __shared__ float shared_sums[2][2];
   extern __shared__ float combine[]; // [warps][2][size], where a row is a warp's
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   constexpr int step = 32 * VEC; // (as in the forward kernel)
   const int at = (row_warps == 1 ? 0 : warp) * (NV * step) + lane * VEC;
-  const int64_t first = row_warps == 1 ? (int64_t)blockIdx.x * warps + warp : (int64_t)blockIdx.x;
-  const int64_t stride = row_warps == 1 ? (int64_t)gridDim.x * warps : (int64_t)gridDim.x;
+  const int64_t block = kCluster ? blockIdx.x / cluster : blockIdx.x, blocks = kCluster ? gridDim.x / cluster : gridDim.x;
+  const int64_t first = row_warps == 1 ? block * warps + warp : block, stride = row_warps == 1 ? blocks * warps : blocks;
+  // this block's columns: [col0, col0 + cols)
+  const int col0 = kCluster ? (int)(blockIdx.x - block * cluster) * slice : 0;
+  const int cols = !kCluster ? size : size - col0 < slice ? size - col0 : slice;
   float sum_dy[NV * VEC], sum_dyu[NV * VEC];
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i)
@@ -300,18 +304,18 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
   Pack<P, VEC> g[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (gamma && at + i * step < size)
-      g[i] = load_pack<P, VEC>(gamma + at + i * step);
+    if (gamma && at + i * step < cols)
+      g[i] = load_pack<P, VEC>(gamma + col0 + at + i * step);
     else
       g[i].fill(1.0f);
   // the next row is on its way while this one is summed up and stored
   Pack<T, VEC> next_x[NV], next_dy[NV];
   float next_mean = 0.0f, next_var = 0.0f;
   auto fetch = [&](int64_t row) {
-    const T *xr = x + row * size + at, *dr = dy + row * size + at;
+    const T *xr = x + row * size + col0 + at, *dr = dy + row * size + col0 + at;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (at + i * step < size) {
+      if (at + i * step < cols) {
         next_x[i] = load_pack_stream<T, VEC>(xr + i * step);
         next_dy[i] = load_pack_stream<T, VEC>(dr + i * step);
       } else { // (a dy of 0 adds nothing to any sum)
@@ -347,12 +351,14 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
     if (!dx)
       continue;
     row_sums<2>(s, row_warps, slots, turn);
+    if constexpr (kCluster)
+      cluster_sums<2>(s, shared_sums[turn], cluster); // (turn alternates: the other slot's readers have passed its barrier)
     // r (gd - m1 - u m2) as r gd + (a x + b)
     const float m1 = s[0] * inv_size, a = -r * r * (s[1] * inv_size), b = fmaf(-mu, a, -r * m1);
-    T *out = dx + row * size + at;
+    T *out = dx + row * size + col0 + at;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (at + i * step >= size)
+      if (at + i * step >= cols)
         continue;
       const int c = i * step;
       float o[VEC];
@@ -369,36 +375,39 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
     }
   }
   if constexpr (kParams) {
-    float *mine = partial + (int64_t)blockIdx.x * 2 * size;
+    float *mine = partial + block * 2 * size + col0;
     if (row_warps > 1) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          if (at + i * step + j < size) {
+          if (at + i * step + j < cols) {
             mine[at + i * step + j] = sum_dy[i * VEC + j];
             mine[size + at + i * step + j] = sum_dyu[i * VEC + j];
           }
-      return;
-    }
-    float *own = combine + (size_t)warp * 2 * size;
+    } else {
+      float *own = combine + (size_t)warp * 2 * size;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (at + i * step + j < size) {
-          own[at + i * step + j] = sum_dy[i * VEC + j];
-          own[size + at + i * step + j] = sum_dyu[i * VEC + j];
-        }
-    __syncthreads();
-    for (int c = threadIdx.x; c < 2 * size; c += blockDim.x) {
-      float s = 0.0f;
-      for (int w = 0; w < warps; ++w)
-        s += combine[(size_t)w * 2 * size + c];
-      mine[c] = s;
+        for (int j = 0; j < VEC; ++j)
+          if (at + i * step + j < size) {
+            own[at + i * step + j] = sum_dy[i * VEC + j];
+            own[size + at + i * step + j] = sum_dyu[i * VEC + j];
+          }
+      __syncthreads();
+      for (int c = threadIdx.x; c < 2 * size; c += blockDim.x) {
+        float s = 0.0f;
+        for (int w = 0; w < warps; ++w)
+          s += combine[(size_t)w * 2 * size + c];
+        mine[c] = s;
+      }
     }
   }
+  if constexpr (kCluster) // no block leaves while another may still read its sums
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+
 
 // The same sums for rows too long for the kernel above: a thread a column, a slab of rows a block, partial sums
 // [slabs][2][size].
@@ -544,7 +553,16 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
   auto run = [&](auto vec) -> int {
     constexpr int kVec = decltype(vec)::value;
     constexpr int kMaxNv = kVec == 1 ? 16 : kVec == 2 ? 8 : 4;
-    const RowShape s = row_shape(size, kVec, rows, 512, kMaxNv, kVec == 1 ? 8 : kVec == 2 ? 4 : 2);
+    const auto shape = [&](int64_t n) { return row_shape(n, kVec, rows, 512, kMaxNv, kVec == 1 ? 8 : kVec == 2 ? 4 : 2); };
+    // rows of more columns than a block holds: a cluster of up to eight
+    int cluster = 1;
+    int64_t slice = size;
+    RowShape s = shape(slice);
+    while (!s.fits && cluster < 8) {
+      cluster *= 2;
+      slice = ((size + kVec - 1) / kVec + cluster - 1) / cluster * kVec;
+      s = shape(slice);
+    }
     if (!s.fits) {
       if (params) {
         const int64_t columns = (size + 255) / 256;
@@ -563,7 +581,8 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
     }
     const int per_block = s.row_warps == 1 ? 8 : 1, threads = 32 * s.row_warps * per_block;
     // as many blocks as are resident, and then no more than their rounds need: each leaves partial sums
-    const int64_t groups = (rows + per_block - 1) / per_block, most = (int64_t)sm_count() * std::max(1, 512 / threads);
+    const int64_t groups = (rows + per_block - 1) / per_block;
+    const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() * std::max(1, 512 / threads) / cluster);
     const int64_t rounds = (groups + most - 1) / most, blocks = (groups + rounds - 1) / rounds;
     if (params) {
       parts = (int)blocks;
@@ -573,13 +592,15 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
     return with_count(s.nv, Counts{}, [&](auto nv) -> int {
       constexpr int kNv = decltype(nv)::value;
       if constexpr (kNv <= kMaxNv) {
-        auto kernel = params ? layer_norm_backward_kernel<T, P, kVec, kNv, true>
-                             : layer_norm_backward_kernel<T, P, kVec, kNv, false>;
+        auto kernel = cluster > 1 ? (params ? layer_norm_backward_kernel<T, P, kVec, kNv, true, true>
+                                            : layer_norm_backward_kernel<T, P, kVec, kNv, false, true>)
+                                  : (params ? layer_norm_backward_kernel<T, P, kVec, kNv, true, false>
+                                            : layer_norm_backward_kernel<T, P, kVec, kNv, false, false>);
         if (smem > 48 * 1024)
           NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        NB_CUDA(launch_dependent(kernel, dim3((unsigned)blocks), dim3(threads), smem, st, x, dy, gamma, mean, var, dx,
-                                 static_cast<float *>(scratch.p), rows, (int)size, 1.0f / (float)size, eps, s.row_warps,
-                                 accum_dx, keep));
+        NB_CUDA(launch_clusters(kernel, (unsigned)(blocks * cluster), cluster, threads, smem, st, x, dy, gamma, mean, var, dx,
+                                static_cast<float *>(scratch.p), rows, (int)size, 1.0f / (float)size, eps, s.row_warps, cluster,
+                                (int)slice, accum_dx, keep));
       }
       return NB200_OK;
     });

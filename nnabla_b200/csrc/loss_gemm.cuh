@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
       const int64_t ldo = p.ldo;
       const bool vec = p.vec != 0, accum = p.accum != 0, out_f32 = kF32 || p.out_f32 != 0;
       const int64_t out0 = at.split * p.stride;
-      const int chunks = (at.kb1 - at.kb0 + prob.chunk - 1) / prob.chunk; // all but the last go to registers
+      const int chunks = (at.kb1 - at.kb0 + prob.chunk - 1) / prob.chunk;
       MaxSum t{-INFINITY, 0.0f};
       if constexpr (kOut != Out::kStore)
         if (prob.bias) { // this warp's columns of it, while the tile is being made
@@ -366,173 +366,153 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
           }
           __syncwarp();
         }
-      for (int kc = 0; kc < chunks && ok; ++kc, ++local) {
-        const int buf = local & 1;
+      // What becomes of 16 columns of this thread's row, v: the h-th half of the warp's ci-th chunk of 32.
+      auto finish = [&](int ci, int h, float(&v)[16]) {
+        const int col0 = n0 + 32 * part + 32 * kParts * ci;
+        const int mine = (int)(label - prob.class0 - col0); // the label's column in this chunk, if in [0, 32)
+        const int col = col0 + 16 * h;
+        if constexpr (kOut == Out::kStore) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            v[j] *= undo;
+          if (!vec) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              stg[lane * 32 + ((16 * h + j) ^ lane)] = v[j];
+          } else if (row_ok && col < N) {
+            const int64_t off = out0 + (int64_t)row * ldo + col;
+            if (out_f32) {
+              float *out = static_cast<float *>(p.out) + off;
+              if (col + 16 > N) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  if (col + j < N)
+                    out[j] = accum ? out[j] + v[j] : v[j];
+              } else if (accum) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4)
+                  add_f32x4(out + j, v + j);
+              } else {
+                store16<float>(out, v);
+              }
+            } else if constexpr (!kF32) {
+              T *out = static_cast<T *>(p.out) + off;
+              if (col + 16 > N) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  if (col + j < N)
+                    out[j] = from_f32<T>(accum ? to_f32(out[j]) + v[j] : v[j]);
+              } else {
+                if (accum) {
+                  const Pack<T, 8> o0 = load_pack<T, 8>(out), o1 = load_pack<T, 8>(out + 8);
+#pragma unroll
+                  for (int j = 0; j < 8; ++j)
+                    v[j] += o0.f(j), v[8 + j] += o1.f(j);
+                }
+                store16<T>(out, v);
+              }
+            }
+          }
+        } else {
+          if (prob.bias)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 b = *reinterpret_cast<const float4 *>(stg + 32 * ci + 16 * h + j);
+              v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+            }
+          const int here = mine >= 16 * h && mine < 16 * h + 16 ? mine - 16 * h : -1;
+          if constexpr (kOut == Out::kSums) {
+            if (col + 16 > N)
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (col + j >= N)
+                  v[j] = -INFINITY;
+            if (here >= 0) {
+              float l = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                l = j == here ? v[j] : l;
+              rows.target[row] = l;
+            }
+            float m4[4] = {t.m, v[1], v[2], v[3]}; // four chains each, for their latency
+            m4[0] = fmaxf(m4[0], v[0]);
+#pragma unroll
+            for (int j = 4; j < 16; ++j)
+              m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+            const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            const float b = m == -INFINITY ? 0.0f : m;
+            float s4[4] = {t.s * ex2((t.m - b) * kLog2e), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              s4[j & 3] += ex2((v[j] - b) * kLog2e);
+            t = {m, (s4[0] + s4[1]) + (s4[2] + s4[3])};
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              v[j] = ex2(fmaf(v[j] - top, kLog2e, -log2_sum));
+            if (here >= 0)
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                v[j] -= j == here ? 1.0f : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              v[j] = label < 0 ? 0.0f : v[j] * factor;
+            if (row_ok) { // (G's rows are as wide as whole tiles)
+              if constexpr (kF32) {
+                __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)row * ldo + col;
+#pragma unroll
+                for (int pl = 0; pl < 3; ++pl) {
+                  store16<__nv_bfloat16>(out + pl * p.stride, v);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    v[j] = __fsub_rn(v[j], __bfloat162float(__float2bfloat16_rn(v[j])));
+                }
+              } else {
+                store16<T>(static_cast<T *>(p.out) + (int64_t)row * ldo + col, v);
+              }
+            }
+          }
+        }
+      };
+      // kStore, rows that begin anywhere: a chunk through shared memory, so that a store writes 32 neighbouring columns of a row.
+      auto flush = [&](int ci) {
+        if constexpr (kOut == Out::kStore) {
+          if (vec)
+            return;
+          const int col0 = n0 + 32 * part + 32 * kParts * ci;
+          __syncwarp();
+          const int rows_here = M - row_base < 32 ? M - row_base : 32;
+          const int64_t off = out0 + (int64_t)row_base * ldo + col0 + lane;
+          if (col0 + lane >= N)
+            return;
+          auto write = [&](auto *out) {
+            using O = std::remove_pointer_t<decltype(out)>;
+            if (accum) {
+#pragma unroll 8
+              for (int i = 0; i < rows_here; ++i, out += ldo)
+                *out = from_f32<O>(to_f32(*out) + stg[i * 32 + (lane ^ i)]);
+            } else {
+#pragma unroll 8
+              for (int i = 0; i < rows_here; ++i, out += ldo)
+                *out = from_f32<O>(stg[i * 32 + (lane ^ i)]);
+            }
+          };
+          if (out_f32)
+            write(static_cast<float *>(p.out) + off);
+          else
+            write(static_cast<T *>(p.out) + off);
+        }
+      };
+      auto wait_for = [&](int buf) {
         const bool got = ptx::mbar_wait(tmem_full + buf, (uint32_t)(local >> 1) & 1u, abort_flag);
         if (!__all_sync(0xffffffffu, got)) {
           if (lane == 0)
             gave_up(kStatusEpilogueTimeout);
           ok = false;
-          break;
         }
         ptx::tc_fence_after_sync();
-        const bool last = kc + 1 == chunks;
-#pragma unroll
-        for (int ci = 0; ci < kMyChunks; ++ci) {
-          const int c0 = 32 * part + 32 * kParts * ci, col0 = n0 + c0;
-          if (col0 >= N)
-            break;
-          const int mine = (int)(label - prob.class0 - col0); // the label's column in this chunk, if in [0, 32)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            __syncwarp(); // (the staged chunk before has been read, and the load below is the whole warp's)
-            uint32_t r[16];
-            float(&sum)[16] = acc[kLong ? 2 * ci + h : 0];
-            ptx::tmem_ld_32x16(lanes + (uint32_t)(buf * BN + c0 + 16 * h), r);
-            ptx::tmem_ld_wait();
-            if (row_base >= M)
-              continue;
-            if (kLong && !last) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                sum[j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
-              continue;
-            }
-            float v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              v[j] = !kLong || kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(sum[j], __uint_as_float(r[j]));
-            const int col = col0 + 16 * h;
-            if constexpr (kOut == Out::kStore) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                v[j] *= undo;
-              if (!vec) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  stg[lane * 32 + ((16 * h + j) ^ lane)] = v[j];
-              } else if (row_ok && col < N) {
-                const int64_t off = out0 + (int64_t)row * ldo + col;
-                if (out_f32) {
-                  float *out = static_cast<float *>(p.out) + off;
-                  if (col + 16 > N) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                      if (col + j < N)
-                        out[j] = accum ? out[j] + v[j] : v[j];
-                  } else if (accum) {
-#pragma unroll
-                    for (int j = 0; j < 16; j += 4)
-                      add_f32x4(out + j, v + j);
-                  } else {
-                    store16<float>(out, v);
-                  }
-                } else if constexpr (!kF32) {
-                  T *out = static_cast<T *>(p.out) + off;
-                  if (col + 16 > N) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                      if (col + j < N)
-                        out[j] = from_f32<T>(accum ? to_f32(out[j]) + v[j] : v[j]);
-                  } else {
-                    if (accum) {
-                      const Pack<T, 8> o0 = load_pack<T, 8>(out), o1 = load_pack<T, 8>(out + 8);
-#pragma unroll
-                      for (int j = 0; j < 8; ++j)
-                        v[j] += o0.f(j), v[8 + j] += o1.f(j);
-                    }
-                    store16<T>(out, v);
-                  }
-                }
-              }
-            } else {
-              if (prob.bias)
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                  const float4 b = *reinterpret_cast<const float4 *>(stg + 32 * ci + 16 * h + j);
-                  v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
-                }
-              const int here = mine >= 16 * h && mine < 16 * h + 16 ? mine - 16 * h : -1;
-              if constexpr (kOut == Out::kSums) {
-                if (col + 16 > N)
-#pragma unroll
-                  for (int j = 0; j < 16; ++j)
-                    if (col + j >= N)
-                      v[j] = -INFINITY;
-                if (here >= 0) {
-                  float l = 0.0f;
-#pragma unroll
-                  for (int j = 0; j < 16; ++j)
-                    l = j == here ? v[j] : l;
-                  rows.target[row] = l;
-                }
-                float m4[4] = {t.m, v[1], v[2], v[3]}; // four chains each, for their latency
-                m4[0] = fmaxf(m4[0], v[0]);
-#pragma unroll
-                for (int j = 4; j < 16; ++j)
-                  m4[j & 3] = fmaxf(m4[j & 3], v[j]);
-                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                const float b = m == -INFINITY ? 0.0f : m;
-                float s4[4] = {t.s * ex2((t.m - b) * kLog2e), 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  s4[j & 3] += ex2((v[j] - b) * kLog2e);
-                t = {m, (s4[0] + s4[1]) + (s4[2] + s4[3])};
-              } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  v[j] = ex2(fmaf(v[j] - top, kLog2e, -log2_sum));
-                if (here >= 0)
-#pragma unroll
-                  for (int j = 0; j < 16; ++j)
-                    v[j] -= j == here ? 1.0f : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  v[j] = label < 0 ? 0.0f : v[j] * factor;
-                if (row_ok) { // (G's rows are as wide as whole tiles)
-                  if constexpr (kF32) {
-                    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)row * ldo + col;
-#pragma unroll
-                    for (int pl = 0; pl < 3; ++pl) {
-                      store16<__nv_bfloat16>(out + pl * p.stride, v);
-#pragma unroll
-                      for (int j = 0; j < 16; ++j)
-                        v[j] = __fsub_rn(v[j], __bfloat162float(__float2bfloat16_rn(v[j])));
-                    }
-                  } else {
-                    store16<T>(static_cast<T *>(p.out) + (int64_t)row * ldo + col, v);
-                  }
-                }
-              }
-            }
-          }
-          if constexpr (kOut == Out::kStore) {
-            if (vec || !last || row_base >= M)
-              continue;
-            // rows that begin anywhere: through shared memory, so that a store writes 32 neighbouring columns of a row
-            __syncwarp();
-            const int rows_here = M - row_base < 32 ? M - row_base : 32;
-            const int64_t off = out0 + (int64_t)row_base * ldo + col0 + lane;
-            if (col0 + lane >= N)
-              continue;
-            auto write = [&](auto *out) {
-              using O = std::remove_pointer_t<decltype(out)>;
-              if (accum) {
-#pragma unroll 8
-                for (int i = 0; i < rows_here; ++i, out += ldo)
-                  *out = from_f32<O>(to_f32(*out) + stg[i * 32 + (lane ^ i)]);
-              } else {
-#pragma unroll 8
-                for (int i = 0; i < rows_here; ++i, out += ldo)
-                  *out = from_f32<O>(stg[i * 32 + (lane ^ i)]);
-              }
-            };
-            if (out_f32)
-              write(static_cast<float *>(p.out) + off);
-            else
-              write(static_cast<T *>(p.out) + off);
-          }
-        }
+      };
+      auto release = [&](int buf) {
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
@@ -541,6 +521,65 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
           else
             ptx::mbar_arrive(tmem_empty + buf);
         }
+      };
+      if constexpr (kLong) {
+        // every chunk of K to registers, the last one too: tensor memory is free again while the sums are worked on
+        for (int kc = 0; kc < chunks; ++kc, ++local) {
+          const int buf = local & 1;
+          wait_for(buf);
+          if (!ok)
+            break;
+#pragma unroll
+          for (int i = 0; i < 2 * kMyChunks; ++i) {
+            const int c = 32 * part + 32 * kParts * (i / 2) + 16 * (i & 1);
+            if (n0 + c >= N)
+              break;
+            uint32_t r[16];
+            ptx::tmem_ld_32x16(lanes + (uint32_t)(buf * BN + c), r);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              acc[i][j] = kc == 0 ? __uint_as_float(r[j]) : __fadd_rn(acc[i][j], __uint_as_float(r[j]));
+          }
+          release(buf);
+        }
+        if (ok && row_base < M) {
+#pragma unroll
+          for (int ci = 0; ci < kMyChunks; ++ci) {
+            if (n0 + 32 * part + 32 * kParts * ci >= N)
+              break;
+            __syncwarp(); // (the staged chunk before has been read)
+            finish(ci, 0, acc[2 * ci]);
+            finish(ci, 1, acc[2 * ci + 1]);
+            flush(ci);
+          }
+        }
+      } else {
+        const int buf = local & 1;
+        wait_for(buf);
+        if (!ok)
+          break;
+#pragma unroll
+        for (int ci = 0; ci < kMyChunks; ++ci) {
+          const int c = 32 * part + 32 * kParts * ci;
+          if (n0 + c >= N || row_base >= M)
+            break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            __syncwarp(); // (the staged chunk before has been read, and the load is the whole warp's)
+            uint32_t r[16];
+            ptx::tmem_ld_32x16(lanes + (uint32_t)(buf * BN + c + 16 * h), r);
+            ptx::tmem_ld_wait();
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              v[j] = __uint_as_float(r[j]);
+            finish(ci, h, v);
+          }
+          flush(ci);
+        }
+        release(buf);
+        ++local;
       }
       if constexpr (kOut == Out::kSums)
         if (ok && row_ok)
