@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *__restrict_
       const Pack<float, V> f = load_pack<float, V>(from + p * stride + r * ldf + c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        s[j] += f.v[j];
+        s[j] += f.f(j);
     }
     T *t = to + r * ldt + c;
     Pack<T, V> old;
@@ -202,19 +202,25 @@ template <typename T> __global__ void __launch_bounds__(256) loss_prepare_kernel
     if (vec && c + 8 <= m.cols) {
       v = load_pack<T, 8>(src);
     } else {
+      v.clear();
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        v.v[j] = c + j < m.cols ? src[j] : from_f32<T>(0.0f);
+        if (c + j < m.cols)
+          v.set(j, src[j]);
     }
     if constexpr (std::is_same<T, float>::value) {
       __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(m.to) + r * m.pitch + c;
+      float left[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        left[j] = v.f(j);
 #pragma unroll
       for (int pl = 0; pl < 3; ++pl) {
-        const Pack<__nv_bfloat16, 8> h = round_pack<__nv_bfloat16, 8>(v.v);
+        const Pack<__nv_bfloat16, 8> h = round_pack<__nv_bfloat16, 8>(left);
         *reinterpret_cast<Pack<__nv_bfloat16, 8> *>(to + pl * m.rows * m.pitch) = h;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          v.v[j] = __fsub_rn(v.v[j], h.f(j));
+          left[j] = __fsub_rn(left[j], h.f(j));
       }
     } else {
       *reinterpret_cast<Pack<T, 8> *>(static_cast<T *>(m.to) + r * m.pitch + c) = v;

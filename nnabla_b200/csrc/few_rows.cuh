@@ -27,11 +27,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 constexpr int kFewBatch = 4, kFewBatches = 3;                         // packs a batch of copies, batches on the way
 constexpr int kFewRing = kFewBatch * kFewBatches * kFewThreads * 16; // bytes
 
-__device__ __forceinline__ void cp_async16(void *to, const void *from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to)), "l"(from) : "memory");
-}
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <typename T, int VEC> constexpr int few_lanes() { return VEC * sizeof(T) == 16 ? 16 : 32; }
 // Shared memory in front of x: the ring, or in its place the warps' sums.
 template <typename T, int R, int VEC> constexpr int few_fixed_bytes() {
@@ -85,7 +80,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
       for (int u = 0; u < kFewBatch; ++u, next += kStep)
         if (here && next < kb)
           cp_async16(&ring[at + u][threadIdx.x], w + next * classes + c);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      cp_async_commit();
     }
   };
   for (int i = 0; i < kFewBatches; ++i)

@@ -55,34 +55,132 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int row_warps, float (*s
   }
 }
 
-// VEC values an access, NV accesses a thread; a row belongs to row_warps warps, and a block holds one row or (row_warps == 1)
-// a row a warp; ROWS such rows at once, for which one barrier serves and one look at the parameters.
-template <typename T, typename P, int VEC, int NV, int ROWS>
-__global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ x, const P *__restrict__ beta,
-                                                          const P *__restrict__ gamma, T *y, float *__restrict__ mean_out,
-                                                          float *__restrict__ var_out, int64_t rows, int size,
-                                                          float inv_size, float eps, int row_warps, bool keep) {
+// Sums over the blocks of a cluster: each leaves its own in its shared memory and reads the others'. Fixed order.
+template <int N> __device__ __forceinline__ void cluster_sums(float (&v)[N], float *slot, int blocks) {
+  // (all threads hold the block's sums; slot: N floats of shared memory, not used again before the next cluster barrier)
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      slot[i] = v[i];
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // every warp for itself, a lane a block
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float f = 0.0f;
+    if (lane < blocks) {
+      const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(slot + i));
+      uint32_t theirs;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(lane));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(theirs) : "memory");
+    }
+    v[i] = warp_sum(f);
+  }
+}
+
+// A thread's part of a row: NV accesses of VEC values, a warp's side by side, so that their offsets are constants. kShift: the
+// row begins `shift` values behind a 16-byte boundary (sizes that are no multiple of VEC), and the accesses lie on the
+// boundaries; those across the row's ends go value by value. Column of access i: first + i * kStep.
+template <int VEC, bool kShift> struct Columns {
+  static constexpr int kStep = 32 * VEC;
+  int first, end; // of the row (or the block's slice of it): [begin, end)
+  int begin;
+  __device__ __forceinline__ int at(int i) const { return first + i * kStep; }
+  __device__ __forceinline__ bool full(int i) const {
+    return kShift ? at(i) >= begin && at(i) + VEC <= end : at(i) < end;
+  }
+  __device__ __forceinline__ bool some(int i) const { return kShift ? at(i) + VEC > begin && at(i) < end : at(i) < end; }
+  __device__ __forceinline__ bool has(int i, int j) const { return !kShift || (at(i) + j >= begin && at(i) + j < end); }
+  // `mine` below: the row, or the parameters, plus `first`, so that the accesses have constant offsets from one address.
+  // values that the row does not have: 0
+  template <typename T, bool kStream> __device__ __forceinline__ Pack<T, VEC> load(const T *mine, int i) const {
+    Pack<T, VEC> p;
+    if (full(i)) {
+      if constexpr (kStream)
+        p = load_pack_stream<T, VEC>(mine + i * kStep);
+      else
+        p = load_pack<T, VEC>(mine + i * kStep);
+    } else {
+      p.clear();
+      if (kShift && some(i))
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (has(i, j))
+            p.set(j, mine[i * kStep + j]);
+    }
+    return p;
+  }
+  // of a parameter, whose columns are not aligned with the row's where kShift
+  template <typename P> __device__ __forceinline__ Pack<P, VEC> parameter(const P *mine, int i, bool given, float none) const {
+    Pack<P, VEC> p;
+    if (!given) {
+      p.fill(none); // (once, not chosen at every value)
+    } else if constexpr (!kShift) {
+      if (full(i))
+        p = load_pack<P, VEC>(mine + i * kStep);
+      else
+        p.clear();
+    } else {
+      p.clear();
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (has(i, j))
+          p.set(j, mine[i * kStep + j]);
+    }
+    return p;
+  }
+  template <typename T> __device__ __forceinline__ void store(T *mine, int i, const float (&v)[VEC], bool keep) const {
+    if (full(i)) {
+      store_pack<T, VEC>(mine + i * kStep, v, keep);
+    } else if (kShift && some(i)) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (has(i, j))
+          mine[i * kStep + j] = from_f32<T>(v[j]);
+    }
+  }
+};
+// The columns of this thread in a row that begins `shift` values behind a boundary; rank: of a cluster's blocks, slice of it.
+template <int VEC, int NV, bool kShift>
+__device__ __forceinline__ Columns<VEC, kShift> columns_of(int warp, int lane, int size, int shift, int rank, int slice) {
+  Columns<VEC, kShift> c;
+  const int from = rank * slice - (kShift ? shift : 0); // in front of the row for the first block
+  c.first = from + warp * (NV * 32 * VEC) + lane * VEC;
+  c.begin = from > 0 ? from : 0;
+  c.end = size - from < slice ? size : from + slice;
+  return c;
+}
+template <int VEC> __device__ __forceinline__ int shift_of(int64_t row, int size) { return (int)(row * size) & (VEC - 1); }
+
+// A row belongs to row_warps warps: a block holds one row, or (row_warps == 1) a row a warp, or (kCluster) a slice of a row; ROWS
+// such rows at once, for which one barrier serves and one look at the parameters.
+template <typename T, typename P, int VEC, int NV, int ROWS, bool kShift, bool kCluster>
+__global__ void __launch_bounds__(512, 2) layer_norm_kernel(const T *__restrict__ x, const P *__restrict__ beta,
+                                                         const P *__restrict__ gamma, T *y, float *__restrict__ mean_out,
+                                                         float *__restrict__ var_out, int64_t rows, int size, float inv_size,
+                                                         float eps, int row_warps, int cluster, int slice, bool keep) {
+  static_assert(ROWS == 1 || !(kShift || kCluster), "rows of one block begin alike");
   __shared__ alignas(16) float slots[2][ROWS][kNormMaxWarps];
+  __shared__ float shared_sums[2][1];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = ((row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x)) * ROWS;
+  const int64_t block = kCluster ? blockIdx.x / cluster : blockIdx.x;
+  const int64_t row = (row_warps == 1 ? block * (blockDim.x >> 5) + warp : block) * ROWS;
   if (row >= rows) // (whole warps, and never where the block shares a row)
     return;
-  // a warp's accesses lie side by side: constant offsets from one address
-  constexpr int step = 32 * VEC;
-  const int at = (row_warps == 1 ? 0 : warp) * (NV * step) + lane * VEC;
   const int here = rows - row < ROWS ? (int)(rows - row) : ROWS;
+  const auto cols = columns_of<VEC, NV, kShift>(row_warps == 1 ? 0 : warp, lane, size, shift_of<VEC>(row, size),
+                                                kCluster ? (int)(blockIdx.x - block * cluster) : 0, kCluster ? slice : size + VEC);
   float v[ROWS][NV][VEC];
   {
     Pack<T, VEC> p[ROWS][NV];
-    const T *xr = x + row * size + at;
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (q < here && at + i * step < size)
-          p[q][i] = load_pack_stream<T, VEC>(xr + (int64_t)q * size + i * step);
+        if (q < here)
+          p[q][i] = cols.template load<T, true>(x + (row + q) * size + cols.first, i);
         else
           p[q][i].clear();
 #pragma unroll
@@ -105,26 +203,36 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
         mean[q] += v[q][i][j];
   }
   row_sums<ROWS>(mean, row_warps, slots, turn);
+  if constexpr (kCluster)
+    cluster_sums<1>(mean, shared_sums[0], cluster);
 #pragma unroll
   for (int q = 0; q < ROWS; ++q) {
     mean[q] *= inv_size;
     r[q] = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float m = at + i * step < size ? mean[q] : 0.0f;
+      const float m = cols.full(i) ? mean[q] : 0.0f;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
+      for (int j = 0; j < VEC; ++j)
         v[q][i][j] -= m;
+      if (kShift && !cols.full(i) && cols.some(i))
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          v[q][i][j] -= cols.has(i, j) ? mean[q] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
         r[q] = fmaf(v[q][i][j], v[q][i][j], r[q]);
-      }
     }
   }
   row_sums<ROWS>(r, row_warps, slots, turn);
+  if constexpr (kCluster)
+    cluster_sums<1>(r, shared_sums[1], cluster);
+  const bool first = kCluster ? threadIdx.x == 0 && blockIdx.x == block * cluster : row_warps == 1 ? lane == 0 : threadIdx.x == 0;
 #pragma unroll
   for (int q = 0; q < ROWS; ++q) {
     const float var = r[q] * inv_size;
     r[q] = rsqrtf(var + eps);
-    if (at == 0 && q < here) {
+    if (first && q < here) {
       if (mean_out)
         mean_out[row + q] = mean[q];
       if (var_out)
@@ -133,18 +241,10 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = at + i * step;
-    if (c >= size)
+    if (!cols.some(i))
       continue;
-    Pack<P, VEC> g, b; // (none: filled once, not chosen at every value)
-    if (gamma)
-      g = load_pack<P, VEC>(gamma + c);
-    else
-      g.fill(1.0f);
-    if (beta)
-      b = load_pack<P, VEC>(beta + c);
-    else
-      b.clear();
+    const Pack<P, VEC> g = cols.template parameter<P>(gamma + cols.first, i, gamma != nullptr, 1.0f);
+    const Pack<P, VEC> b = cols.template parameter<P>(beta + cols.first, i, beta != nullptr, 0.0f);
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       if (q >= here)
@@ -153,32 +253,11 @@ __global__ void __launch_bounds__(1024) layer_norm_kernel(const T *__restrict__ 
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
         o[j] = fmaf(v[q][i][j] * r[q], g.f(j), b.f(j));
-      store_pack<T, VEC>(y + (row + q) * size + at + i * step, o, keep);
+      cols.store(y + (row + q) * size + cols.first, i, o, keep);
     }
   }
-}
-
-// Sums over the blocks of a cluster: each leaves its own in its shared memory and reads the others'. Fixed order.
-template <int N> __device__ __forceinline__ void cluster_sums(float (&v)[N], float *slot, int blocks) {
-  // (all threads hold the block's sums; slot: N floats of shared memory, not used again before the next cluster barrier)
-  if (threadIdx.x == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      slot[i] = v[i];
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    v[i] = 0.0f;
-  for (int b = 0; b < blocks; ++b)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(slot + i));
-      uint32_t theirs;
-      float f;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(b));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(theirs) : "memory");
-      v[i] += f;
-    }
+  if constexpr (kCluster) // no block leaves while another may still read its sums
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 constexpr int kLongThreads = 512, kLongBlocks = 8;
@@ -276,10 +355,13 @@ __global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThrea
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// dx, and where kParams the sums over this block's rows of dy and dy u, each thread for the columns that it holds: a block
-// (or a warp of it, for short rows; kCluster, for rows that one block does not hold: a cluster of blocks, each with `slice`
-// columns) walks over the rows, and leaves partial sums [blocks or clusters][2][size] for layer_norm_param_kernel.
-template <typename T, typename P, int VEC, int NV, bool kParams, bool kCluster>
+// dx, and where kParams the sums over this block's rows of dy and dy u, each thread for the columns that it holds: a block (or
+// a warp of it, for short rows) walks over the rows, and leaves partial sums [blocks][2][size] for layer_norm_param_kernel.
+// kShift: the rows that a block walks over are VEC or a multiple of it apart, so that all begin alike. kCluster, for rows that
+// one block does not hold: a cluster of blocks, each with a slice of the columns, takes one row (dx only).
+// The next row of x and dy is on its way in registers while one is worked on (three rows in asynchronous copies to shared memory
+// take no less: a row costs a warp 150 to 250 instructions beside those of its values, and those are what bounds it).
+template <typename T, typename P, int VEC, int NV, bool kParams, bool kShift, bool kCluster>
 __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
     const T *__restrict__ x, const T *__restrict__ dy, const P *__restrict__ gamma, const float *__restrict__ mean,
     const float *__restrict__ var, T *dx, float *__restrict__ partial, int64_t rows, int size, float inv_size, float eps,
@@ -290,13 +372,10 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  constexpr int step = 32 * VEC; // (as in the forward kernel)
-  const int at = (row_warps == 1 ? 0 : warp) * (NV * step) + lane * VEC;
   const int64_t block = kCluster ? blockIdx.x / cluster : blockIdx.x, blocks = kCluster ? gridDim.x / cluster : gridDim.x;
   const int64_t first = row_warps == 1 ? block * warps + warp : block, stride = row_warps == 1 ? blocks * warps : blocks;
-  // this block's columns: [col0, col0 + cols)
-  const int col0 = kCluster ? (int)(blockIdx.x - block * cluster) * slice : 0;
-  const int cols = !kCluster ? size : size - col0 < slice ? size - col0 : slice;
+  const auto cols = columns_of<VEC, NV, kShift>(row_warps == 1 ? 0 : warp, lane, size, shift_of<VEC>(first, size),
+                                                kCluster ? (int)(blockIdx.x - block * cluster) : 0, kCluster ? slice : size + VEC);
   float sum_dy[NV * VEC], sum_dyu[NV * VEC];
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i)
@@ -304,24 +383,16 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
   Pack<P, VEC> g[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (gamma && at + i * step < cols)
-      g[i] = load_pack<P, VEC>(gamma + col0 + at + i * step);
-    else
-      g[i].fill(1.0f);
-  // the next row is on its way while this one is summed up and stored
+    g[i] = cols.template parameter<P>(gamma + cols.first, i, gamma != nullptr, 1.0f);
   Pack<T, VEC> next_x[NV], next_dy[NV];
   float next_mean = 0.0f, next_var = 0.0f;
   auto fetch = [&](int64_t row) {
-    const T *xr = x + row * size + col0 + at, *dr = dy + row * size + col0 + at;
+    const T *xr = x + row * size + cols.first, *dr = dy + row * size + cols.first;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (at + i * step < cols) {
-        next_x[i] = load_pack_stream<T, VEC>(xr + i * step);
-        next_dy[i] = load_pack_stream<T, VEC>(dr + i * step);
-      } else { // (a dy of 0 adds nothing to any sum)
-        next_x[i].clear();
-        next_dy[i].clear();
-      }
+    for (int i = 0; i < NV; ++i) { // (beyond the row a dy of 0 adds nothing to any sum)
+      next_x[i] = cols.template load<T, true>(xr, i);
+      next_dy[i] = cols.template load<T, true>(dr, i);
+    }
     next_mean = mean[row], next_var = var[row];
   };
   if (first < rows)
@@ -355,46 +426,36 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
       cluster_sums<2>(s, shared_sums[turn], cluster); // (turn alternates: the other slot's readers have passed its barrier)
     // r (gd - m1 - u m2) as r gd + (a x + b)
     const float m1 = s[0] * inv_size, a = -r * r * (s[1] * inv_size), b = fmaf(-mu, a, -r * m1);
-    T *out = dx + row * size + col0 + at;
+    T *out = dx + row * size + cols.first;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (at + i * step >= cols)
+      if (!cols.some(i))
         continue;
-      const int c = i * step;
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
         o[j] = fmaf(dv[i].f(j) * g[i].f(j), r, fmaf(xv[i].f(j), a, b));
       if (accum) {
-        const Pack<T, VEC> old = load_pack<T, VEC>(out + c);
+        const Pack<T, VEC> old = cols.template load<T, false>(out, i);
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
           o[j] += old.f(j);
       }
-      store_pack<T, VEC>(out + c, o, keep);
+      cols.store(out, i, o, keep);
     }
   }
   if constexpr (kParams) {
-    float *mine = partial + block * 2 * size + col0;
-    if (row_warps > 1) {
+    float *mine = partial + block * 2 * size, *own = row_warps > 1 ? mine : combine + (size_t)warp * 2 * size;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (at + i * step + j < cols) {
-            mine[at + i * step + j] = sum_dy[i * VEC + j];
-            mine[size + at + i * step + j] = sum_dyu[i * VEC + j];
-          }
-    } else {
-      float *own = combine + (size_t)warp * 2 * size;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i)
+      if (cols.some(i))
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          if (at + i * step + j < size) {
-            own[at + i * step + j] = sum_dy[i * VEC + j];
-            own[size + at + i * step + j] = sum_dyu[i * VEC + j];
+          if (cols.has(i, j)) {
+            own[cols.at(i) + j] = sum_dy[i * VEC + j];
+            own[size + cols.at(i) + j] = sum_dyu[i * VEC + j];
           }
+    if (row_warps == 1) {
       __syncthreads();
       for (int c = threadIdx.x; c < 2 * size; c += blockDim.x) {
         float s = 0.0f;
@@ -407,7 +468,6 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
   if constexpr (kCluster) // no block leaves while another may still read its sums
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-
 
 // The same sums for rows too long for the kernel above: a thread a column, a slab of rows a block, partial sums
 // [slabs][2][size].
@@ -434,60 +494,67 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const T *__rest
   partial[(int64_t)blockIdx.y * 2 * size + size + c] = b;
 }
 
-// dbeta (+)= sum over the parts of [part][0][c], dgamma of [part][1][c], in a fixed order: a block takes 32 columns, its 32
-// warps the parts in turn.
+// dbeta (+)= sum over the parts of [part][0][c], dgamma of [part][1][c], in a fixed order: `share` of a block's 32 warps take the
+// parts of 32 columns in turn.
 template <typename P>
-__global__ void __launch_bounds__(1024) layer_norm_param_kernel(const float *__restrict__ partial, int parts, int64_t size,
-                                                               P *dbeta, P *dgamma, bool accum_beta, bool accum_gamma) {
+__global__ void __launch_bounds__(1024) layer_norm_param_kernel(const float *__restrict__ partial, int parts, int share,
+                                                                int64_t size, P *dbeta, P *dgamma, bool accum_beta,
+                                                                bool accum_gamma) {
   __shared__ float sums[32][33];
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % share;
   P *out = blockIdx.y == 0 ? dbeta : dgamma;
   if (!out)
     return;
   const bool accum = blockIdx.y == 0 ? accum_beta : accum_gamma;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = ((int64_t)blockIdx.x * (32 / share) + warp / share) * 32 + lane;
   float s = 0.0f;
   if (c < size) {
     const float *p = partial + (int64_t)blockIdx.y * size + c;
 #pragma unroll 8
-    for (int k = warp; k < parts; k += 32)
+    for (int k = mine; k < parts; k += share)
       s += p[(int64_t)k * 2 * size];
   }
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && c < size) {
-    s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 32; ++w)
-      s += sums[w][lane];
+  if (mine == 0 && c < size) {
+    for (int w = 1; w < share; ++w)
+      s += sums[warp + w][lane];
     if (accum)
       s += to_f32(out[c]);
     out[c] = from_f32<P>(s);
   }
 }
 
-// Threads of a row and accesses of a thread. Rows of up to four accesses a lane are a warp's (no barrier); longer ones a
-// block's, with `want` accesses a thread where the rows are enough to fill the SMs and one where they are few.
+// Threads of a row, accesses of a thread, and blocks of a cluster that share a row. Rows of up to four accesses a lane are a
+// warp's (no barrier); longer ones a block's, with `want` accesses a thread where the rows are enough to fill the SMs and one
+// where they are few, and of up to eight blocks where one does not hold them in registers, or where the rows leave SMs idle.
 struct RowShape {
-  int row_warps, nv;
+  int row_warps, nv, cluster;
+  int64_t slice; // columns of a cluster's block
   bool fits;
 };
-RowShape row_shape(int64_t size, int vec, int64_t rows, int max_threads, int max_nv, int want) {
-  const int64_t packs = (size + vec - 1) / vec;
+RowShape row_shape(int64_t size, int vec, bool shift, int64_t rows, int max_nv, int want) {
+  const int64_t packs = (size + (shift ? vec - 1 : 0) + vec - 1) / vec;
   if (packs <= 32)
-    return {1, 1, true};
+    return {1, 1, 1, 0, true};
   const bool few = rows < 2 * sm_count();
-  if (packs <= 128 && !few)
-    return {1, packs <= 64 ? 2 : 4, true};
+  if (packs <= 32 * std::min(4, max_nv) && !few)
+    return {1, packs <= 64 ? 2 : 4, 1, 0, true};
+  // (in a cluster 256 threads a block: several rows an SM hide the latency of their barriers)
+  const int64_t most = packs > 512 * max_nv ? 256 * max_nv : 512 * max_nv;
+  int cluster = 1;
+  while (cluster < 8 && ((packs + cluster - 1) / cluster > most || (rows * cluster < sm_count() && packs >= 1024 * cluster)))
+    cluster *= 2;
+  const int64_t each = (packs + cluster - 1) / cluster;
   int threads = 128;
-  while (threads < max_threads && (int64_t)threads * (few ? 1 : want) < packs)
+  while (threads < 512 && (int64_t)threads * (few ? 1 : want) < each)
     threads *= 2;
   int nv = 1;
-  while (nv < max_nv && (int64_t)threads * nv < packs)
+  while (nv < max_nv && (int64_t)threads * nv < each)
     nv *= 2;
-  return {threads / 32, nv, (int64_t)threads * nv >= packs};
+  return {threads / 32, nv, cluster, each * vec, (int64_t)threads * nv >= each};
 }
 
 template <int... N, typename F> int with_count(int n, std::integer_sequence<int, N...>, F f) {
@@ -495,7 +562,7 @@ template <int... N, typename F> int with_count(int n, std::integer_sequence<int,
   ((n == N ? (rc = f(std::integral_constant<int, N>{}), 0) : 0), ...);
   return rc;
 }
-using Counts = std::integer_sequence<int, 1, 2, 4, 8, 16, 32>;
+using Counts = std::integer_sequence<int, 1, 2, 4, 8, 16>;
 
 int check_sizes(int64_t rows, int64_t size, int64_t per_row_blocks) {
   NB_CHECK(size > 0, NB200_EVALUE, "an empty row has no mean");
@@ -504,44 +571,55 @@ int check_sizes(int64_t rows, int64_t size, int64_t per_row_blocks) {
   return NB200_OK;
 }
 
+// How rows are accessed: 16 bytes at a time, from boundaries in front of the rows where their size is no multiple of that, or
+// (tensors that begin off a boundary) value by value.
+template <typename T, typename F> int with_access(int64_t size, bool aligned_rows, bool aligned_params, F f) {
+  if (!aligned_rows || (size % kPackOf<T> == 0 && !aligned_params))
+    return f(std::integral_constant<int, 1>{}, std::false_type{});
+  return size % kPackOf<T> == 0 ? f(std::integral_constant<int, kPackOf<T>>{}, std::false_type{})
+                                : f(std::integral_constant<int, kPackOf<T>>{}, std::true_type{});
+}
+
 template <typename T, typename P>
 int forward(const T *x, const P *beta, const P *gamma, T *y, float *mean, float *var, int64_t rows, int64_t size, float eps,
             cudaStream_t st) {
   const bool keep = (size_t)rows * size * sizeof(T) <= kKeepBytes;
-  auto run = [&](auto vec) -> int {
-    constexpr int kVec = decltype(vec)::value;
-    constexpr int kMaxNv = kVec == 1 ? 32 : kVec == 2 ? 16 : 8;
-    const RowShape s = row_shape(size, kVec, rows, 1024, kMaxNv, kVec == 1 ? 8 : 4);
-    if (!s.fits || (rows <= sm_count() / kLongBlocks && size >= 32768)) {
+  return with_access<T>(size, aligned16(x) && aligned16(y), aligned16(gamma) && aligned16(beta), [&](auto vec, auto shift) -> int {
+    constexpr int kVec = decltype(vec)::value, kMaxNv = kVec == 1 ? 16 : kVec == 4 ? 8 : 4;
+    constexpr bool kShift = decltype(shift)::value;
+    const RowShape s = row_shape(size, kVec, kShift, rows, kMaxNv, kVec == 1 ? 8 : 4);
+    if (!s.fits) {
       NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, false>, dim3((unsigned)(rows * kLongBlocks)), dim3(kLongThreads),
                                0, st, x, (const T *)nullptr, beta, gamma, y, mean, var, size, eps, false));
       return NB200_OK;
     }
     const int per_block = s.row_warps == 1 ? 4 : 1;
-    // two rows at once where that leaves enough blocks
     return with_count(s.nv, Counts{}, [&](auto nv) -> int {
       constexpr int kNv = decltype(nv)::value;
-      auto launch = [&](auto count) -> int {
+      auto launch = [&](auto count, auto clustered) -> int {
         constexpr int kRows = decltype(count)::value;
         const int64_t blocks = (rows + per_block * kRows - 1) / (per_block * kRows);
-        NB_CUDA(launch_dependent(layer_norm_kernel<T, P, kVec, kNv, kRows>, dim3((unsigned)blocks),
-                                 dim3(32 * s.row_warps * per_block), 0, st, x, beta, gamma, y, mean, var, rows, (int)size,
-                                 1.0f / (float)size, eps, s.row_warps, keep));
+        auto kernel = layer_norm_kernel<T, P, kVec, kNv, kRows, kShift, decltype(clustered)::value>;
+        const int threads = 32 * s.row_warps * per_block;
+        if (decltype(clustered)::value)
+          NB_CUDA(launch_clusters(kernel, (unsigned)(blocks * s.cluster), s.cluster, threads, 0, st, x, beta, gamma, y, mean, var,
+                                  rows, (int)size, 1.0f / (float)size, eps, s.row_warps, s.cluster, (int)s.slice, keep));
+        else
+          NB_CUDA(launch_dependent(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, x, beta, gamma, y, mean, var, rows,
+                                   (int)size, 1.0f / (float)size, eps, s.row_warps, 1, 0, keep));
         return NB200_OK;
       };
-      if constexpr (kVec * kNv <= 16)
-        if (rows / per_block >= 64 * sm_count())
-          return launch(std::integral_constant<int, 2>{});
-      if constexpr (kNv <= kMaxNv)
-        return launch(std::integral_constant<int, 1>{});
+      if constexpr (kNv <= kMaxNv) {
+        if (s.cluster > 1)
+          return launch(std::integral_constant<int, 1>{}, std::true_type{});
+        if constexpr (!kShift && kVec * kNv <= 16)
+          if (rows / per_block >= 64 * sm_count()) // two rows at once where that leaves enough blocks
+            return launch(std::integral_constant<int, 2>{}, std::false_type{});
+        return launch(std::integral_constant<int, 1>{}, std::false_type{});
+      }
       return NB200_EVALUE;
     });
-  };
-  const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(beta);
-  const bool pairs = size % 2 == 0 && aligned8(x) && aligned8(y) && aligned8(gamma) && aligned8(beta);
-  return vec     ? run(std::integral_constant<int, kPackOf<T>>{})
-         : pairs ? run(std::integral_constant<int, 2>{})
-                 : run(std::integral_constant<int, 1>{});
+  });
 }
 
 template <typename T, typename P>
@@ -550,71 +628,77 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
   const bool params = dbeta || dgamma, keep = (size_t)rows * size * sizeof(T) <= kKeepBytes;
   AsyncScratch scratch(st);
   int parts = 0;
-  auto run = [&](auto vec) -> int {
-    constexpr int kVec = decltype(vec)::value;
-    constexpr int kMaxNv = kVec == 1 ? 16 : kVec == 2 ? 8 : 4;
-    const auto shape = [&](int64_t n) { return row_shape(n, kVec, rows, 512, kMaxNv, kVec == 1 ? 8 : kVec == 2 ? 4 : 2); };
-    // rows of more columns than a block holds: a cluster of up to eight
-    int cluster = 1;
-    int64_t slice = size;
-    RowShape s = shape(slice);
-    while (!s.fits && cluster < 8) {
-      cluster *= 2;
-      slice = ((size + kVec - 1) / kVec + cluster - 1) / cluster * kVec;
-      s = shape(slice);
+  auto run = [&](auto vec, auto shift) -> int {
+    constexpr int kVec = decltype(vec)::value, kMaxNv = kVec == 1 ? 16 : kVec == 4 ? 4 : 2;
+    constexpr bool kShift = decltype(shift)::value;
+    RowShape s = row_shape(size, kVec, kShift, rows, kMaxNv, kVec == 1 ? 8 : 2);
+    const bool walk = s.fits && s.cluster == 1; // one kernel for dx and the sums over the rows
+    if (!walk) // (without those sums a thread has room for twice as much of a row)
+      s = row_shape(size, kVec, kShift, rows, std::min(16, 2 * kMaxNv), kVec == 1 ? 8 : 4);
+    if (!walk && params) {
+      const int64_t columns = (size + 255) / 256;
+      const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, 8 * sm_count() / columns));
+      const int64_t slab = (rows + slabs - 1) / slabs;
+      parts = (int)((rows + slab - 1) / slab);
+      NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));
+      NB_CUDA(launch_dependent(layer_norm_columns_kernel<T>, dim3((unsigned)columns, (unsigned)parts), dim3(256), 0, st, x, dy,
+                               mean, var, static_cast<float *>(scratch.p), rows, size, slab, eps));
     }
-    if (!s.fits) {
-      if (params) {
-        const int64_t columns = (size + 255) / 256;
-        const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, 8 * sm_count() / columns));
-        const int64_t slab = (rows + slabs - 1) / slabs;
-        parts = (int)((rows + slab - 1) / slab);
-        NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));
-        NB_CUDA(launch_dependent(layer_norm_columns_kernel<T>, dim3((unsigned)columns, (unsigned)parts), dim3(256), 0, st, x,
-                                 dy, mean, var, static_cast<float *>(scratch.p), rows, size, slab, eps));
-      }
-      if (dx) // (after the sums: it may overwrite x or dy)
-        NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, true>, dim3((unsigned)(rows * kLongBlocks)),
-                                 dim3(kLongThreads), 0, st, x, dy, (const P *)nullptr, gamma, dx, const_cast<float *>(mean),
-                                 const_cast<float *>(var), size, eps, accum_dx));
+    if (!walk && !dx)
+      return NB200_OK;
+    if (!s.fits) { // (after the sums: it may overwrite x or dy)
+      NB_CUDA(launch_dependent(layer_norm_long_kernel<T, P, true>, dim3((unsigned)(rows * kLongBlocks)), dim3(kLongThreads), 0, st,
+                               x, dy, (const P *)nullptr, gamma, dx, const_cast<float *>(mean), const_cast<float *>(var), size,
+                               eps, accum_dx));
       return NB200_OK;
     }
     const int per_block = s.row_warps == 1 ? 8 : 1, threads = 32 * s.row_warps * per_block;
-    // as many blocks as are resident, and then no more than their rounds need: each leaves partial sums
-    const int64_t groups = (rows + per_block - 1) / per_block;
-    const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() * std::max(1, 512 / threads) / cluster);
-    const int64_t rounds = (groups + most - 1) / most, blocks = (groups + rounds - 1) / rounds;
-    if (params) {
+    // As many blocks as are resident, and then no more than their rounds need: each leaves partial sums. With kShift a multiple
+    // of VEC, where any has a second row.
+    const int64_t groups = (rows + per_block - 1) / per_block, most = (int64_t)sm_count() * std::max(1, 512 / threads);
+    const int64_t rounds = walk ? (groups + most - 1) / most : 1;
+    int64_t blocks = (groups + rounds - 1) / rounds;
+    if (kShift && rounds > 1)
+      blocks = (blocks + kVec - 1) / kVec * kVec;
+    if (walk && params) {
       parts = (int)blocks;
       NB_TRY(scratch.alloc((size_t)parts * 2 * size * 4));
     }
-    const size_t smem = params && s.row_warps == 1 ? (size_t)per_block * 2 * size * 4 : 0;
     return with_count(s.nv, Counts{}, [&](auto nv) -> int {
       constexpr int kNv = decltype(nv)::value;
-      if constexpr (kNv <= kMaxNv) {
-        auto kernel = cluster > 1 ? (params ? layer_norm_backward_kernel<T, P, kVec, kNv, true, true>
-                                            : layer_norm_backward_kernel<T, P, kVec, kNv, false, true>)
-                                  : (params ? layer_norm_backward_kernel<T, P, kVec, kNv, true, false>
-                                            : layer_norm_backward_kernel<T, P, kVec, kNv, false, false>);
+      const size_t smem = walk && params && s.row_warps == 1 ? (size_t)per_block * 2 * size * 4 : 0;
+      auto launch = [&](auto kernel, auto clustered) -> int {
         if (smem > 48 * 1024)
           NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        NB_CUDA(launch_clusters(kernel, (unsigned)(blocks * cluster), cluster, threads, smem, st, x, dy, gamma, mean, var, dx,
-                                static_cast<float *>(scratch.p), rows, (int)size, 1.0f / (float)size, eps, s.row_warps, cluster,
-                                (int)slice, accum_dx, keep));
-      }
-      return NB200_OK;
+        if (decltype(clustered)::value)
+          NB_CUDA(launch_clusters(kernel, (unsigned)(blocks * s.cluster), s.cluster, threads, smem, st, x, dy, gamma, mean, var, dx,
+                                  static_cast<float *>(nullptr), rows, (int)size, 1.0f / (float)size, eps, s.row_warps, s.cluster,
+                                  (int)s.slice, accum_dx, keep));
+        else
+          NB_CUDA(launch_dependent(kernel, dim3((unsigned)blocks), dim3(threads), smem, st, x, dy, gamma, mean, var, dx,
+                                   static_cast<float *>(scratch.p), rows, (int)size, 1.0f / (float)size, eps, s.row_warps, 1, 0,
+                                   accum_dx, keep));
+        return NB200_OK;
+      };
+      if constexpr (kNv <= kMaxNv)
+        if (walk && params)
+          return launch(layer_norm_backward_kernel<T, P, kVec, kNv, true, kShift, false>, std::false_type{});
+      if constexpr (kNv <= 2 * kMaxNv && kNv <= 16)
+        return s.cluster > 1 ? launch(layer_norm_backward_kernel<T, P, kVec, kNv, false, kShift, true>, std::true_type{})
+                             : launch(layer_norm_backward_kernel<T, P, kVec, kNv, false, kShift, false>, std::false_type{});
+      return NB200_EVALUE;
     });
   };
-  if (rows > 0) {
-    const bool vec = size % kPackOf<T> == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gamma);
-    const bool pairs = size % 2 == 0 && aligned8(x) && aligned8(dy) && aligned8(dx) && aligned8(gamma);
-    NB_TRY(vec     ? run(std::integral_constant<int, kPackOf<T>>{})
-           : pairs ? run(std::integral_constant<int, 2>{})
-                   : run(std::integral_constant<int, 1>{}));
+  if (rows > 0)
+    NB_TRY(with_access<T>(size, aligned16(x) && aligned16(dy) && aligned16(dx), aligned16(gamma), run));
+  if (params) {
+    int share = 1;
+    while (share < 32 && share < parts)
+      share *= 2;
+    const int64_t columns = 32 * (32 / share);
+    NB_CUDA(launch_dependent(layer_norm_param_kernel<P>, dim3((unsigned)((size + columns - 1) / columns), 2), dim3(1024), 0, st,
+                             static_cast<const float *>(scratch.p), parts, share, size, dbeta, dgamma, accum_beta, accum_gamma));
   }
-  if (params)
-    NB_CUDA(launch_dependent(layer_norm_param_kernel<P>, dim3((unsigned)((size + 31) / 32), 2), dim3(1024), 0, st,
-                             static_cast<const float *>(scratch.p), parts, size, dbeta, dgamma, accum_beta, accum_gamma));
   return NB200_OK;
 }
 

@@ -18,34 +18,46 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// N neighbouring values as they lie in memory (16-byte accesses where N values are 16 bytes or a multiple of it)
+// N neighbouring values as they lie in memory (16-byte accesses where N values are 16 bytes or a multiple of it), kept as words
+// where they fill some: 16-bit values that are picked out one by one cost an instruction or two more each.
 template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
-  T v[N];
-  // Value i in fp32. Of 16-bit pairs by words: taken one by one they cost an instruction more each to pick them out.
+  static constexpr bool kWords = N * sizeof(T) % 4 == 0;
+  static constexpr int kPer = sizeof(T) == 4 || !kWords ? 1 : 2; // values a word
+  std::conditional_t<kWords, uint32_t, uint16_t> w[N / kPer];
   __device__ __forceinline__ float f(int i) const {
-    if constexpr (N % 2 == 0 && std::is_same<T, __nv_bfloat16>::value) {
-      const uint32_t w = reinterpret_cast<const uint32_t *>(v)[i / 2];
-      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-    } else if constexpr (N % 2 == 0 && std::is_same<T, __half>::value) {
-      const __half2 h = reinterpret_cast<const __half2 *>(v)[i / 2];
-      return i & 1 ? __high2float(h) : __low2float(h);
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return kPer == 1 ? __uint_as_float((uint32_t)w[i] << 16)
+                       : __uint_as_float(i & 1 ? w[i / kPer] & 0xffff0000u : (uint32_t)w[i / kPer] << 16);
+    } else if constexpr (kPer == 1) {
+      return __half2float(__ushort_as_half(w[i]));
     } else {
-      return to_f32(v[i]);
+      const __half2 h = *reinterpret_cast<const __half2 *>(&w[i / 2]);
+      return i & 1 ? __high2float(h) : __low2float(h);
     }
   }
-  __device__ __forceinline__ void fill(float f) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = from_f32<T>(f);
+  __device__ __forceinline__ void set(int i, T v) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+      const uint32_t b = *reinterpret_cast<const uint16_t *>(&v);
+      if constexpr (kPer == 1)
+        w[i] = (uint16_t)b;
+      else
+        w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | b << 16 : (w[i / 2] & 0xffff0000u) | b;
+    }
   }
   __device__ __forceinline__ void clear() {
-    if constexpr (N * sizeof(T) % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < (int)(N * sizeof(T) / 4); ++i)
-        reinterpret_cast<uint32_t *>(v)[i] = 0u;
-    } else {
-      fill(0.0f);
-    }
+    for (int i = 0; i < N / kPer; ++i)
+      w[i] = 0;
+  }
+  __device__ __forceinline__ void fill(float f) {
+    clear();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      set(i, from_f32<T>(f));
   }
 };
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
@@ -65,18 +77,21 @@ template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack_str
 // Rounding of neighbouring values, two at a time where the type has it.
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> round_pack(const float (&v)[N]) {
   Pack<T, N> o;
-  if constexpr (N % 2 == 0 && std::is_same<T, __nv_bfloat16>::value) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2)
-      *reinterpret_cast<__nv_bfloat162 *>(&o.v[i]) = __floats2bfloat162_rn(v[i], v[i + 1]);
-  } else if constexpr (N % 2 == 0 && std::is_same<T, __half>::value) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2)
-      *reinterpret_cast<__half2 *>(&o.v[i]) = __floats2half2_rn(v[i], v[i + 1]);
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+        o.w[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+        o.w[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      o.v[i] = from_f32<T>(v[i]);
+      o.set(i, from_f32<T>(v[i]));
   }
   return o;
 }
@@ -89,6 +104,16 @@ template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, co
 }
 
 template <typename T> constexpr int kPackOf = (int)(16 / sizeof(T)); // values in 16 bytes
+
+// Asynchronous copies to shared memory, in groups: cp_async_wait<N> waits until at most N of this thread's groups are under way.
+__device__ __forceinline__ void cp_async16(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void *to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
