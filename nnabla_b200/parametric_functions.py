@@ -166,6 +166,30 @@ def batch_normalization(inp, axes=[1], decay_rate=0.9, eps=1e-5, batch_stat=True
     return F.batch_normalization(inp, beta, gamma, mean, var, axes, decay_rate, eps, batch_stat, output_stat)
 
 
+def layer_normalization(inp, batch_axis=0, eps=1e-5, output_stat=False, fix_parameters=False, param_init=None,
+                        no_scale=False, no_bias=False):
+    axes = [batch_axis] if isinstance(batch_axis, int) else list(batch_axis)
+    axes = [a + inp.dim() if a < 0 else a for a in axes]
+    shape = tuple(1 if i in axes else int(n) for i, n in enumerate(inp.shape))
+    init = param_init or {}
+    with parameter_scope("layer_normalization"):
+        beta = None if no_bias else get_parameter_or_create("beta", shape, init.get("beta", _zeros))
+        gamma = None if no_scale else get_parameter_or_create(
+            "gamma", shape, init.get("gamma", lambda s: np.ones(s, np.float32)))
+    return F.layer_normalization(inp, beta, gamma, batch_axis, eps, output_stat)
+
+
+def affine_softmax_cross_entropy(inp, label, n_outmaps, base_axis=1, w_init=None, b_init=None, fix_parameters=False, rng=None,
+                                 with_bias=True):
+    """softmax_cross_entropy(affine(inp, n_outmaps), label) on the parameters of `affine`, without the logits."""
+    inmaps = int(np.prod(inp.shape[base_axis:]))
+    with parameter_scope("affine"):
+        w = get_parameter_or_create("W", (inmaps, n_outmaps),
+                                    w_init or _glorot_uniform(inmaps, n_outmaps, (1, 1), _rng(rng)))
+        b = get_parameter_or_create("b", (n_outmaps,), b_init or _zeros) if with_bias else None
+    return F.affine_softmax_cross_entropy(inp, w, label, b, base_axis)
+
+
 def fixed_point_quantized_affine(inp, n_outmaps, base_axis=1, w_init=None, b_init=None, fix_parameters=False, rng=None,
                                  with_bias=True, quantize_w=True, sign_w=True, n_w=8, delta_w=2 ** -4,
                                  ste_fine_grained_w=True, quantize_b=True, sign_b=True, n_b=8, delta_b=2 ** -4,

@@ -198,6 +198,37 @@ class Runner:
 
 
 # ---------------------------------------------------------------------------
+# Training the head: the loss on pooled features, against labels and a teacher
+# ---------------------------------------------------------------------------
+
+def head_loss(features, weight, bias, label, teacher=None, temperature=4.0, share=0.5):
+    """The head's loss and its gradients: the mean, over the rows whose label is not negative, of
+    (1 - share) * softmax cross entropy + share * distillation from a teacher's best classes.
+
+    features [rows, inputs], weight [inputs, classes], bias [classes]: one type (float32, bfloat16 or float16 for the cross
+    entropy alone, float32 with a teacher). label [rows, 1]: int32 or int64. teacher: (index, logits) of each row's best
+    classes, as functions.top_k_distillation takes them, or None (share is then 0). Without a teacher no logits are made.
+    Returns (loss, (dfeatures, dweight, dbias)), the loss a float32 tensor of one value."""
+    from . import functions as F
+    counts = label >= 0
+    each = counts.float() / counts.sum().clamp(min=1)  # the weight of a row in the mean
+    if teacher is None:
+        share = 0.0
+    loss, stat = F.affine_softmax_cross_entropy(features, weight, label, bias, output_stat=True)
+    total = (1.0 - share) * (loss * each).sum()
+    grads = F.affine_softmax_cross_entropy_backward(features, weight, label, stat, (1.0 - share) * each, bias)
+    if teacher is not None:
+        index, best = teacher
+        logits = F.affine(features, weight, bias)
+        loss, stat = F.top_k_distillation(logits, index, best, temperature, output_stat=True)
+        total = total + share * (loss * each).sum()
+        # (in place: the logits are not needed any more)
+        dlogits = F.top_k_distillation_backward(logits, index, best, stat, share * each, temperature, dx=logits)
+        grads = F.affine_backward(features, weight, dlogits, accum=(True, True, True), grads=grads)
+    return total, grads
+
+
+# ---------------------------------------------------------------------------
 # The same network with BatchNormalization folded into the convolutions
 # ---------------------------------------------------------------------------
 
