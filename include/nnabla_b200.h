@@ -671,7 +671,9 @@ int nb200_layer_normalization_backward(const void *x, const void *dy, const void
  *   loss = log sum exp(l) - l[label]   (fp32, [rows])
  * stat [rows, 2], fp32: the row's largest l, and log sum exp(l - largest).
  * A row with a negative label has the loss 0; a label >= classes makes its row's loss NaN. The logits are never
- * kept: the scratch that a call takes grows with the rows and not with rows * classes. */
+ * kept: beside copies of x and w where these have to be laid out anew (fp32: 1.5 times their size; rows that are
+ * no multiple of 16 bytes) a call takes some 64 MB of scratch, or what 256 rows (forward) or classes (backward)
+ * need. */
 int nb200_affine_softmax_cross_entropy(const void *x, const void *w, const void *bias, const void *label,
                                        float *loss, float *stat, int64_t rows, int64_t size, int64_t classes,
                                        int type, int label_bytes, void *stream);

@@ -238,7 +238,7 @@ template <typename T> size_t operand_bytes(const T *p, int64_t rows, int64_t col
 }
 template <typename T> Operand operand(const T *p, int64_t rows, int64_t cols, void *scratch, Layout &layout) {
   constexpr bool kF32 = std::is_same<T, float>::value;
-  Operand o{scratch, rows, cols, up(cols, kF32 ? 64 : 8), kF32 ? 3 : 1};
+  Operand o{scratch, rows, cols, up(cols, kF32 ? 64 : 8), kF32 ? 3 : 1, rows};
   layout = Layout{};
   if (operand_bytes(p, rows, cols) == 0)
     o.p = p;
@@ -292,9 +292,11 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
   const int kblocks = (int)((size + 63) / 64);
   const bool pair = pays_pairs({{rows, classes, kblocks}});
   r.tiles = loss_sum_tiles<T>(classes, kblocks, pair);
+  // so many rows at a time that their maxima and sums are 64 MB (the largest head in use: 8192 rows of 128000 classes)
+  const int64_t slab = std::min(rows, std::max<int64_t>(256, (1 << 23) / r.tiles / 256 * 256));
   Parts parts;
   const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
-  const size_t at_partial = parts.take((size_t)rows * r.tiles * 8), at_target = parts.take((size_t)rows * 4);
+  const size_t at_partial = parts.take((size_t)slab * r.tiles * 8), at_target = parts.take((size_t)slab * 4);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc(parts.bytes));
   char *base = static_cast<char *>(scratch.p);
@@ -303,13 +305,21 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
   Preparation pre{};
   const Operand ox = operand(x, rows, size, base + at_x, pre.m[0]), ow = operand(w, size, classes, base + at_w, pre.m[1]);
   NB_TRY(prepare<T>(pre, st));
-  Products prob{};
-  prob.count = 1;
-  prob.bias = bias;
-  prob.rows = r;
-  prob.p[0].M = (int)rows, prob.p[0].N = (int)classes, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
-  NB_TRY((run_loss_gemm<T, Out::kSums>(pair, prob, &ox, &ow, st)));
-  NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, r, rows, loss, stat));
+  const char *label = static_cast<const char *>(r.label);
+  for (int64_t r0 = 0; r0 < rows; r0 += slab) {
+    const int64_t n = std::min(slab, rows - r0);
+    Operand part = ox; // (its planes stay as far apart)
+    part.p = static_cast<const char *>(ox.p) + 2 * r0 * ox.pitch;
+    part.rows = n;
+    r.label = label + r0 * r.label_bytes;
+    Products prob{};
+    prob.count = 1;
+    prob.bias = bias;
+    prob.rows = r;
+    prob.p[0].M = (int)n, prob.p[0].N = (int)classes, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
+    NB_TRY((run_loss_gemm<T, Out::kSums>(pair, prob, &part, &ow, st)));
+    NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, r, n, loss + r0, stat + r0));
+  }
   return NB200_OK;
 }
 
@@ -320,7 +330,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   constexpr int kPlanes = kF32 ? 3 : 1;
   using G = std::conditional_t<kF32, __nv_bfloat16, T>;
   // A piece's G is 64 MB: both products read it from L2, and their tiles are rounds enough to leave few SMs idle.
-  int64_t piece = std::max<int64_t>(1024, (int64_t)(1 << 25) / kPlanes / rows);
+  int64_t piece = std::max<int64_t>(256, (int64_t)(1 << 25) / kPlanes / rows);
   const int64_t count = (classes + piece - 1) / piece;
   piece = up((classes + count - 1) / count, 256);
   const bool pieces = piece < classes;
@@ -363,7 +373,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   r.scale = scale;
   for (int64_t c0 = 0; c0 < classes; c0 += piece) {
     const int64_t n = std::min(piece, classes - c0);
-    const Operand og{base + at_g, rows, n, piece, kPlanes}, owc = columns(ow, c0, n);
+    const Operand og{base + at_g, rows, n, piece, kPlanes, rows}, owc = columns(ow, c0, n);
     Products prob{};
     prob.count = 1;
     prob.bias = bias;

@@ -17,28 +17,52 @@ namespace {
 
 constexpr int kMaxEntries = 1024;
 
-// The row's teacher, by one warp: each lane's entries are k = lane, lane + 32, ... An entry is one with a class that is not
-// negative.
-template <typename T, typename I>
-__device__ __forceinline__ MaxSum teacher_sums(const I *index, const T *teacher, int best, float scale, int lane) {
-  MaxSum t{-INFINITY, 0.0f};
-  float top = -INFINITY;
-  bool nan = false;
-  for (int k = lane; k < best; k += 32)
-    if (index[k] >= 0) {
-      const float v = to_f32(teacher[k]);
+// The row's teacher, by one warp: each lane's entries are k = lane, lane + 32, ... The first kHeld of them stay in registers, on
+// their way while the row of x is read. An entry is one with a class that is not negative.
+constexpr int kHeld = 4;
+template <typename T, typename I> struct Entries {
+  const I *index;
+  const T *teacher;
+  int best, lane;
+  I c[kHeld];
+  T t[kHeld];
+  __device__ __forceinline__ Entries(const I *index_, const T *teacher_, int best_, int lane_)
+      : index(index_), teacher(teacher_), best(best_), lane(lane_) {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      c[u] = -1;
+      if (lane + 32 * u < best) {
+        c[u] = index[lane + 32 * u];
+        t[u] = teacher[lane + 32 * u];
+      }
+    }
+  }
+  // f(class, logit, u) for this lane's entries; u: the held one's number, kHeld for the others
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (c[u] >= 0)
+        f((int64_t)c[u], to_f32(t[u]), u);
+    for (int k = lane + 32 * kHeld; k < best; k += 32)
+      if (index[k] >= 0)
+        f((int64_t)index[k], to_f32(teacher[k]), kHeld);
+  }
+  __device__ __forceinline__ MaxSum sums(float scale) const {
+    MaxSum s{-INFINITY, 0.0f};
+    float top = -INFINITY;
+    bool nan = false;
+    each([&](int64_t, float v, int) {
       top = fmaxf(top, v);
       nan |= v != v;
-    }
-  top = __any_sync(0xffffffffu, nan) ? NAN : warp_max(top);
-  t.m = top;
-  const float base = top == -INFINITY ? 0.0f : top;
-  for (int k = lane; k < best; k += 32)
-    if (index[k] >= 0)
-      t.s += ex2((to_f32(teacher[k]) - base) * scale);
-  t.s = warp_sum(t.s);
-  return t;
-}
+    });
+    top = __any_sync(0xffffffffu, nan) ? NAN : warp_max(top);
+    s.m = top;
+    const float base = top == -INFINITY ? 0.0f : top;
+    each([&](int64_t, float v, int) { s.s += ex2((v - base) * scale); });
+    s.s = warp_sum(s.s);
+    return s;
+  }
+};
 
 // [start, start + n) of x cut into values before the first 16-byte boundary, whole 16-byte packs, and the rest.
 template <typename T> struct Run {
@@ -78,6 +102,13 @@ __global__ void __launch_bounds__(kSumThreads, 4) distill_forward_kernel(const T
   const float scale = kLog2e / tau;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const Run<T> run(xr + c0, c1 - c0);
+  // the teacher's entries, and x there, for the first block's first warp (none for the others)
+  const Entries<T, I> entries(index + row * best, teacher + row * best, part == 0 && warp == 0 ? best : 0, lane);
+  T named[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (entries.c[u] >= 0 && (int64_t)entries.c[u] < classes)
+      named[u] = xr[entries.c[u]];
   float m = -INFINITY, s = 0.0f;
   auto add = [&](auto &v, int n) {
     float top = m;
@@ -142,25 +173,28 @@ __global__ void __launch_bounds__(kSumThreads, 4) distill_forward_kernel(const T
   }
   if (part == 0 && warp == 0) {
     const float log_sum = log2f(t.s) * kLn2;
-    const I *ir = index + row * best;
-    const T *tr = teacher + row * best;
-    const MaxSum p = teacher_sums(ir, tr, best, scale, lane);
+    const MaxSum p = entries.sums(scale);
     // In 64 bits, and divided by the shares' own sum: a class that the student masks with the type's lowest value and the
     // teacher names gives a loss next to the largest float.
     double sum = 0.0, mass = 0.0;
+    const double per = 1.0 / (double)tau;
     if (p.m != -INFINITY) {
-      const double log_mass = log((double)p.s);
-      for (int k = lane; k < best; k += 32) {
-        const int64_t c = (int64_t)ir[k];
-        if (c < 0)
-          continue;
-        const float d = to_f32(tr[k]) - p.m, share = ex2(d * scale);
+      const double log_mass = log2f(p.s) * kLn2;
+      entries.each([&](int64_t c, float v, int u) {
+        const float d = v - p.m, share = ex2(d * scale);
         mass += share;
-        if (c >= classes)
+        if (c >= classes) {
           sum = NAN;
-        else if (!(share == 0.0f))
-          sum += share * (((double)d / tau - log_mass) - (((double)to_f32(xr[c]) - t.m) / tau - log_sum));
-      }
+        } else if (!(share == 0.0f)) {
+          float at = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kHeld; ++i)
+            at = u == i ? to_f32(named[i]) : at;
+          if (u == kHeld)
+            at = to_f32(xr[c]);
+          sum += share * ((d * per - log_mass) - (((double)at - t.m) * per - log_sum));
+        }
+      });
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -205,28 +239,42 @@ __global__ void __launch_bounds__(kGradThreads, 4) distill_backward_kernel(
   c1 = c1 < classes && part + 1 < parts ? c1 : classes;
   c0 = c0 < c1 ? c0 : c1;
   const Run<T> run(xr + c0, c1 - c0);
+  // the first loads of the stream are on their way while the entries are looked at
+  Pack<T, V> ahead[kGradPacks];
+#pragma unroll
+  for (int u = 0; u < kGradPacks; ++u)
+    if (threadIdx.x + u * kGradThreads < run.packs)
+      ahead[u] = load_pack_stream<T, V>(run.body + (threadIdx.x + u * kGradThreads) * V);
   const float scale = kLog2e / tau, d = dloss[row] * tau, top = stat[row].x, log2_sum = stat[row].y * kLog2e;
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    const I *ir = index + row * best;
-    const T *tr = teacher + row * best;
-    const MaxSum t = teacher_sums(ir, tr, best, scale, lane);
+    const Entries<T, I> all(index + row * best, teacher + row * best, best, lane);
+    const MaxSum t = all.sums(scale);
     int n = 0;
     bool bad = false;
     if (t.m != -INFINITY) {
       const float log2_p = log2f(t.s);
       for (int k0 = 0; k0 < best; k0 += 32) {
         const int k = k0 + lane;
-        const int64_t c = k < best ? (int64_t)ir[k] : -1;
+        int64_t c = -1;
+        float v = 0.0f;
+        if (k0 < 32 * kHeld) {
+#pragma unroll
+          for (int u = 0; u < kHeld; ++u)
+            if (k0 == 32 * u && all.c[u] >= 0)
+              c = all.c[u], v = to_f32(all.t[u]);
+        } else if (k < best) {
+          c = (int64_t)all.index[k], v = to_f32(all.teacher[k]);
+        }
         bad |= c >= classes;
         const bool here = c >= c0 && c < c1;
-        const unsigned all = __ballot_sync(0xffffffffu, here);
+        const unsigned found = __ballot_sync(0xffffffffu, here);
         if (here) {
-          const int to = n + __popc(all & ((1u << lane) - 1u));
+          const int to = n + __popc(found & ((1u << lane) - 1u));
           at[to] = (int)(c - c0);
-          share[to] = ex2(fmaf(to_f32(tr[k]) - t.m, scale, -log2_p));
+          share[to] = ex2(fmaf(v - t.m, scale, -log2_p));
         }
-        n += __popc(all);
+        n += __popc(found);
       }
     }
     bad = __any_sync(0xffffffffu, bad);
@@ -250,11 +298,12 @@ __global__ void __launch_bounds__(kGradThreads, 4) distill_backward_kernel(
       continue;
     float sum = 0.0f;
     bool only = true;
-    for (int j = 0; j < n; ++j)
-      if (at[j] == at[i]) {
-        only &= j >= i;
-        sum += share[j];
-      }
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const bool same = at[j] == at[i];
+      only &= !same || j >= i;
+      sum += same ? share[j] : 0.0f;
+    }
     if (only) {
       first |= 1u << u;
       fixed[u] = (q(to_f32(xr[c0 + at[i]])) - sum) * factor;
@@ -284,7 +333,11 @@ __global__ void __launch_bounds__(kGradThreads, 4) distill_backward_kernel(
     }
   };
   T *body = out + (run.body - xr);
-  int64_t i = threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < kGradPacks; ++u)
+    if (threadIdx.x + u * kGradThreads < run.packs)
+      store(body + (threadIdx.x + u * kGradThreads) * V, ahead[u]);
+  int64_t i = threadIdx.x + kGradPacks * kGradThreads;
   for (; i + (kGradPacks - 1) * kGradThreads < run.packs; i += kGradPacks * kGradThreads) {
     Pack<T, V> p[kGradPacks];
 #pragma unroll

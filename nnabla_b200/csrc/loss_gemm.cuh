@@ -607,15 +607,17 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
   }
 }
 
-// An operand in memory: [planes][rows][pitch] of 16-bit values, 16-byte aligned, pitch a multiple of 8.
+// An operand in memory: `planes` matrices [rows][pitch] of 16-bit values, plane_rows rows apart; 16-byte aligned, pitch a
+// multiple of 8.
 struct Operand {
   const void *p;
   int64_t rows, cols, pitch;
   int planes;
+  int64_t plane_rows;
 };
 inline int loss_operand_map(CUtensorMap *map, const Operand &o, bool mn, int box_rows) {
   const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.planes};
-  const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)(o.pitch * o.rows) * 2};
+  const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)(o.pitch * o.plane_rows) * 2};
   const uint32_t box[3] = {64, mn ? 64u : (uint32_t)box_rows, 1};
   return encode_tiled(map, 0, 3, o.p, dims, strides, box, nullptr, 128);
 }

@@ -251,3 +251,23 @@ def test_no_rows():
     held = [torch.empty_like(x), torch.ones_like(w), torch.ones_like(bias)]
     F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias, accum=(True,) * 3, grads=held)
     assert (held[1] == 1).all() and (held[2] == 1).all()
+
+
+def test_more_rows_than_one_pass_takes():
+    """The forward pass takes the rows in slabs (here 16384 at a time: 512 pairs of a maximum and a sum a row)."""
+    x, w, label, bias, dloss = data(20000, 16, 32700, torch.bfloat16)
+    loss, stat = F.affine_softmax_cross_entropy(x, w, label, bias, output_stat=True)
+    for at in (0, 8000, 16000, 19500):
+        rows = slice(at, at + 500)
+        logits, lse, want, _ = reference(x[rows], w, label[rows], bias, dloss[rows])
+        e = 1e-5 * rms(logits) + 1e-6
+        assert ((loss[rows].double() - want).abs() <= 3 * e + 2.0 ** -20 * want.abs()).all()
+        s = stat[rows].double()
+        assert ((s[:, :1] + s[:, 1:] - lse).abs() <= 2 * e + 2.0 ** -20 * lse.abs()).all()
+
+
+@pytest.mark.parametrize("rows,size,classes", [(9, 200, 3000), (17, 64, 11008), (600, 96, 128), (3000, 40, 70), (2600, 320, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_products_with_a_long_axis(rows, size, classes, dtype):
+    """Shapes whose gradients have few tiles and a long K."""
+    check(*data(rows, size, classes, dtype))
