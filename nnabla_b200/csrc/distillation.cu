@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kSumThreads, 4) distill_forward_kernel(const T
       whole[0] = t.m, whole[1] = t.s;
   }
   if (parts > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
     if (part == 0 && warp == 0) {
       MaxSum o{-INFINITY, 0.0f};
       if (lane < parts) {
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kSumThreads, 4) distill_forward_kernel(const T
     }
   }
   if (parts > 1) // no block leaves while another may still read its sums
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
 }
 
 constexpr int kGradThreads = 256, kGradPacks = 4;

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
     own[i] = s;
   }
   if (splits > 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
   else
     __syncthreads();
   if (split == 0)
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
       }
     }
   if (splits > 1) // no block leaves while the first may still read its sums
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
 }
 
 // dx = G W^T and dW = x^T G in one pass over W. A thread has eight columns of G in registers, [R][8] in fp32, and walks along

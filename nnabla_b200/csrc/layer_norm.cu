@@ -62,7 +62,7 @@ template <int N> __device__ __forceinline__ void cluster_sums(float (&v)[N], flo
 #pragma unroll
     for (int i = 0; i < N; ++i)
       slot[i] = v[i];
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_barrier();
   // every warp for itself, a lane a block
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(512, 2) layer_norm_kernel(const T *__restrict_
     }
   }
   if constexpr (kCluster) // no block leaves while another may still read its sums
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
 }
 
 constexpr int kLongThreads = 512, kLongBlocks = 8;
@@ -352,7 +352,7 @@ __global__ void __cluster_dims__(kLongBlocks, 1, 1) __launch_bounds__(kLongThrea
     }
   }
   // no block leaves while another may still read its sums
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_barrier();
 }
 
 // dx, and where kParams the sums over this block's rows of dy and dy u, each thread for the columns that it holds: a block (or
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(
     }
   }
   if constexpr (kCluster) // no block leaves while another may still read its sums
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
 }
 
 // The same sums for rows too long for the kernel above: a thread a column, a slab of rows a block, partial sums

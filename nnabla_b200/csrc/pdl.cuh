@@ -63,7 +63,13 @@ inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// The same with clusters of `cluster` blocks.
+// Barrier of a cluster's blocks: what the others wrote to their shared memory before it can be read after it.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The same as launch_dependent with clusters of `cluster` blocks.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_clusters(void (*kernel)(KArgs...), unsigned grid, int cluster, int block, size_t smem,
                                    cudaStream_t st, Args... args) {
