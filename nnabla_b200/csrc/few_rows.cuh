@@ -24,6 +24,10 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+template <int R> struct alignas(R > 1 ? 16 : 8) Few { // a value of x of each row, twice
+  uint64_t v[R];
+};
+
 constexpr int kFewBatch = 4, kFewBatches = 3;                         // packs a batch of copies, batches on the way
 constexpr int kFewRing = kFewBatch * kFewBatches * kFewThreads * 16; // bytes
 
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
 
 // dx = G W^T and dW = x^T G in one pass over W. A thread has eight columns of G in registers, [R][8] in fp32, and walks along
 // the rows of W: of each it loads its columns, stores those of dW and has R products for dx, which its warp sums up (the first
-// steps exchange halves of the R values, so that eight values take nine shuffles). The sums of a block's columns, 256 * 8, go to
+// steps exchange halves of the values, so that the sixteen of two rows take sixteen shuffles). The sums of a block's columns, 256 * 8, go to
 // partial[block column][R][size]. (With the threads along a row and G read from L2 for every four rows of W [5, 1792] . [1792,
 // 109056] bf16 took 398 us.)
 constexpr int kFewWalk = 32; // rows of W between two exchanges of the warps' sums
@@ -204,7 +208,8 @@ __global__ void __launch_bounds__(kFewGradThreads) few_grads_kernel(const T *__r
                                                                     int64_t size, int64_t slab, int64_t classes,
                                                                     bool accum_dw, bool keep) {
   constexpr int kGroups = 8 / VEC, kWarps = kFewGradThreads / 32; // groups of VEC neighbouring columns
-  __shared__ float xs[kFewWalk][R], sums[kWarps][kFewWalk][R];
+  __shared__ Few<R> xs[kFewWalk];
+  __shared__ float sums[kWarps][kFewWalk][R];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -239,54 +244,55 @@ __global__ void __launch_bounds__(kFewGradThreads) few_grads_kernel(const T *__r
     const int n = (int)(h1 - h < kFewWalk ? h1 - h : kFewWalk);
     for (int i = threadIdx.x; i < kFewWalk * R; i += kFewGradThreads) {
       const int r = i / kFewWalk, k = i % kFewWalk;
-      xs[k][r] = r < count && k < n ? to_f32(x[r * size + h + k]) : 0.0f;
+      const float v = r < count && k < n ? to_f32(x[r * size + h + k]) : 0.0f;
+      xs[k].v[r] = pair_of(v, v);
     }
     __syncthreads();
-    auto row = [&](int k, int from) {
-      uint64_t wv[4], xv[R];
-      {
-        float f[8];
+    // two rows at a time, for the latency of their chains
+    for (int k = 0; k < n; k += 2) {
+      float s[2 * R];
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i)
+      for (int q = 0; q < 2; ++q) {
+        uint64_t wv[4];
+        {
+          float f[8];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            f[i * VEC + j] = next[from][i].f(j);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          wv[j] = pair_of(f[2 * j], f[2 * j + 1]);
-      }
-      fetch(h + k + 2, from);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        xv[r] = pair_of(xs[k][r], xs[k][r]);
-      if (dw) {
-        float o[kGroups][VEC];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint64_t t = 0;
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            t = fma2(xv[r], gv[r][j], t);
-          const float2 both = unpair(t);
-          o[2 * j / VEC][2 * j % VEC] = both.x;
-          o[(2 * j + 1) / VEC][(2 * j + 1) % VEC] = both.y;
-        }
-#pragma unroll
-        for (int i = 0; i < kGroups; ++i) {
-          if (column(i) >= classes)
-            continue;
-          T *to = dw + (h + k) * classes + column(i);
-          if (accum_dw) {
-            const Pack<T, VEC> old = load_pack<T, VEC>(to);
+          for (int i = 0; i < kGroups; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-              o[i][j] += old.f(j);
-          }
-          store_pack<T, VEC>(to, o[i], keep);
+              f[i * VEC + j] = next[q][i].f(j);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            wv[j] = pair_of(f[2 * j], f[2 * j + 1]);
         }
-      }
-      if (want_dx) {
-        float s[R];
+        fetch(h + k + q + 2, q);
+        if (dw && k + q < n) {
+          const Few<R> xv = xs[k + q];
+          float o[kGroups][VEC];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint64_t t = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+              t = fma2(xv.v[r], gv[r][j], t);
+            const float2 both = unpair(t);
+            o[2 * j / VEC][2 * j % VEC] = both.x;
+            o[(2 * j + 1) / VEC][(2 * j + 1) % VEC] = both.y;
+          }
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) {
+            if (column(i) >= classes)
+              continue;
+            T *to = dw + (h + k + q) * classes + column(i);
+            if (accum_dw) {
+              const Pack<T, VEC> old = load_pack<T, VEC>(to);
+#pragma unroll
+              for (int j = 0; j < VEC; ++j)
+                o[i][j] += old.f(j);
+            }
+            store_pack<T, VEC>(to, o[i], keep);
+          }
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           uint64_t t = 0;
@@ -294,29 +300,27 @@ __global__ void __launch_bounds__(kFewGradThreads) few_grads_kernel(const T *__r
           for (int j = 0; j < 4; ++j)
             t = fma2(gv[r][j], wv[j], t);
           const float2 both = unpair(t);
-          s[r] = both.x + both.y;
+          s[q * R + r] = both.x + both.y;
         }
+      }
+      if (want_dx) {
         int d = 16;
 #pragma unroll
-        for (int m = R / 2; m >= 1; m /= 2, d /= 2) {
+        for (int m = R; m >= 1; m /= 2, d /= 2) {
           const bool upper = lane & d;
 #pragma unroll
-          for (int r = 0; r < m; ++r) {
-            const float away = upper ? s[r] : s[r + m];
-            s[r] = (upper ? s[r + m] : s[r]) + __shfl_xor_sync(0xffffffffu, away, d);
+          for (int i = 0; i < m; ++i) {
+            const float away = upper ? s[i] : s[i + m];
+            s[i] = (upper ? s[i + m] : s[i]) + __shfl_xor_sync(0xffffffffu, away, d);
           }
         }
 #pragma unroll
         for (; d >= 1; d /= 2)
           s[0] += __shfl_xor_sync(0xffffffffu, s[0], d);
-        if (lane % (32 / R) == 0) // lane's leading bits are the row that it ended with
-          sums[warp][k][lane / (32 / R)] = s[0];
+        const int i = lane / (16 / R); // lane's leading bits are the row of W and the row that it ended with
+        if (lane % (16 / R) == 0 && k + i / R < n)
+          sums[warp][k + i / R][i % R] = s[0];
       }
-    };
-    for (int k = 0; k < n; k += 2) {
-      row(k, 0);
-      if (k + 1 < n)
-        row(k + 1, 1);
     }
     __syncthreads();
     if (want_dx)
