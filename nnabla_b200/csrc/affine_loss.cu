@@ -260,20 +260,24 @@ Operand columns(Operand o, int64_t c0, int64_t n) {
   return o;
 }
 
-// Time of a launch's tiles, in MMA cycles of an SM: rounds of 256 x 256 tiles on pairs of SMs, 512 cycles a K block, or of
-// 128 x 64 ones, 204 (51 an instruction, for its operands' reads; 32 by its products).
+// Time of a launch's tiles, in cycles of an SM: rounds of 256 x 256 tiles on pairs of SMs, 512 MMA cycles a K block, or of
+// 128 x 64 ones, 204 (51 an instruction, for its operands' reads; 32 by its products); an epilogue at least, 4500 and 2000.
 struct TileCount {
   int64_t M, N, kblocks;
 };
 bool pays_pairs(std::initializer_list<TileCount> products) {
-  int64_t pair_tiles = 0, single_tiles = 0, blocks = 1;
+  int64_t pair_tiles = 0, single_tiles = 0, pair_work = 0, single_work = 0;
   for (const TileCount &p : products) {
-    pair_tiles += ((p.M + 255) / 256) * ((p.N + 255) / 256);
-    single_tiles += ((p.M + 127) / 128) * ((p.N + 63) / 64);
-    blocks = std::max(blocks, p.kblocks);
+    const int64_t pairs = ((p.M + 255) / 256) * ((p.N + 255) / 256), singles = ((p.M + 127) / 128) * ((p.N + 63) / 64);
+    pair_tiles += pairs, single_tiles += singles;
+    pair_work += pairs * std::max<int64_t>(512 * p.kblocks, 4500);
+    single_work += singles * std::max<int64_t>(204 * p.kblocks, 2000);
   }
-  auto rounds = [](int64_t tiles, int64_t units) { return (tiles + units - 1) / units; };
-  return rounds(pair_tiles, sm_count() / 2) * 512 <= rounds(single_tiles, sm_count()) * 204;
+  // the mean tile, in whole rounds
+  auto time = [](int64_t work, int64_t tiles, int64_t units) {
+    return tiles == 0 ? 0 : (tiles + units - 1) / units * (work / tiles);
+  };
+  return time(pair_work, pair_tiles, sm_count() / 2) <= time(single_work, single_tiles, sm_count());
 }
 
 // Scratch for a call, in parts that begin at 256-byte boundaries.
@@ -316,7 +320,7 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
     prob.count = 1;
     prob.bias = bias;
     prob.rows = r;
-    prob.p[0].M = (int)n, prob.p[0].N = (int)classes, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
+    prob.p[0].M = (int)n, prob.p[0].N = (int)classes, prob.p[0].K = (int)size, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
     NB_TRY((run_loss_gemm<T, Out::kSums>(pair, prob, &part, &ow, st)));
     NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, r, n, loss + r0, stat + r0));
   }
@@ -380,7 +384,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
     prob.class0 = (int)c0;
     prob.rows = r;
     Product &l = prob.p[0];
-    l.M = (int)rows, l.N = (int)n, l.kblocks = (int)size_blocks, l.b_mn = 1;
+    l.M = (int)rows, l.N = (int)n, l.K = (int)size, l.kblocks = (int)size_blocks, l.b_mn = 1;
     l.out = base + at_g, l.ldo = piece, l.stride = rows * piece;
     NB_TRY((run_loss_gemm<T, Out::kGrad>(pair_grad, prob, &ox, &owc, st)));
     Operand a[2], b[2];
@@ -388,7 +392,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
     if (dw) {
       Product &p = prob.p[prob.count];
       p = Product{};
-      p.M = (int)size, p.N = (int)n, p.kblocks = (int)row_blocks, p.a_mn = p.b_mn = 1;
+      p.M = (int)size, p.N = (int)n, p.K = (int)rows, p.kblocks = (int)row_blocks, p.a_mn = p.b_mn = 1;
       if (dw_splits > 1) {
         p.splits = dw_splits, p.split_blocks = dw_blocks, p.stride = size * piece;
         p.out = dw32, p.ldo = piece, p.out_f32 = 1, p.vec = 1;
@@ -401,7 +405,7 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
     if (dx) {
       Product &p = prob.p[prob.count];
       p = Product{};
-      p.M = (int)rows, p.N = (int)size, p.kblocks = (int)((n + 63) / 64), p.ldo = direct ? size : ld_dx;
+      p.M = (int)rows, p.N = (int)size, p.K = (int)n, p.kblocks = (int)((n + 63) / 64), p.ldo = direct ? size : ld_dx;
       p.splits = (p.kblocks + dx_blocks - 1) / dx_blocks, p.split_blocks = dx_blocks, p.stride = rows * ld_dx;
       p.out = direct ? static_cast<void *>(dx) : dx32, p.out_f32 = !direct;
       p.accum = c0 > 0 || (direct && accum[0]);

@@ -43,7 +43,9 @@ enum class Out { kSums, kGrad, kStore };
 
 constexpr int kMaxProducts = 2;
 struct Product {
-  int M, N, kblocks, m_tiles, n_tiles;
+  int M, N, K, kblocks, m_tiles, n_tiles;
+  int steps;    // MMA steps of a K block: four, or what a single short block needs
+  int tx_bytes; // that a stage's loads bring to a CTA
   int splits, split_blocks; // kStore: K in `splits` tiles of split_blocks K blocks, each with a result of its own
   int a_mn, b_mn;           // memory rows run along K
   // kStore: out [splits][M][ldo] (+)= scale[2] * D; kGrad: out is G [planes][M][ldo]. stride: between splits or planes
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
           uint8_t *st = smem + stage * kStageBytes;
           const uint32_t full = kPair ? ptx::map_to_cta(ptx::smem_u32(full_bar + stage), 0) : 0;
           if (rank == 0)
-            ptx::mbar_expect_tx(full_bar + stage, kCtas * kStageBytes); // bytes of both CTAs
+            ptx::mbar_expect_tx(full_bar + stage, kCtas * (uint32_t)prob.p[t.which].tx_bytes); // bytes of both CTAs
           auto load = [&](uint8_t *dst, const CUtensorMap *map, int c0, int c1, int pl) {
             if constexpr (kPair)
               ptx::tma_load_3d_pair(dst, map, full, c0, c1, pl, keep);
@@ -273,6 +275,7 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
                                (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
         // leading byte offset of an MN-major operand; 16 of K are 16 rows there, 32 bytes of a row otherwise
         const uint64_t a_lbo = a_mn ? (uint64_t)(kChunkBytes >> 4) << 16 : 0, b_lbo = b_mn ? (uint64_t)(kChunkBytes >> 4) << 16 : 0;
+        const int steps = prob.p[t.which].steps;
         const uint32_t a_step = a_mn ? (16 * kRowBytes) >> 4 : 2, b_step = b_mn ? (16 * kRowBytes) >> 4 : 2;
         for (int kb0 = t.kb0; kb0 < t.kb1 && ok; kb0 += prob.chunk, ++local) {
           const int buf = local & 1;
@@ -303,6 +306,8 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
                 const uint64_t bd = ptx::smem_desc_k_sw128(st + PL * kABytes + (sum - pa) * kBBytes) | b_lbo;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
+                  if (k >= steps)
+                    break;
                   if constexpr (kPair)
                     ptx::mma_pair_bf16(d, ad + k * a_step, bd + k * b_step, idesc, accumulate);
                   else
@@ -615,10 +620,13 @@ struct Operand {
   int planes;
   int64_t plane_rows;
 };
-inline int loss_operand_map(CUtensorMap *map, const Operand &o, bool mn, int box_rows) {
+// Boxes of 64 values by box_rows rows of memory. The copy engine takes 4 to 6 cycles a row of a box, rows outside the matrix
+// included, so boxes are as high as the matrix where that is low: of 8 rows of x a box of 128 took most of a tile's time
+// ([8, 1792] . [1792, 109056] bf16 184 us). What the MMAs read beyond a box is of rows that no one stores.
+inline int loss_operand_map(CUtensorMap *map, const Operand &o, int box_rows) {
   const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.planes};
   const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)(o.pitch * o.plane_rows) * 2};
-  const uint32_t box[3] = {64, mn ? 64u : (uint32_t)box_rows, 1};
+  const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
   return encode_tiled(map, 0, 3, o.p, dims, strides, box, nullptr, 128);
 }
 
@@ -663,8 +671,12 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
     p.n_tiles = (p.N + S::kTileCols - 1) / S::kTileCols;
     tiles[i] = (int64_t)p.m_tiles * p.n_tiles * p.splits;
     cost[i] = p.split_blocks;
-    NB_TRY(loss_operand_map(&ma[i], oa[i], p.a_mn, kTileM));
-    NB_TRY(loss_operand_map(&mb[i], ob[i], p.b_mn, S::kCtaCols));
+    p.steps = p.kblocks == 1 ? (p.K + 15) / 16 : 4;
+    const int a_rows = p.a_mn ? 16 * p.steps : p.M < kTileM ? (p.M + 7) / 8 * 8 : kTileM;
+    const int b_rows = p.b_mn ? 16 * p.steps : S::kCtaCols;
+    p.tx_bytes = PL * kRowBytes * ((p.a_mn ? kTileM / 64 : 1) * a_rows + (p.b_mn ? S::kCtaCols / 64 : 1) * b_rows);
+    NB_TRY(loss_operand_map(&ma[i], oa[i], a_rows));
+    NB_TRY(loss_operand_map(&mb[i], ob[i], b_rows));
   }
   NB_CHECK(tiles[0] + tiles[1] < (1ll << 31), NB200_EVALUE, "too many rows and classes");
   if (prob.count == 1)
