@@ -260,20 +260,20 @@ Operand columns(Operand o, int64_t c0, int64_t n) {
   return o;
 }
 
-// Time of a launch's tiles, in cycles of an SM: rounds of 256 x 256 tiles on pairs of SMs, 512 MMA cycles a K block, or of
-// 128 x 64 ones, 204 (51 an instruction, for its operands' reads; 32 by its products); an epilogue at least, 4500 and 2000.
+// Whether a launch's tiles take less time as pairs of SMs' 256 x 256 ones than as 128 x 64 ones: the mean tile, in whole rounds.
 struct TileCount {
   int64_t M, N, kblocks;
+  int64_t splits = 1; // tiles along K, each of kblocks
 };
 bool pays_pairs(std::initializer_list<TileCount> products) {
   int64_t pair_tiles = 0, single_tiles = 0, pair_work = 0, single_work = 0;
   for (const TileCount &p : products) {
-    const int64_t pairs = ((p.M + 255) / 256) * ((p.N + 255) / 256), singles = ((p.M + 127) / 128) * ((p.N + 63) / 64);
+    const int64_t pairs = ((p.M + 255) / 256) * ((p.N + 255) / 256) * p.splits;
+    const int64_t singles = ((p.M + 127) / 128) * ((p.N + 63) / 64) * p.splits;
     pair_tiles += pairs, single_tiles += singles;
-    pair_work += pairs * std::max<int64_t>(512 * p.kblocks, 4500);
-    single_work += singles * std::max<int64_t>(204 * p.kblocks, 2000);
+    pair_work += pairs * loss_tile_cycles(p.kblocks, true);
+    single_work += singles * loss_tile_cycles(p.kblocks, false);
   }
-  // the mean tile, in whole rounds
   auto time = [](int64_t work, int64_t tiles, int64_t units) {
     return tiles == 0 ? 0 : (tiles + units - 1) / units * (work / tiles);
   };
@@ -412,8 +412,19 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
       p.vec = p.ldo * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
       a[prob.count] = og, b[prob.count++] = owc;
     }
-    if (prob.count)
+    if (!kF32 && prob.count == 2 && loss_is_long<T>(dx_blocks) != loss_is_long<T>(dw_blocks)) {
+      // (of two forms of the kernel: together both would take the one with eight epilogue warps)
+      for (int i = 0; i < 2; ++i) {
+        Products one = prob;
+        one.count = 1;
+        one.p[0] = prob.p[i];
+        const Product &p = one.p[0];
+        const int64_t blocks = p.splits > 1 ? p.split_blocks : p.kblocks;
+        NB_TRY((run_loss_gemm<T, Out::kStore>(pays_pairs({{p.M, p.N, blocks, std::max(1, p.splits)}}), one, a + i, b + i, st)));
+      }
+    } else if (prob.count) {
       NB_TRY((run_loss_gemm<T, Out::kStore>(pair, prob, a, b, st)));
+    }
     if (dw && dw_splits > 1)
       NB_TRY(add_parts<T>(dw32, dw_splits, size * piece, size, n, piece, nullptr, dw + c0, classes, accum[1], st));
     if (db)

@@ -630,6 +630,12 @@ inline int loss_operand_map(CUtensorMap *map, const Operand &o, int box_rows) {
   return encode_tiled(map, 0, 3, o.p, dims, strides, box, nullptr, 128);
 }
 
+// Time of a tile in cycles of an SM: 512 MMA cycles a K block of a pair's 256 x 256 tile, 204 of a 128 x 64 one (51 an
+// instruction, for its operands' reads; 32 by its products); its epilogue at least.
+inline int64_t loss_tile_cycles(int64_t kblocks, bool pair) {
+  return std::max<int64_t>((pair ? 512 : 204) * kblocks, pair ? 4500 : 2000);
+}
+
 // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
 // last four steps are the only ones on a large accumulator
 template <typename T> constexpr int loss_chunk() { return std::is_same<T, float>::value ? 1 : 24; }
@@ -670,7 +676,7 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
     p.m_tiles = (p.M + S::kTileRows - 1) / S::kTileRows;
     p.n_tiles = (p.N + S::kTileCols - 1) / S::kTileCols;
     tiles[i] = (int64_t)p.m_tiles * p.n_tiles * p.splits;
-    cost[i] = p.split_blocks;
+    cost[i] = loss_tile_cycles(p.split_blocks, kPair);
     p.steps = p.kblocks == 1 ? (p.K + 15) / 16 : 4;
     const int a_rows = p.a_mn ? 16 * p.steps : p.M < kTileM ? (p.M + 7) / 8 * 8 : kTileM;
     const int b_rows = p.b_mn ? 16 * p.steps : S::kCtaCols;
