@@ -15,27 +15,43 @@
 namespace nb200 {
 namespace {
 
-// The rows' loss and statistics from the tiles' maxima and sums: a warp a row.
-__global__ void __launch_bounds__(256) loss_rows_kernel(LossRows rows, int64_t count, float *__restrict__ loss,
+// The rows' loss and statistics from the tiles' maxima and sums: `share` of a block's eight warps a row (all of them where rows
+// are few and their tiles many: 3408 of nine rows took one warp each 17 us).
+__global__ void __launch_bounds__(256) loss_rows_kernel(LossRows rows, int64_t count, int share, float *__restrict__ loss,
                                                         float2 *__restrict__ stat) {
+  __shared__ float2 parts[8];
   pdl_wait();
   pdl_trigger();
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= count)
-    return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % share;
+  const int64_t row = (int64_t)blockIdx.x * (8 / share) + warp / share;
   MaxSum t{-INFINITY, 0.0f};
-  for (int i = lane; i < rows.tiles; i += 32) {
-    const float2 p = rows.partial[row * rows.tiles + i];
-    t = join(t, MaxSum{p.x, p.y}, kLog2e);
-  }
+  if (row < count)
+#pragma unroll 4
+    for (int i = mine * 32 + lane; i < rows.tiles; i += 32 * share) {
+      const float2 p = rows.partial[row * rows.tiles + i];
+      t = join(t, MaxSum{p.x, p.y}, kLog2e);
+    }
   t = warp_join(t, kLog2e);
-  if (lane == 0) {
+  if (share > 1) {
+    if (lane == 0)
+      parts[warp] = make_float2(t.m, t.s);
+    __syncthreads();
+    if (mine == 0)
+      for (int w = 1; w < share; ++w)
+        t = join(t, MaxSum{parts[warp + w].x, parts[warp + w].y}, kLog2e);
+  }
+  if (lane == 0 && mine == 0 && row < count) {
     const int64_t label = rows.label_of(row);
     const float log_sum = log2f(t.s) * kLn2;
     stat[row] = make_float2(t.m, log_sum);
     loss[row] = label < 0 ? 0.0f : label >= rows.classes ? NAN : (t.m - rows.target[row]) + log_sum;
   }
+}
+int loss_rows(const LossRows &r, int64_t count, float *loss, float2 *stat, cudaStream_t st) {
+  const int share = r.tiles > 64 && count <= 8 * sm_count() ? 8 : 1;
+  NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((count * share + 7) / 8)), dim3(256), 0, st, r, count, share, loss,
+                           stat));
+  return NB200_OK;
 }
 
 // Column sums of G, [planes][rows][ld]: a thread eight (fp32: four) neighbouring columns, a block's eight warps its slab of
@@ -322,7 +338,7 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
     prob.rows = r;
     prob.p[0].M = (int)n, prob.p[0].N = (int)classes, prob.p[0].K = (int)size, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
     NB_TRY((run_loss_gemm<T, Out::kSums>(pair, prob, &part, &ow, st)));
-    NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, r, n, loss + r0, stat + r0));
+    NB_TRY(loss_rows(r, n, loss + r0, stat + r0, st));
   }
   return NB200_OK;
 }
@@ -451,8 +467,7 @@ int forward(const T *x, const T *w, const T *bias, LossRows r, float *loss, floa
   NB_TRY(few_variant<T>(rows, vec, [&](auto n, auto v) {
     return few_logits<T, decltype(n)::value, decltype(v)::value>(x, w, bias, r, (int)rows, size, nullptr, 0, st);
   }));
-  NB_CUDA(launch_dependent(loss_rows_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, r, rows, loss, stat));
-  return NB200_OK;
+  return loss_rows(r, rows, loss, stat, st);
 }
 
 template <typename T>
