@@ -81,6 +81,8 @@ template <typename T> struct Run {
   }
 };
 
+// Measured at [4096, 128000] bf16, 64 entries a row: forward 186 us (5.7 TB/s), gradient 354 us (5.9 TB/s; 624 with a block a piece
+// of 8192 classes, each of which waited for the teacher's sums).
 constexpr int kSumThreads = 256;
 
 // One row a cluster of blocks (one block where the rows are many). stat: the row's maximum, and log sum exp((x - maximum) / tau).

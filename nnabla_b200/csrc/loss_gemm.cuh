@@ -17,6 +17,9 @@
 //   kGrad   G, in 16 bits (fp32: three bf16 planes)
 //   kStore  the product itself, two products (dx and dW of a piece of the classes) in one launch: with one after the other,
 //           each would end in a round of tiles that leaves SMs idle
+//
+// Bound by the tensor pipe: 1500 to 1600 TFLOP/s in bf16 ([8192, 2048] . [2048, 128000]: the logits 2.68 ms, G of 8192 classes
+// 0.19, both gradients of such a piece 0.37), which the power limit brings down to 1240 over a whole step.
 #pragma once
 #include "gemm2.cuh"
 #include "softmax_sums.cuh"

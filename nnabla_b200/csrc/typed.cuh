@@ -109,9 +109,6 @@ template <typename T> constexpr int kPackOf = (int)(16 / sizeof(T)); // values i
 __device__ __forceinline__ void cp_async16(void *to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
-__device__ __forceinline__ void cp_async4(void *to, const void *from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -138,7 +135,6 @@ template <typename F> int with_type(int code, F f) {
   return fail(NB200_EVALUE, "unknown type code %d", code);
 }
 inline size_t type_bytes(int code) { return code == NB200_F32 ? 4 : 2; }
-inline bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 } // namespace nb200
