@@ -140,19 +140,17 @@ int add_parts(const float *from, int parts, int64_t stride, int64_t rows, int64_
   return NB200_OK;
 }
 
-// db (+)= the column sums of G [planes * rows][ld], of which `part` holds slabs() rows of ld sums.
-template <typename G> int64_t column_slabs(int64_t all_rows, int64_t columns) {
-  const int64_t wide = (columns + 32 * kPackOf<G> - 1) / (32 * kPackOf<G>);
-  return std::max<int64_t>(1, std::min<int64_t>((all_rows + 31) / 32, 4 * sm_count() / wide));
-}
+// db (+)= the column sums of G [planes * rows][ld], of which `part`, room floats of scratch, holds a row of ld sums for each slab.
 template <typename G, typename T>
-int column_sums(const G *g, int64_t all_rows, int64_t columns, int64_t ld, float *part, const float *scale, T *db, bool accum,
-                cudaStream_t st) {
-  const int64_t slabs = column_slabs<G>(all_rows, columns), slab = (all_rows + slabs - 1) / slabs;
-  const int64_t count = (all_rows + slab - 1) / slab, wide = (columns + 32 * kPackOf<G> - 1) / (32 * kPackOf<G>);
-  NB_CUDA(launch_dependent(column_sums_kernel<G>, dim3((unsigned)wide, (unsigned)count), dim3(256), 0, st, g, all_rows, slab,
-                           columns, ld, part, ld));
-  return add_parts<T>(part, (int)count, ld, 1, columns, ld, scale, db, 0, accum, st);
+int column_sums(const G *g, int64_t all_rows, Slabs slabs, int64_t columns, int64_t ld, float *part, int64_t room,
+                const float *scale, T *db, bool accum, cudaStream_t st) {
+  static_assert(32 * kPackOf<G> == kSumColumns, "a block's columns");
+  NB_CHECK(slabs.count * ld <= room && slabs.count * slabs.rows >= all_rows, NB200_EVALUE, "sums of %lld slabs of %lld classes",
+           (long long)slabs.count, (long long)ld);
+  const int64_t wide = (columns + kSumColumns - 1) / kSumColumns;
+  NB_CUDA(launch_dependent(column_sums_kernel<G>, dim3((unsigned)wide, (unsigned)slabs.count), dim3(256), 0, st, g, all_rows,
+                           slabs.rows, columns, ld, part, ld));
+  return add_parts<T>(part, (int)slabs.count, ld, 1, columns, ld, scale, db, 0, accum, st);
 }
 
 // What the tensor-core products need before they start, in one launch: up to two matrices laid out as operands (fp32: three
@@ -244,8 +242,6 @@ template <typename T> __global__ void __launch_bounds__(256) loss_prepare_kernel
   }
 }
 
-int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-
 // A matrix as an operand of the tensor-core products: as it lies, or laid out anew in operand_bytes() of scratch.
 template <typename T> size_t operand_bytes(const T *p, int64_t rows, int64_t cols) {
   if (std::is_same<T, float>::value)
@@ -276,41 +272,11 @@ Operand columns(Operand o, int64_t c0, int64_t n) {
   return o;
 }
 
-// Whether a launch's tiles take less time as pairs of SMs' 256 x 256 ones than as 128 x 64 ones: the mean tile, in whole rounds.
-struct TileCount {
-  int64_t M, N, kblocks;
-  int64_t splits = 1; // tiles along K, each of kblocks
-};
-bool pays_pairs(std::initializer_list<TileCount> products) {
-  int64_t pair_tiles = 0, single_tiles = 0, pair_work = 0, single_work = 0;
-  for (const TileCount &p : products) {
-    const int64_t pairs = ((p.M + 255) / 256) * ((p.N + 255) / 256) * p.splits;
-    const int64_t singles = ((p.M + 127) / 128) * ((p.N + 63) / 64) * p.splits;
-    pair_tiles += pairs, single_tiles += singles;
-    pair_work += pairs * loss_tile_cycles(p.kblocks, true);
-    single_work += singles * loss_tile_cycles(p.kblocks, false);
-  }
-  auto time = [](int64_t work, int64_t tiles, int64_t units) {
-    return tiles == 0 ? 0 : (tiles + units - 1) / units * (work / tiles);
-  };
-  return time(pair_work, pair_tiles, sm_count() / 2) <= time(single_work, single_tiles, sm_count());
-}
-
-// Scratch for a call, in parts that begin at 256-byte boundaries.
-struct Parts {
-  size_t bytes = 0;
-  size_t take(size_t n) {
-    const size_t at = bytes;
-    bytes += (n + 255) / 256 * 256;
-    return at;
-  }
-};
-
 template <typename T>
 int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *loss, float2 *stat, int64_t rows, int64_t size,
                    int64_t classes, cudaStream_t st) {
   const int kblocks = (int)((size + 63) / 64);
-  const bool pair = pays_pairs({{rows, classes, kblocks}});
+  const bool pair = pays_pairs({{rows, classes, kblocks}}, sm_count());
   r.tiles = loss_sum_tiles<T>(classes, kblocks, pair);
   // so many rows at a time that their maxima and sums are 64 MB (the largest head in use: 8192 rows of 128000 classes)
   const int64_t slab = std::min(rows, std::max<int64_t>(256, (1 << 23) / r.tiles / 256 * 256));
@@ -349,68 +315,40 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kPlanes = kF32 ? 3 : 1;
   using G = std::conditional_t<kF32, __nv_bfloat16, T>;
-  // A piece's G is 64 MB: both products read it from L2, and their tiles are rounds enough to leave few SMs idle.
-  int64_t piece = std::max<int64_t>(256, (int64_t)(1 << 25) / kPlanes / rows);
-  const int64_t count = (classes + piece - 1) / piece;
-  piece = up((classes + count - 1) / count, 256);
-  const bool pieces = piece < classes;
-  const int64_t size_blocks = (size + 63) / 64, row_blocks = (rows + 63) / 64, piece_blocks = (std::min(piece, classes) + 63) / 64;
-  const bool pair_grad = pays_pairs({{rows, piece, size_blocks}});
-  const bool pair = pays_pairs({{dw ? size : 0, piece, row_blocks}, {dx ? rows : 0, size, piece_blocks}});
-  // A product with few tiles and a long K (dx of few rows, dW of many) has it in up to 16 parts, each with sums of its own that
-  // add_parts joins, until a tile is a third of an SM's share at most.
-  const int64_t tile_m = pair ? 256 : 128, tile_n = pair ? 256 : 64, units = pair ? sm_count() / 2 : sm_count();
-  const int64_t dw_tiles = dw ? (size + tile_m - 1) / tile_m * ((piece + tile_n - 1) / tile_n) : 0;
-  const int64_t dx_tiles = dx ? (rows + tile_m - 1) / tile_m * ((size + tile_n - 1) / tile_n) : 0;
-  const int64_t share = std::max<int64_t>(8, (dw_tiles * row_blocks + dx_tiles * piece_blocks) / (3 * units));
-  auto split = [&](int64_t tiles, int64_t blocks, int &splits, int &split_blocks) {
-    splits = 1;
-    while (splits < 16 && tiles * splits < 4 * units && blocks > share * splits)
-      splits *= 2;
-    split_blocks = (int)((blocks + splits - 1) / splits);
-    splits = (int)((blocks + split_blocks - 1) / split_blocks); // no empty part (a last, smaller piece may leave some)
-  };
-  int dx_splits, dx_blocks, dw_splits, dw_blocks;
-  split(dx_tiles, piece_blocks, dx_splits, dx_blocks);
-  split(dw_tiles, row_blocks, dw_splits, dw_blocks);
-  const bool direct = dx_splits == 1 && (!pieces || (kF32 && !accum[0])); // dx without sums of its own
-  Parts parts;
-  const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
-  const size_t at_g = parts.take((size_t)kPlanes * rows * piece * 2), at_scale = parts.take(12);
-  const int64_t ld_dx = up(size, 4); // of dx's own sums
-  const size_t at_dx = parts.take(dx && !direct ? (size_t)dx_splits * rows * ld_dx * 4 : 0);
-  const size_t at_dw = parts.take(dw && dw_splits > 1 ? (size_t)dw_splits * size * piece * 4 : 0);
-  const size_t at_db = parts.take(db ? (size_t)column_slabs<G>(kPlanes * rows, piece) * piece * 4 : 0);
+  const HeadGradients plan(rows, size, classes, kF32, dx, dw, db, accum[0], operand_bytes(x, rows, size),
+                           operand_bytes(w, size, classes), sm_count());
+  const int64_t piece = plan.piece, ld_dx = plan.ld_dx;
+  const bool direct = plan.direct;
   AsyncScratch scratch(st);
-  NB_TRY(scratch.alloc(parts.bytes));
+  NB_TRY(scratch.alloc(plan.bytes));
   char *base = static_cast<char *>(scratch.p);
-  float *dx32 = reinterpret_cast<float *>(base + at_dx), *dw32 = reinterpret_cast<float *>(base + at_dw);
-  float *scale = reinterpret_cast<float *>(base + at_scale);
+  float *dx32 = reinterpret_cast<float *>(base + plan.at_dx), *dw32 = reinterpret_cast<float *>(base + plan.at_dw);
+  float *scale = reinterpret_cast<float *>(base + plan.at_scale);
   Preparation pre{};
-  const Operand ox = operand(x, rows, size, base + at_x, pre.m[0]), ow = operand(w, size, classes, base + at_w, pre.m[1]);
+  const Operand ox = operand(x, rows, size, base + plan.at_x, pre.m[0]), ow = operand(w, size, classes, base + plan.at_w, pre.m[1]);
   pre.rows = r, pre.count = rows, pre.scale = scale, pre.times = std::is_same<T, __half>::value ? 16384.0f : 1.0f;
   NB_TRY(prepare<T>(pre, st));
   r.scale = scale;
   for (int64_t c0 = 0; c0 < classes; c0 += piece) {
-    const int64_t n = std::min(piece, classes - c0);
-    const Operand og{base + at_g, rows, n, piece, kPlanes, rows}, owc = columns(ow, c0, n);
+    const int64_t n = plan.classes_at(c0);
+    const Operand og{base + plan.at_g, rows, n, piece, kPlanes, rows}, owc = columns(ow, c0, n);
     Products prob{};
     prob.count = 1;
     prob.bias = bias;
     prob.class0 = (int)c0;
     prob.rows = r;
     Product &l = prob.p[0];
-    l.M = (int)rows, l.N = (int)n, l.K = (int)size, l.kblocks = (int)size_blocks, l.b_mn = 1;
-    l.out = base + at_g, l.ldo = piece, l.stride = rows * piece;
-    NB_TRY((run_loss_gemm<T, Out::kGrad>(pair_grad, prob, &ox, &owc, st)));
+    l.M = (int)rows, l.N = (int)n, l.K = (int)size, l.kblocks = (int)((size + 63) / 64), l.b_mn = 1;
+    l.out = base + plan.at_g, l.ldo = piece, l.stride = rows * piece;
+    NB_TRY((run_loss_gemm<T, Out::kGrad>(plan.pair_grad, prob, &ox, &owc, st)));
     Operand a[2], b[2];
     prob.count = 0;
     if (dw) {
       Product &p = prob.p[prob.count];
       p = Product{};
-      p.M = (int)size, p.N = (int)n, p.K = (int)rows, p.kblocks = (int)row_blocks, p.a_mn = p.b_mn = 1;
-      if (dw_splits > 1) {
-        p.splits = dw_splits, p.split_blocks = dw_blocks, p.stride = size * piece;
+      p.M = (int)size, p.N = (int)n, p.K = (int)rows, p.kblocks = (int)((rows + 63) / 64), p.a_mn = p.b_mn = 1;
+      if (plan.dw_splits > 1) {
+        p.splits = plan.dw_splits, p.split_blocks = plan.dw_blocks, p.stride = size * piece;
         p.out = dw32, p.ldo = piece, p.out_f32 = 1, p.vec = 1;
       } else {
         p.out = dw + c0, p.ldo = classes, p.accum = accum[1];
@@ -422,13 +360,13 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
       Product &p = prob.p[prob.count];
       p = Product{};
       p.M = (int)rows, p.N = (int)size, p.K = (int)n, p.kblocks = (int)((n + 63) / 64), p.ldo = direct ? size : ld_dx;
-      p.splits = (p.kblocks + dx_blocks - 1) / dx_blocks, p.split_blocks = dx_blocks, p.stride = rows * ld_dx;
+      p.splits = (p.kblocks + plan.dx_blocks - 1) / plan.dx_blocks, p.split_blocks = plan.dx_blocks, p.stride = rows * ld_dx;
       p.out = direct ? static_cast<void *>(dx) : dx32, p.out_f32 = !direct;
       p.accum = c0 > 0 || (direct && accum[0]);
       p.vec = p.ldo * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
       a[prob.count] = og, b[prob.count++] = owc;
     }
-    if (!kF32 && prob.count == 2 && loss_is_long<T>(dx_blocks) != loss_is_long<T>(dw_blocks)) {
+    if (!kF32 && prob.count == 2 && loss_is_long<T>(plan.dx_blocks) != loss_is_long<T>(plan.dw_blocks)) {
       // (of two forms of the kernel: together both would take the one with eight epilogue warps)
       for (int i = 0; i < 2; ++i) {
         Products one = prob;
@@ -436,19 +374,21 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
         one.p[0] = prob.p[i];
         const Product &p = one.p[0];
         const int64_t blocks = p.splits > 1 ? p.split_blocks : p.kblocks;
-        NB_TRY((run_loss_gemm<T, Out::kStore>(pays_pairs({{p.M, p.N, blocks, std::max(1, p.splits)}}), one, a + i, b + i, st)));
+        NB_TRY((run_loss_gemm<T, Out::kStore>(pays_pairs({{p.M, p.N, blocks, std::max(1, p.splits)}}, sm_count()), one, a + i,
+                                               b + i, st)));
       }
     } else if (prob.count) {
-      NB_TRY((run_loss_gemm<T, Out::kStore>(pair, prob, a, b, st)));
+      NB_TRY((run_loss_gemm<T, Out::kStore>(plan.pair, prob, a, b, st)));
     }
-    if (dw && dw_splits > 1)
-      NB_TRY(add_parts<T>(dw32, dw_splits, size * piece, size, n, piece, nullptr, dw + c0, classes, accum[1], st));
+    if (dw && plan.dw_splits > 1)
+      NB_TRY(add_parts<T>(dw32, plan.dw_splits, size * piece, size, n, piece, nullptr, dw + c0, classes, accum[1], st));
     if (db)
-      NB_TRY((column_sums<G, T>(reinterpret_cast<const G *>(base + at_g), kPlanes * rows, n, piece,
-                                reinterpret_cast<float *>(base + at_db), scale, db + c0, accum[2], st)));
+      NB_TRY((column_sums<G, T>(reinterpret_cast<const G *>(base + plan.at_g), kPlanes * rows, plan.db, n, piece,
+                                reinterpret_cast<float *>(base + plan.at_db), (int64_t)(plan.bytes - plan.at_db) / 4, scale,
+                                db + c0, accum[2], st)));
   }
   if (dx && !direct)
-    NB_TRY(add_parts<T>(dx32, dx_splits, rows * ld_dx, rows, size, ld_dx, nullptr, dx, size, accum[0], st));
+    NB_TRY(add_parts<T>(dx32, plan.dx_splits, rows * ld_dx, rows, size, ld_dx, nullptr, dx, size, accum[0], st));
   return NB200_OK;
 }
 

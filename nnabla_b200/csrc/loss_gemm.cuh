@@ -22,6 +22,7 @@
 // 0.19, both gradients of such a piece 0.37), which the power limit brings down to 1240 over a whole step.
 #pragma once
 #include "gemm2.cuh"
+#include "loss_plan.h"
 #include "softmax_sums.cuh"
 
 namespace nb200 {
@@ -631,12 +632,6 @@ inline int loss_operand_map(CUtensorMap *map, const Operand &o, int box_rows) {
   const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)(o.pitch * o.plane_rows) * 2};
   const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
   return encode_tiled(map, 0, 3, o.p, dims, strides, box, nullptr, 128);
-}
-
-// Time of a tile in cycles of an SM: 512 MMA cycles a K block of a pair's 256 x 256 tile, 204 of a 128 x 64 one (51 an
-// instruction, for its operands' reads; 32 by its products); its epilogue at least.
-inline int64_t loss_tile_cycles(int64_t kblocks, bool pair) {
-  return std::max<int64_t>((pair ? 512 : 204) * kblocks, pair ? 4500 : 2000);
 }
 
 // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose

@@ -1,0 +1,119 @@
+// The arithmetic of a head's products on the host: tiles, pieces, and where a call's scratch holds what. No CUDA, so that it can
+// be gone through for any size and number of SMs without a GPU.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <initializer_list>
+
+namespace nb200 {
+
+inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// Scratch for a call, in parts that begin at 256-byte boundaries.
+struct Parts {
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+};
+
+// Time of a tile in cycles of an SM: 512 MMA cycles a K block of a pair's 256 x 256 tile, 204 of a 128 x 64 one (51 an
+// instruction, for its operands' reads; 32 by its products); its epilogue at least.
+inline int64_t loss_tile_cycles(int64_t kblocks, bool pair) {
+  return std::max<int64_t>((pair ? 512 : 204) * kblocks, pair ? 4500 : 2000);
+}
+
+// Whether a launch's tiles take less time as pairs of SMs' 256 x 256 ones than as 128 x 64 ones: the mean tile, in whole rounds.
+struct TileCount {
+  int64_t M, N, kblocks;
+  int64_t splits = 1; // tiles along K, each of kblocks
+};
+inline bool pays_pairs(std::initializer_list<TileCount> products, int sms) {
+  int64_t pair_tiles = 0, single_tiles = 0, pair_work = 0, single_work = 0;
+  for (const TileCount &p : products) {
+    const int64_t pairs = ((p.M + 255) / 256) * ((p.N + 255) / 256) * p.splits;
+    const int64_t singles = ((p.M + 127) / 128) * ((p.N + 63) / 64) * p.splits;
+    pair_tiles += pairs, single_tiles += singles;
+    pair_work += pairs * loss_tile_cycles(p.kblocks, true);
+    single_work += singles * loss_tile_cycles(p.kblocks, false);
+  }
+  auto time = [](int64_t work, int64_t tiles, int64_t units) {
+    return tiles == 0 ? 0 : (tiles + units - 1) / units * (work / tiles);
+  };
+  return time(pair_work, pair_tiles, sms / 2) <= time(single_work, single_tiles, sms);
+}
+
+// The rows of a matrix in slabs, each of whose column sums a block makes for itself (256 columns a block).
+constexpr int kSumColumns = 256;
+struct Slabs {
+  int64_t rows, count; // of a slab; slabs
+};
+inline Slabs column_slabs(int64_t all_rows, int64_t columns, int sms) {
+  const int64_t wide = (columns + kSumColumns - 1) / kSumColumns;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>((all_rows + 31) / 32, 4 * sms / wide));
+  const int64_t rows = (all_rows + most - 1) / most;
+  return {rows, (all_rows + rows - 1) / rows};
+}
+
+// A head's gradients on the tensor cores: the pieces of the classes, the tiles and parts of K of the products, and what of it
+// lies where in the scratch. `planes`: three bf16 pieces an fp32 value, or one of 16 bits.
+struct HeadGradients {
+  int planes;
+  int64_t rows, size, classes;
+  int64_t piece;        // classes at a time, a multiple of 256; the last piece has what is left
+  bool pieces;          // more than one
+  bool pair_grad, pair; // tiles of G, of dx and dW
+  int dx_splits, dx_blocks, dw_splits, dw_blocks; // parts of K, K blocks of each
+  bool direct;          // dx without sums of its own
+  int64_t ld_dx;        // of dx's own sums
+  Slabs db; // of G's rows, the same ones for every piece: with fewer classes a piece of its own would have more of them
+  // of the scratch: the operands, G [planes][rows][piece], its scale, fp32 sums [dx_splits][rows][ld_dx],
+  // [dw_splits][size][piece], [db.count][piece]
+  size_t at_x, at_w, at_g, at_scale, at_dx, at_dw, at_db, bytes;
+
+  int64_t classes_at(int64_t c0) const { return std::min(piece, classes - c0); }
+
+  HeadGradients(int64_t rows_, int64_t size_, int64_t classes_, bool f32, bool dx, bool dw, bool with_db, bool accum_dx,
+                size_t x_bytes, size_t w_bytes, int sms)
+      : planes(f32 ? 3 : 1), rows(rows_), size(size_), classes(classes_) {
+    // A piece's G is 64 MB: both products read it from L2, and their tiles are rounds enough to leave few SMs idle.
+    piece = std::max<int64_t>(256, (int64_t)(1 << 25) / planes / rows);
+    const int64_t count = (classes + piece - 1) / piece;
+    piece = up((classes + count - 1) / count, 256);
+    pieces = piece < classes;
+    const int64_t size_blocks = (size + 63) / 64, row_blocks = (rows + 63) / 64, piece_blocks = (std::min(piece, classes) + 63) / 64;
+    pair_grad = pays_pairs({{rows, piece, size_blocks}}, sms);
+    pair = pays_pairs({{dw ? size : 0, piece, row_blocks}, {dx ? rows : 0, size, piece_blocks}}, sms);
+    // A product with few tiles and a long K (dx of few rows, dW of many) has it in up to 16 parts, each with sums of its own that
+    // add_parts joins, until a tile is a third of an SM's share at most.
+    const int64_t tile_m = pair ? 256 : 128, tile_n = pair ? 256 : 64, units = pair ? sms / 2 : sms;
+    const int64_t dw_tiles = dw ? (size + tile_m - 1) / tile_m * ((piece + tile_n - 1) / tile_n) : 0;
+    const int64_t dx_tiles = dx ? (rows + tile_m - 1) / tile_m * ((size + tile_n - 1) / tile_n) : 0;
+    const int64_t share = std::max<int64_t>(8, (dw_tiles * row_blocks + dx_tiles * piece_blocks) / (3 * units));
+    auto split = [&](int64_t tiles, int64_t blocks, int &splits, int &split_blocks) {
+      splits = 1;
+      while (splits < 16 && tiles * splits < 4 * units && blocks > share * splits)
+        splits *= 2;
+      split_blocks = (int)((blocks + splits - 1) / splits);
+      splits = (int)((blocks + split_blocks - 1) / split_blocks); // no empty part (a last, smaller piece may leave some)
+    };
+    split(dx_tiles, piece_blocks, dx_splits, dx_blocks);
+    split(dw_tiles, row_blocks, dw_splits, dw_blocks);
+    direct = dx_splits == 1 && (!pieces || (f32 && !accum_dx));
+    ld_dx = up(size, 4);
+    db = column_slabs(planes * rows, piece, sms);
+    Parts parts;
+    at_x = parts.take(x_bytes), at_w = parts.take(w_bytes);
+    at_g = parts.take((size_t)planes * rows * piece * 2), at_scale = parts.take(12);
+    at_dx = parts.take(dx && !direct ? (size_t)dx_splits * rows * ld_dx * 4 : 0);
+    at_dw = parts.take(dw && dw_splits > 1 ? (size_t)dw_splits * size * piece * 4 : 0);
+    at_db = parts.take(with_db ? (size_t)db.count * piece * 4 : 0);
+    bytes = parts.bytes;
+  }
+};
+
+} // namespace nb200
