@@ -169,9 +169,10 @@ struct Preparation {
   float *scale;
 };
 
-// scale = {the largest |dloss| of a row that counts, 2^e, their quotient}: what G is kept relative to. With the largest taken
-// out, the gradient of a mean, the same in every row, is no rounded factor of G: at the label G is -1 + p. e is 14 for an fp16 G,
-// which so has eleven bits down to 2^-28 of the largest gradient, and 0 for the others.
+// scale = {the largest finite |dloss| of a row whose label is a class, 2^e, their quotient}: what G is kept relative to (the other
+// rows of G are 0, infinite or NaN whatever it is, and no gradient of theirs changes how another row is rounded). With the
+// largest taken out, the gradient of a mean, the same in every row, is no rounded factor of G: at the label G is -1 + p. e is 14
+// for an fp16 G, which so has eleven bits down to 2^-28 of the largest gradient, and 0 for the others.
 __device__ void gradient_scale(const Preparation &p) {
   __shared__ float tops[8];
   float top = 0.0f;
@@ -179,7 +180,7 @@ __device__ void gradient_scale(const Preparation &p) {
   for (int64_t r = threadIdx.x; r < p.count; r += 256) {
     const int64_t label = p.rows.label_of(r);
     const float d = fabsf(p.rows.dloss[r]);
-    top = fmaxf(top, label >= 0 ? d : 0.0f);
+    top = fmaxf(top, label >= 0 && label < p.rows.classes && d < INFINITY ? d : 0.0f);
   }
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0)
@@ -189,8 +190,7 @@ __device__ void gradient_scale(const Preparation &p) {
 #pragma unroll
     for (int w = 1; w < 8; ++w)
       top = fmaxf(top, tops[w]);
-    // (none, or one that is not finite: G as it is)
-    const bool plain = !(top >= 1.17549435e-38f && top < INFINITY);
+    const bool plain = !(top >= 1.17549435e-38f); // none, or none that can be divided by
     p.scale[0] = plain ? 1.0f : top;
     p.scale[1] = p.times;
     p.scale[2] = (plain ? 1.0f : top) / p.times;

@@ -1,0 +1,46 @@
+"""affine_softmax_cross_entropy_backward where one row's gradient says nothing of the others'. Tolerances as in test_affine_loss_gpu."""
+import math
+
+import pytest
+import torch
+
+from nnabla_b200 import functions as F
+from test_affine_loss_gpu import TYPES, data, reference, rms
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_of_dx(x, w, label, bias, dloss, keep):
+    """dx of the rows `keep` against the formula of these rows alone: a row of dx depends on nothing else."""
+    loss, stat = F.affine_softmax_cross_entropy(x, w, label, bias, output_stat=True)
+    dx = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias)[0][keep].double()
+    logits, _, _, G = reference(x[keep], w, label[keep], bias, dloss[keep])
+    half, dl = torch.finfo(x.dtype).eps / 2, dloss[keep].double()
+    e = 1e-5 * rms(logits) + 1e-6
+    relative = 2 * e + (half if x.dtype != torch.float32 else 2.0 ** -20)
+    floor = float(dl.abs().max()) * 2.0 ** -38 if x.dtype == torch.float16 else 0.0
+    dG = G.abs() * relative + floor + dl.abs() * 1e-6 * (label[keep] == torch.arange(w.shape[1], device="cuda"))
+    want = G @ w.double().t()
+    tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    bound = dG @ w.double().abs().t() + half * want.abs() * 1.01 + 1e-5 * rms(want) + tiny
+    bad = ~((dx - want).abs() <= bound)
+    assert not bad.any(), (int(bad.sum()), float(((dx - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 40, 300])
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+def test_a_gradient_that_is_not_finite_stays_in_its_row(dtype, rows, what):
+    x, w, label, bias, dloss = data(rows, 96, 500, dtype, ignored=0.0)
+    dloss = torch.sign(dloss) * 100.0
+    dloss[3] = what
+    rows_of_dx(x, w, label, bias, dloss, [i for i in range(rows) if i != 3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 40])
+def test_a_row_whose_label_does_not_exist_sets_no_scale(dtype, rows):
+    x, w, label, bias, dloss = data(rows, 96, 500, dtype, ignored=0.0)
+    label[3], dloss[3] = 500, 1e30
+    label[4], dloss[4] = -1, 1e30
+    rows_of_dx(x, w, label, bias, dloss, [i for i in range(rows) if i not in (3, 4)])
