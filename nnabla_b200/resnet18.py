@@ -207,7 +207,8 @@ def head_loss(features, weight, bias, label, teacher=None, temperature=4.0, shar
 
     features [rows, inputs], weight [inputs, classes], bias [classes]: one type (float32, bfloat16 or float16 for the cross
     entropy alone, float32 with a teacher). label [rows, 1]: int32 or int64. teacher: (index, logits) of each row's best
-    classes, as functions.top_k_distillation takes them, or None (share is then 0). Without a teacher no logits are made.
+    classes, as functions.top_k_distillation takes them, or None (share is then 0); of a row that does not count neither is
+    looked at. Without a teacher no logits are made.
     Returns (loss, (dfeatures, dweight, dbias)), the loss a float32 tensor of one value."""
     from . import functions as F
     counts = label >= 0
@@ -219,6 +220,7 @@ def head_loss(features, weight, bias, label, teacher=None, temperature=4.0, shar
     grads = F.affine_softmax_cross_entropy_backward(features, weight, label, stat, (1.0 - share) * each, bias)
     if teacher is not None:
         index, best = teacher
+        index = index.masked_fill(~counts, -1)  # no entries: the loss and the gradient of such a row are 0, not 0 times them
         logits = F.affine(features, weight, bias)
         loss, stat = F.top_k_distillation(logits, index, best, temperature, output_stat=True)
         total = total + share * (loss * each).sum()

@@ -1,0 +1,42 @@
+"""resnet18.head_loss: rows that do not count, whatever the teacher says of them."""
+import math
+
+import pytest
+import torch
+
+from nnabla_b200 import resnet18
+from test_training_head_gpu import data
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b):
+    return torch.equal(a[0], b[0]) and all(torch.equal(p, q) for p, q in zip(a[1], b[1]))
+
+
+@pytest.mark.parametrize("rows", [5, 60])
+def test_the_teacher_of_a_row_that_does_not_count(rows):
+    _, _, _, w, b, label, index, best = data(rows, 48, 100, torch.float32)
+    x = torch.randn((rows, 48), device="cuda")
+    assert label[0] == -1
+    b[17] = -math.inf  # ruled out by the student; no row that counts names it
+    index[index == 17] = -1
+    clean = index.clone()
+    clean[0] = -1
+    want = resnet18.head_loss(x, w, b, label, (clean, best), temperature=2.0, share=0.3)
+    assert torch.isfinite(want[0]) and all(torch.isfinite(g).all() for g in want[1])
+    for entry, logit in [(100, 1.0), (1 << 20, 1.0), (17, 1.0), (3, math.nan), (3, math.inf)]:
+        row, kept = index.clone(), best.clone()
+        row[0, 0], kept[0, 0] = entry, logit
+        given = row.clone()
+        assert same(resnet18.head_loss(x, w, b, label, (row, kept), temperature=2.0, share=0.3), want), (entry, logit)
+        assert torch.equal(row, given)  # the caller's tensor stays
+
+
+def test_no_row_counts():
+    _, _, _, w, b, label, index, best = data(12, 48, 100, torch.float32)
+    x = torch.randn((12, 48), device="cuda")
+    label.fill_(-1)
+    index[3, 0] = 100
+    loss, grads = resnet18.head_loss(x, w, b, label, (index, best))
+    assert loss == 0 and all((g == 0).all() for g in grads)
