@@ -206,11 +206,12 @@ def head_loss(features, weight, bias, label, teacher=None, temperature=4.0, shar
     (1 - share) * softmax cross entropy + share * distillation from a teacher's best classes.
 
     features [rows, inputs], weight [inputs, classes], bias [classes]: one type (float32, bfloat16 or float16 for the cross
-    entropy alone, float32 with a teacher). label [rows, 1]: int32 or int64. teacher: (index, logits) of each row's best
+    entropy alone, float32 with a teacher). label [rows, 1] or [rows]: int32 or int64. teacher: (index, logits) of each row's best
     classes, as functions.top_k_distillation takes them, or None (share is then 0); of a row that does not count neither is
     looked at. Without a teacher no logits are made.
     Returns (loss, (dfeatures, dweight, dbias)), the loss a float32 tensor of one value."""
     from . import functions as F
+    label = label.reshape(-1, 1)  # (beside the losses, [rows, 1], a vector would spread to a matrix)
     counts = label >= 0
     each = counts.float() / counts.sum().clamp(min=1)  # the weight of a row in the mean
     if teacher is None:

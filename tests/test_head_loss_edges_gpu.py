@@ -40,3 +40,14 @@ def test_no_row_counts():
     index[3, 0] = 100
     loss, grads = resnet18.head_loss(x, w, b, label, (index, best))
     assert loss == 0 and all((g == 0).all() for g in grads)
+
+
+@pytest.mark.parametrize("teacher", [False, True])
+def test_labels_as_a_vector(teacher):
+    _, _, _, w, b, label, index, best = data(30, 48, 100, torch.float32)
+    x = torch.randn((30, 48), device="cuda")
+    given = (index, best) if teacher else None
+    want = resnet18.head_loss(x, w, b, label, given)
+    assert same(resnet18.head_loss(x, w, b, label[:, 0], given), want)
+    with pytest.raises(RuntimeError, match="label"):
+        resnet18.head_loss(x, w, b, label[:29, 0], given)
