@@ -205,11 +205,11 @@ def head_loss(features, weight, bias, label, teacher=None, temperature=4.0, shar
     """The head's loss and its gradients: the mean, over the rows whose label is not negative, of
     (1 - share) * softmax cross entropy + share * distillation from a teacher's best classes.
 
-    features [rows, inputs], weight [inputs, classes], bias [classes]: one type (float32, bfloat16 or float16 for the cross
-    entropy alone, float32 with a teacher). label [rows, 1] or [rows]: int32 or int64. teacher: (index, logits) of each row's best
-    classes, as functions.top_k_distillation takes them, or None (share is then 0); of a row that does not count neither is
-    looked at. Without a teacher no logits are made.
-    Returns (loss, (dfeatures, dweight, dbias)), the loss a float32 tensor of one value."""
+    features [rows, inputs], weight [inputs, classes], bias [classes] or None: one type (float32, bfloat16 or float16 for the
+    cross entropy alone, float32 with a teacher). label [rows, 1] or [rows]: int32 or int64. teacher: (index, logits) of each
+    row's best classes, as functions.top_k_distillation takes them, or None (share is then 0); of a row that does not count
+    neither is looked at. Without a teacher no logits are made.
+    Returns (loss, (dfeatures, dweight, dbias)), the loss a float32 tensor of one value, dbias None without a bias."""
     from . import functions as F
     label = label.reshape(-1, 1)  # (beside the losses, [rows, 1], a vector would spread to a matrix)
     counts = label >= 0
@@ -227,7 +227,8 @@ def head_loss(features, weight, bias, label, teacher=None, temperature=4.0, shar
         total = total + share * (loss * each).sum()
         # (in place: the logits are not needed any more)
         dlogits = F.top_k_distillation_backward(logits, index, best, stat, share * each, temperature, dx=logits)
-        grads = F.affine_backward(features, weight, dlogits, accum=(True, True, True), grads=grads)
+        grads = F.affine_backward(features, weight, dlogits, propagate_down=(True, True, bias is not None),
+                                  accum=(True, True, True), grads=grads)
     return total, grads
 
 

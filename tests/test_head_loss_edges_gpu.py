@@ -51,3 +51,13 @@ def test_labels_as_a_vector(teacher):
     assert same(resnet18.head_loss(x, w, b, label[:, 0], given), want)
     with pytest.raises(RuntimeError, match="label"):
         resnet18.head_loss(x, w, b, label[:29, 0], given)
+
+
+@pytest.mark.parametrize("teacher", [False, True])
+def test_a_head_without_bias(teacher):
+    _, _, _, w, b, label, index, best = data(30, 48, 100, torch.float32)
+    x = torch.randn((30, 48), device="cuda")
+    given = (index, best) if teacher else None
+    loss, (dx, dw, db) = resnet18.head_loss(x, w, None, label, given)
+    want = resnet18.head_loss(x, w, torch.zeros_like(b), label, given)
+    assert db is None and same((loss, (dx, dw)), (want[0], want[1][:2]))
