@@ -1010,7 +1010,7 @@ struct Head {
     if (!p.ok)
       return;
     rows = x->size(0), size = x->size(1), classes = w->size(1);
-    p.require(label->size(0) == rows && label->numel() == rows && label->dim() <= 2 &&
+    p.require(label->numel() == rows && label->dim() >= 1 && label->dim() <= 2 && label->size(0) == rows &&
               (!bias || (bias->dim() == 1 && bias->size(0) == classes && bias->scalar_type() == x->scalar_type())));
   }
   const void *b() const { return bias ? bias->data_ptr() : nullptr; }

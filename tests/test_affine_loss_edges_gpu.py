@@ -44,3 +44,12 @@ def test_a_row_whose_label_does_not_exist_sets_no_scale(dtype, rows):
     label[3], dloss[3] = 500, 1e30
     label[4], dloss[4] = -1, 1e30
     rows_of_dx(x, w, label, bias, dloss, [i for i in range(rows) if i not in (3, 4)])
+
+
+def test_a_label_without_axes_is_refused():
+    x, w, label, bias, dloss = data(1, 24, 50, torch.float32, ignored=0.0)
+    loss, stat = F.affine_softmax_cross_entropy(x, w, label, bias, output_stat=True)
+    with pytest.raises(RuntimeError, match="label must have the shape"):
+        F.affine_softmax_cross_entropy(x, w, label[0, 0], bias)
+    with pytest.raises(RuntimeError, match="label must have the shape"):
+        F.affine_softmax_cross_entropy_backward(x, w, label[0, 0], stat, dloss, bias)
