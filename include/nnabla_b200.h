@@ -693,7 +693,7 @@ int nb200_affine_softmax_cross_entropy_backward(const void *x, const void *w, co
  *   loss = temperature^2 * sum p (log p - log q)   (fp32, [rows])
  * stat [rows, 2], fp32: the row's maximum, and log sum exp((x - maximum) / temperature).
  * A class named twice counts twice. A row without entries has the loss 0. A class >= classes makes its row's loss
- * NaN. best is 1 to 1024. */
+ * NaN. best is 1 to 1024, temperature 2^-126 or more. */
 int nb200_top_k_distillation(const void *x, const void *index, const void *teacher, float *loss, float *stat,
                              int64_t rows, int64_t classes, int best, float temperature, int type, int index_bytes,
                              void *stream);

@@ -370,7 +370,9 @@ int check(int64_t rows, int64_t classes, int best, float temperature, int index_
   NB_CHECK(rows >= 0 && rows < (1ll << 24), NB200_EVALUE, "%lld rows", (long long)rows);
   NB_CHECK(classes > 0 && classes < (1ll << 24), NB200_EVALUE, "%lld classes outside [1, 2^24)", (long long)classes);
   NB_CHECK(best >= 1 && best <= kMaxEntries, NB200_EVALUE, "%d entries a row outside [1, %d]", best, kMaxEntries);
-  NB_CHECK(temperature > 0.0f && temperature < INFINITY, NB200_EVALUE, "temperature = %g is not positive", temperature);
+  // (the inverse of a smaller one is infinite)
+  NB_CHECK(temperature >= 1.17549435e-38f && temperature < INFINITY, NB200_EVALUE, "temperature = %g outside [2^-126, infinity)",
+           temperature);
   NB_CHECK(index_bytes == 4 || index_bytes == 8, NB200_EVALUE, "the classes are 4 or 8 byte integers, not %d", index_bytes);
   return NB200_OK;
 }
