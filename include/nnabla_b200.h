@@ -699,7 +699,7 @@ int nb200_top_k_distillation(const void *x, const void *index, const void *teach
                              void *stream);
 /* dx (+)= temperature * (q - p) * dloss of each row, zero for a row without entries; stat is the forward
  * pass's. dx == x is allowed. */
-int nb200_top_k_distillation_backward(const void *x, const void *index, const void *teacher, const float *log_sum,
+int nb200_top_k_distillation_backward(const void *x, const void *index, const void *teacher, const float *stat,
                                       const float *dloss, void *dx, int64_t rows, int64_t classes, int best,
                                       float temperature, int type, int index_bytes, int accum, void *stream);
 
