@@ -180,14 +180,15 @@ def layer_normalization(inp, batch_axis=0, eps=1e-5, output_stat=False, fix_para
 
 
 def affine_softmax_cross_entropy(inp, label, n_outmaps, base_axis=1, w_init=None, b_init=None, fix_parameters=False, rng=None,
-                                 with_bias=True):
-    """softmax_cross_entropy(affine(inp, n_outmaps), label) on the parameters of `affine`, without the logits."""
+                                 with_bias=True, output_stat=False):
+    """softmax_cross_entropy(affine(inp, n_outmaps), label) on the parameters of `affine`, without the logits.
+    output_stat=True also returns what functions.affine_softmax_cross_entropy_backward needs."""
     inmaps = int(np.prod(inp.shape[base_axis:]))
     with parameter_scope("affine"):
         w = get_parameter_or_create("W", (inmaps, n_outmaps),
                                     w_init or _glorot_uniform(inmaps, n_outmaps, (1, 1), _rng(rng)))
         b = get_parameter_or_create("b", (n_outmaps,), b_init or _zeros) if with_bias else None
-    return F.affine_softmax_cross_entropy(inp, w, label, b, base_axis)
+    return F.affine_softmax_cross_entropy(inp, w, label, b, base_axis, output_stat)
 
 
 def fixed_point_quantized_affine(inp, n_outmaps, base_axis=1, w_init=None, b_init=None, fix_parameters=False, rng=None,

@@ -61,3 +61,18 @@ def test_a_head_without_bias(teacher):
     loss, (dx, dw, db) = resnet18.head_loss(x, w, None, label, given)
     want = resnet18.head_loss(x, w, torch.zeros_like(b), label, given)
     assert db is None and same((loss, (dx, dw)), (want[0], want[1][:2]))
+
+
+def test_a_parametric_head_is_trained():
+    from nnabla_b200 import functions as F
+    from nnabla_b200 import parametric_functions as PF
+    PF.clear_parameters()
+    x, label = torch.randn((24, 10), device="cuda"), torch.randint(0, 33, (24, 1), device="cuda")
+    loss, stat = PF.affine_softmax_cross_entropy(x, label, 33, output_stat=True)
+    assert torch.equal(loss, PF.affine_softmax_cross_entropy(x, label, 33))
+    p = PF.get_parameters()
+    w, b = p["affine/W"], p["affine/b"]
+    grads = F.affine_softmax_cross_entropy_backward(x, w, label, stat, torch.full((24, 1), 1 / 24, device="cuda"), b)
+    want = resnet18.head_loss(x, w, b, label)
+    assert all(torch.equal(g, v) for g, v in zip(grads, want[1]))
+    PF.clear_parameters()
