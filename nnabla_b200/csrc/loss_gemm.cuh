@@ -687,18 +687,7 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
     ma[1] = ma[0], mb[1] = mb[0];
   constexpr int kCtas = kPair ? 2 : 1;
   const int64_t units = std::min<int64_t>(sm_count() / kCtas, tiles[0] + tiles[1]);
-  // How many of the second product's tiles the units with one more of the first's get, so that the last one ends first.
-  const int64_t more = tiles[0] % units;
-  prob.extra_tiles = 0;
-  if (more && tiles[1]) {
-    int64_t best = -1;
-    for (int64_t n = 0; n <= (tiles[1] + more - 1) / more; ++n) {
-      const int64_t rest = std::max<int64_t>(0, tiles[1] - more * n);
-      const int64_t time = std::max(cost[0] + n * cost[1], (rest + units - more - 1) / (units - more) * cost[1]);
-      if (best < 0 || time < best)
-        best = time, prob.extra_tiles = (int)n;
-    }
-  }
+  prob.extra_tiles = (int)extra_tiles(tiles[0], tiles[1], cost[0], cost[1], units);
   prob.chunk = loss_chunk<T>();
   int *status = nullptr;
   NB_TRY(device_status_word(&status));

@@ -47,6 +47,31 @@ inline bool pays_pairs(std::initializer_list<TileCount> products, int sms) {
   return time(pair_work, pair_tiles, sms / 2) <= time(single_work, single_tiles, sms);
 }
 
+// Two products' tiles on `units`: the first's dealt out one by one, and of the second's this many to each of the units that got
+// one more of the first's, the rest to the others, so that the last one ends first.
+inline int64_t extra_tiles(int64_t first, int64_t second, int64_t first_cycles, int64_t second_cycles, int64_t units) {
+  const int64_t more = first % units;
+  if (more == 0 || second == 0)
+    return 0;
+  // With n tiles the former end at first_cycles + n second_cycles, which grows, the others at rounds(n) second_cycles, which
+  // falls: the best lies where the two cross, found by halves.
+  auto rounds = [&](int64_t n) {
+    return (std::max<int64_t>(0, second - more * n) + units - more - 1) / (units - more);
+  };
+  int64_t n = 0, top = (second + more - 1) / more; // rounds(top) is 0
+  while (n < top) {
+    const int64_t half = (n + top) / 2;
+    if (first_cycles + half * second_cycles >= rounds(half) * second_cycles)
+      top = half;
+    else
+      n = half + 1;
+  }
+  if (n == 0 || first_cycles + n * second_cycles < rounds(n - 1) * second_cycles)
+    return n;
+  // the fewest with as many rounds as n - 1 leaves
+  return std::max<int64_t>(0, (second - rounds(n - 1) * (units - more) + more - 1) / more);
+}
+
 // The rows of a matrix in slabs, each of whose column sums a block makes for itself (256 columns a block).
 constexpr int kSumColumns = 256;
 struct Slabs {
