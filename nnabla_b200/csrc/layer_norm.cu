@@ -671,9 +671,8 @@ int backward(const T *x, const T *dy, const P *gamma, const float *mean, const f
     return with_count(s.nv, Counts{}, [&](auto nv) -> int {
       constexpr int kNv = decltype(nv)::value;
       const size_t smem = walk && params && s.row_warps == 1 ? (size_t)per_block * 2 * size * 4 : 0;
+      static_assert(8 * 2 * 32 * std::min(4, kMaxNv) * kVec * 4 <= 48 * 1024, "a warp's rows need no opt-in");
       auto launch = [&](auto kernel, auto clustered) -> int {
-        if (smem > 48 * 1024)
-          NB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (decltype(clustered)::value)
           NB_CUDA(launch_clusters(kernel, (unsigned)(blocks * s.cluster), s.cluster, threads, smem, st, x, dy, gamma, mean, var, dx,
                                   static_cast<float *>(nullptr), rows, (int)size, 1.0f / (float)size, eps, s.row_warps, s.cluster,
