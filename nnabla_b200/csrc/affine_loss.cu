@@ -397,15 +397,16 @@ int forward(const T *x, const T *w, const T *bias, LossRows r, float *loss, floa
             cudaStream_t st) {
   if (rows > kFewRows)
     return forward_tensor<T>(x, w, bias, r, loss, stat, rows, size, r.classes, st);
-  const bool vec = r.classes % kPackOf<T> == 0 && aligned16(w);
-  const int64_t columns = vec ? few_lanes<T, kPackOf<T>>() * kPackOf<T> : 32;
+  const bool aligned = few_aligned(w, r.classes);
+  const int64_t columns = aligned ? few_columns<T, false>() : few_columns<T, true>();
   r.tiles = (int)((r.classes + columns - 1) / columns);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc((size_t)rows * r.tiles * 8 + (size_t)rows * 4));
   r.partial = static_cast<float2 *>(scratch.p);
   r.target = reinterpret_cast<float *>(r.partial + rows * r.tiles);
-  NB_TRY(few_variant<T>(rows, vec, [&](auto n, auto v) {
-    return few_logits<T, decltype(n)::value, decltype(v)::value>(x, w, bias, r, (int)rows, size, nullptr, 0, st);
+  NB_TRY(few_variant(rows, [&](auto n) {
+    constexpr int R = decltype(n)::value;
+    return (aligned ? few_logits<T, R, false> : few_logits<T, R, true>)(x, w, bias, r, (int)rows, size, nullptr, 0, st);
   }));
   return loss_rows(r, rows, loss, stat, st);
 }
@@ -422,18 +423,20 @@ int backward(const T *x, const T *w, const T *bias, LossRows r, T *dx, T *dw, T 
   NB_TRY(scratch.alloc(parts.bytes));
   char *base = static_cast<char *>(scratch.p);
   float *g = reinterpret_cast<float *>(base + at_g), *dx32 = reinterpret_cast<float *>(base + at_dx);
-  const bool vec = classes % kPackOf<T> == 0 && aligned16(w);
-  NB_TRY(few_variant<T>(rows, vec, [&](auto n, auto v) {
-    return few_logits<T, decltype(n)::value, decltype(v)::value>(x, w, bias, r, (int)rows, size, g, ldg, st);
+  const bool aligned = few_aligned(w, classes);
+  NB_TRY(few_variant(rows, [&](auto n) {
+    constexpr int R = decltype(n)::value;
+    return (aligned ? few_logits<T, R, false> : few_logits<T, R, true>)(x, w, bias, r, (int)rows, size, g, ldg, st);
   }));
   if (dx || dw) {
     const bool keep = (size_t)size * classes * sizeof(T) <= kKeepBytes;
     const int64_t walks = (size + kFewWalk - 1) / kFewWalk, slabs = std::min<int64_t>(walks, (4 * sm_count() + columns - 1) / columns);
     const int64_t slab = (walks + slabs - 1) / slabs * kFewWalk;
-    NB_TRY(few_variant<T>(rows, vec && aligned16(dw), [&](auto n, auto v) -> int {
-      NB_CUDA(launch_dependent(few_grads_kernel<T, decltype(n)::value, decltype(v)::value>,
-                               dim3((unsigned)columns, (unsigned)((size + slab - 1) / slab)), dim3(kFewGradThreads), 0, st, x, w,
-                               (const float *)g, ldg, dx != nullptr, dw, dx32, (int)rows, size, slab, classes, accum[1], keep));
+    NB_TRY(few_variant(rows, [&](auto n) -> int {
+      constexpr int R = decltype(n)::value;
+      auto kernel = aligned && aligned16(dw) ? few_grads_kernel<T, R, kPackOf<T>> : few_grads_kernel<T, R, 1>;
+      NB_CUDA(launch_dependent(kernel, dim3((unsigned)columns, (unsigned)((size + slab - 1) / slab)), dim3(kFewGradThreads), 0, st,
+                               x, w, (const float *)g, ldg, dx != nullptr, dw, dx32, (int)rows, size, slab, classes, accum[1], keep));
       return NB200_OK;
     }));
     if (dx)

@@ -31,39 +31,48 @@ template <int R> struct alignas(R > 1 ? 16 : 8) Few { // a value of x of each ro
 constexpr int kFewBatch = 4, kFewBatches = 3;                         // packs a batch of copies, batches on the way
 constexpr int kFewRing = kFewBatch * kFewBatches * kFewThreads * 16; // bytes
 
-template <typename T, int VEC> constexpr int few_lanes() { return VEC * sizeof(T) == 16 ? 16 : 32; }
-// Shared memory in front of x: the ring, or in its place the warps' sums.
-template <typename T, int R, int VEC> constexpr int few_fixed_bytes() {
-  const int ring = VEC * sizeof(T) == 16 ? kFewRing : 0, sums = kFewThreads / 32 * R * few_lanes<T, VEC>() * VEC * 4;
-  return ring > sums ? ring : sums;
+constexpr int kFewLanes = 16; // that read a row of W side by side
+// Classes of a group. kShift: the sixteen accesses of a row begin up to VEC - 1 values in front of the group's first class.
+template <typename T, bool kShift> constexpr int few_columns() { return (kFewLanes - (kShift ? 1 : 0)) * kPackOf<T>; }
+// Shared memory in front of x: the ring, or in its place the warps' sums (kShift: the half warps').
+template <typename T, int R, bool kShift> constexpr int few_fixed_bytes() {
+  const int sums = kFewThreads / (kShift ? kFewLanes : 32) * R * few_columns<T, kShift>() * 4;
+  return kFewRing > sums ? kFewRing : sums;
 }
 
-// l = x W + b for a group of classes, kLanes * VEC: half a warp reads 256 bytes of a row of W at a time ([1, 2048] . [2048,
+// l = x W + b for a group of classes: half a warp reads 256 bytes of a row of W at a time ([1, 2048] . [2048,
 // 32000] bf16, with the second kernel, 26.4 us; with runs of 128 bytes 30.2). Where the groups are fewer than the SMs a cluster
 // of `splits` blocks shares one, each with its part of K, and its first block adds up their sums, in order (where they are
 // enough that costs more than it brings: 29.6 us with two blocks, 33.7 with four). Of those kSums leaves the maximum and the
 // sum of the exponentials, kGrad G in fp32.
-template <typename T, int R, int VEC, Out kOut>
+// kShift: rows of W that begin anywhere. A thread's rows are sixteen apart, a multiple of VEC, so that all of them begin equally
+// far behind a 16-byte boundary; it reads from the boundaries, and its sums are those of the classes `shift` further back.
+// (Value by value, in runs of 128 or 64 bytes: [2, 4096] . [4096, 131071] fp32 1147 us, 323 with 131072 classes.)
+template <typename T, int R, bool kShift, Out kOut>
 __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__restrict__ x, const T *__restrict__ w,
                                                                  const T *__restrict__ bias, LossRows rows, int count,
                                                                  int64_t size, int splits, float *__restrict__ g,
                                                                  int64_t ldg) {
-  constexpr bool kAsync = VEC * sizeof(T) == 16;
-  constexpr int kLanes = few_lanes<T, VEC>(), kCols = kLanes * VEC, kWarps = kFewThreads / 32, kStep = kFewThreads / kLanes;
+  constexpr int VEC = kPackOf<T>, kCols = few_columns<T, kShift>(), kStep = kFewThreads / kFewLanes;
+  constexpr int kWarps = kFewThreads / 32, kParts = kShift ? kStep : kWarps; // of the sums: one a half warp, or a warp
+  static_assert(kStep % VEC == 0, "a thread's rows begin alike");
   constexpr int kFewK = kFewValues / R;
   extern __shared__ __align__(16) uint8_t few_smem[];
   uint4(*ring)[kFewThreads] = reinterpret_cast<uint4(*)[kFewThreads]>(few_smem); // [kFewBatches * kFewBatch]
   float(*sums)[R][kCols] = reinterpret_cast<float(*)[R][kCols]>(few_smem);       // behind the last use of the ring
-  float *xs = reinterpret_cast<float *>(few_smem + few_fixed_bytes<T, R, VEC>());
+  float *xs = reinterpret_cast<float *>(few_smem + few_fixed_bytes<T, R, kShift>());
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t group = blockIdx.x / splits;
   const int split = blockIdx.x - (int)group * splits;
-  const int64_t classes = rows.classes, c0 = group * kCols, c = c0 + (threadIdx.x % kLanes) * VEC;
-  const bool here = c < classes; // (VEC divides classes, or is 1)
   const int64_t each = (size + splits - 1) / splits, ka = split * each, kb = ka + each < size ? ka + each : size;
-  constexpr int kPairs = (VEC + 1) / 2; // of neighbouring classes
+  const int k_first = threadIdx.x / kFewLanes;
+  const int64_t classes = rows.classes, c0 = group * kCols;
+  const int shift = kShift ? (int)(reinterpret_cast<uintptr_t>(w) / sizeof(T) + (ka + k_first) * classes) & (VEC - 1) : 0;
+  const int64_t c = c0 + (threadIdx.x % kFewLanes) * VEC - shift; // of the thread's access
+  const bool here = c < classes;                                  // (kShift: some of it; otherwise VEC divides classes)
+  constexpr int kPairs = VEC / 2;                                 // of neighbouring classes
   uint64_t acc[R][kPairs];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -73,19 +82,28 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
   // W by asynchronous copies, each thread for itself: kFewBatches batches of kFewBatch packs on the way, whatever the compiler
   // makes of the registers (of eight ordinary loads a step it kept few in flight: 3.4 TB/s). The batches are those of the loop
   // below, a full piece of K being whole batches.
-  static_assert(!kAsync || kFewK % (kFewBatch * kStep) == 0, "a piece of K is whole batches");
-  const int k_first = threadIdx.x / kLanes;
+  static_assert(kFewK % (kFewBatch * kStep) == 0, "a piece of K is whole batches");
   int64_t next = ka + k_first;
   int fetched = 0, batch = 0;
   auto fetch = [&]() {
-    if constexpr (kAsync) {
-      const int at = fetched++ % kFewBatches * kFewBatch;
+    const int at = fetched++ % kFewBatches * kFewBatch;
 #pragma unroll
-      for (int u = 0; u < kFewBatch; ++u, next += kStep)
-        if (here && next < kb)
-          cp_async16(&ring[at + u][threadIdx.x], w + next * classes + c);
-      cp_async_commit();
-    }
+    for (int u = 0; u < kFewBatch; ++u, next += kStep)
+      if (here && next < kb) {
+        const int64_t e = next * classes + c; // (kShift: beside its row an access reads the neighbouring rows)
+        if (!kShift || (e >= 0 && e + VEC <= size * classes)) {
+          cp_async16(&ring[at + u][threadIdx.x], w + e);
+        } else { // nothing in front of W or behind it
+          Pack<T, VEC> p;
+          p.clear();
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (e + j >= 0 && e + j < size * classes)
+              p.set(j, w[e + j]);
+          *reinterpret_cast<Pack<T, VEC> *>(&ring[at + u][threadIdx.x]) = p;
+        }
+      }
+    cp_async_commit();
   };
   for (int i = 0; i < kFewBatches; ++i)
     fetch();
@@ -103,7 +121,7 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
       uint64_t wv[kPairs];
 #pragma unroll
       for (int j = 0; j < kPairs; ++j)
-        wv[j] = pair_of(v.f(2 * j), 2 * j + 1 < VEC ? v.f(2 * j + 1) : 0.0f);
+        wv[j] = pair_of(v.f(2 * j), v.f(2 * j + 1));
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float xv = xs[k * R + r];
@@ -113,25 +131,18 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
           acc[r][j] = fma2(xx, wv[j], acc[r][j]);
       }
     };
-    if constexpr (kAsync) {
-      for (int k = k_first; k < n; k += kFewBatch * kStep) {
-        const int at = batch++ % kFewBatches * kFewBatch;
-        cp_async_wait<kFewBatches - 1>();
-        if (here)
+    for (int k = k_first; k < n; k += kFewBatch * kStep) {
+      const int at = batch++ % kFewBatches * kFewBatch;
+      cp_async_wait<kFewBatches - 1>();
+      if (here)
 #pragma unroll
-          for (int u = 0; u < kFewBatch; ++u)
-            if (k + u * kStep < n)
-              add(*reinterpret_cast<const Pack<T, VEC> *>(&ring[at + u][threadIdx.x]), k + u * kStep);
-        fetch();
-      }
-    } else if (here) {
-#pragma unroll 8
-      for (int k = k_first; k < n; k += kStep)
-        add(load_pack<T, VEC>(w + (k0 + k) * classes + c), k);
+        for (int u = 0; u < kFewBatch; ++u)
+          if (k + u * kStep < n)
+            add(*reinterpret_cast<const Pack<T, VEC> *>(&ring[at + u][threadIdx.x]), k + u * kStep);
+      fetch();
     }
   }
-  if constexpr (kAsync)
-    cp_async_wait<0>();
+  cp_async_wait<0>();
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -139,18 +150,22 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
     for (int j = 0; j < VEC; ++j) {
       const float2 both = unpair(acc[r][j / 2]);
       float s = j & 1 ? both.y : both.x;
-#pragma unroll
-      for (int d = 16; d >= kLanes; d >>= 1)
-        s += __shfl_xor_sync(0xffffffffu, s, d);
-      if (lane < kLanes)
-        sums[warp][r][lane * VEC + j] = s;
+      if constexpr (kShift) { // the halves of a warp begin differently
+        const int i = lane % kFewLanes * VEC + j - shift;
+        if (i >= 0 && i < kCols)
+          sums[k_first][r][i] = s;
+      } else {
+        s += __shfl_xor_sync(0xffffffffu, s, kFewLanes);
+        if (lane < kFewLanes)
+          sums[warp][r][lane * VEC + j] = s;
+      }
     }
   __syncthreads();
   float *own = &sums[0][0][0]; // [R][kCols], the block's
   for (int i = threadIdx.x; i < R * kCols; i += kFewThreads) {
     float s = 0.0f;
 #pragma unroll
-    for (int u = 0; u < kWarps; ++u)
+    for (int u = 0; u < kParts; ++u)
       s += own[u * R * kCols + i];
     own[i] = s;
   }
@@ -337,22 +352,22 @@ __global__ void __launch_bounds__(kFewGradThreads) few_grads_kernel(const T *__r
   }
 }
 
-template <typename T, int R, int VEC>
+template <typename T, int R, bool kShift>
 int few_logits(const T *x, const T *w, const T *bias, const LossRows &r, int count, int64_t size, float *g, int64_t ldg,
                cudaStream_t st) {
-  constexpr int kCols = few_lanes<T, VEC>() * VEC, kXs = kFewValues * 4, kFixed = few_fixed_bytes<T, R, VEC>();
+  constexpr int kCols = few_columns<T, kShift>(), kXs = kFewValues * 4, kFixed = few_fixed_bytes<T, R, kShift>();
   const int64_t groups = (r.classes + kCols - 1) / kCols;
   int splits = 1;
   while (splits < 8 && groups * splits < sm_count() && size >= 128 * splits)
     splits *= 2;
   const int smem = kFixed + (int)std::min<int64_t>(kXs, (size + splits - 1) / splits * R * 4);
-  auto kernel = g ? few_logits_kernel<T, R, VEC, Out::kGrad> : few_logits_kernel<T, R, VEC, Out::kSums>;
+  auto kernel = g ? few_logits_kernel<T, R, kShift, Out::kGrad> : few_logits_kernel<T, R, kShift, Out::kSums>;
   static std::atomic<bool> configured[64]{};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    NB_CUDA(cudaFuncSetAttribute(few_logits_kernel<T, R, VEC, Out::kGrad>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kXs));
-    NB_CUDA(cudaFuncSetAttribute(few_logits_kernel<T, R, VEC, Out::kSums>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kXs));
+    NB_CUDA(cudaFuncSetAttribute(few_logits_kernel<T, R, kShift, Out::kGrad>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kXs));
+    NB_CUDA(cudaFuncSetAttribute(few_logits_kernel<T, R, kShift, Out::kSums>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kXs));
     configured[dev & 63] = true;
   }
   NB_CUDA(launch_clusters(kernel, (unsigned)(groups * splits), splits, kFewThreads, smem, st, x, w, bias, r, count, size,
@@ -360,15 +375,14 @@ int few_logits(const T *x, const T *w, const T *bias, const LossRows &r, int cou
   return NB200_OK;
 }
 
-// f(rows rounded up to 1, 2, 4 or 8; values an access) as compile-time constants
-template <typename T, typename F> int few_variant(int64_t rows, bool vec, F f) {
-  auto with_vec = [&](auto r) -> int {
-    return vec ? f(r, std::integral_constant<int, kPackOf<T>>{}) : f(r, std::integral_constant<int, 1>{});
-  };
-  return rows <= 1   ? with_vec(std::integral_constant<int, 1>{})
-         : rows <= 2 ? with_vec(std::integral_constant<int, 2>{})
-         : rows <= 4 ? with_vec(std::integral_constant<int, 4>{})
-                     : with_vec(std::integral_constant<int, 8>{});
+// f(rows rounded up to 1, 2, 4 or 8) as a compile-time constant
+template <typename F> int few_variant(int64_t rows, F f) {
+  return rows <= 1   ? f(std::integral_constant<int, 1>{})
+         : rows <= 2 ? f(std::integral_constant<int, 2>{})
+         : rows <= 4 ? f(std::integral_constant<int, 4>{})
+                     : f(std::integral_constant<int, 8>{});
 }
+// Whether rows of W, or of dW, begin at 16-byte boundaries.
+template <typename T> bool few_aligned(const T *w, int64_t classes) { return classes % kPackOf<T> == 0 && aligned16(w); }
 
 } // namespace nb200

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from nnabla_b200 import functions as F
-from test_affine_loss_gpu import TYPES, data, reference, rms
+from test_affine_loss_gpu import TYPES, check, data, reference, rms
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,16 @@ def test_a_label_without_axes_is_refused():
         F.affine_softmax_cross_entropy(x, w, label[0, 0], bias)
     with pytest.raises(RuntimeError, match="label must have the shape"):
         F.affine_softmax_cross_entropy_backward(x, w, label[0, 0], stat, dloss, bias)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 3, 8])
+@pytest.mark.parametrize("size,classes", [(1, 1), (5, 3), (16, 7), (17, 15), (33, 59), (200, 60), (31, 61), (130, 119), (40, 121),
+                                          (300, 1001), (700, 16), (900, 33)])
+def test_few_rows_with_rows_of_the_weights_that_begin_anywhere(dtype, rows, size, classes):
+    """Every distance of W from a 16-byte boundary, with NaN around it, and every distance of its rows from one."""
+    x, w, label, bias, dloss = data(rows, size, classes, dtype)
+    for off in range(16 // w.element_size()):
+        base = torch.full((16 + w.numel() + 16,), math.nan, dtype=dtype, device="cuda")
+        at = base[8 + off:8 + off + w.numel()].view_as(w).copy_(w)
+        check(x, at, label, bias, dloss)
