@@ -398,7 +398,12 @@ int forward(const T *x, const T *w, const T *bias, LossRows r, float *loss, floa
   if (rows > kFewRows)
     return forward_tensor<T>(x, w, bias, r, loss, stat, rows, size, r.classes, st);
   const bool aligned = few_aligned(w, r.classes);
-  const int64_t columns = aligned ? few_columns<T, false>() : few_columns<T, true>();
+  int columns = 0;
+  NB_TRY(few_variant(rows, [&](auto n) -> int {
+    constexpr int R = decltype(n)::value;
+    columns = aligned ? few_columns<T, R, false>() : few_columns<T, R, true>();
+    return NB200_OK;
+  }));
   r.tiles = (int)((r.classes + columns - 1) / columns);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc((size_t)rows * r.tiles * 8 + (size_t)rows * 4));
@@ -416,31 +421,38 @@ int backward(const T *x, const T *w, const T *bias, LossRows r, T *dx, T *dw, T 
              const bool accum[3], cudaStream_t st) {
   if (rows > kFewRows)
     return backward_tensor<T>(x, w, bias, r, dx, dw, db, rows, size, r.classes, accum, st);
-  const int64_t classes = r.classes, ldg = up(classes, 4), columns = (classes + 8 * kFewGradThreads - 1) / (8 * kFewGradThreads);
+  const int64_t classes = r.classes, ldg = up(classes, 4);
+  const bool aligned = few_aligned(w, classes);
+  // Both gradients in one pass, unless rows of W and dW begin differently far behind a 16-byte boundary.
+  const bool alike = !dx || !dw || ((reinterpret_cast<uintptr_t>(w) ^ reinterpret_cast<uintptr_t>(dw)) & 15) == 0;
+  const FewGradients plan(size, classes, kPackOf<T>, !few_aligned(dx ? w : dw, classes), sm_count());
   Parts parts;
-  const size_t at_g = parts.take((size_t)rows * ldg * 4), at_dx = parts.take(dx ? (size_t)columns * rows * size * 4 : 0);
+  const size_t at_g = parts.take((size_t)rows * ldg * 4), at_dx = parts.take(dx ? (size_t)plan.columns * rows * size * 4 : 0);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc(parts.bytes));
   char *base = static_cast<char *>(scratch.p);
   float *g = reinterpret_cast<float *>(base + at_g), *dx32 = reinterpret_cast<float *>(base + at_dx);
-  const bool aligned = few_aligned(w, classes);
   NB_TRY(few_variant(rows, [&](auto n) {
     constexpr int R = decltype(n)::value;
     return (aligned ? few_logits<T, R, false> : few_logits<T, R, true>)(x, w, bias, r, (int)rows, size, g, ldg, st);
   }));
   if (dx || dw) {
     const bool keep = (size_t)size * classes * sizeof(T) <= kKeepBytes;
-    const int64_t walks = (size + kFewWalk - 1) / kFewWalk, slabs = std::min<int64_t>(walks, (4 * sm_count() + columns - 1) / columns);
-    const int64_t slab = (walks + slabs - 1) / slabs * kFewWalk;
-    NB_TRY(few_variant(rows, [&](auto n) -> int {
-      constexpr int R = decltype(n)::value;
-      auto kernel = aligned && aligned16(dw) ? few_grads_kernel<T, R, kPackOf<T>> : few_grads_kernel<T, R, 1>;
-      NB_CUDA(launch_dependent(kernel, dim3((unsigned)columns, (unsigned)((size + slab - 1) / slab)), dim3(kFewGradThreads), 0, st,
-                               x, w, (const float *)g, ldg, dx != nullptr, dw, dx32, (int)rows, size, slab, classes, accum[1], keep));
-      return NB200_OK;
-    }));
+    auto grads = [&](const FewGradients &p, T *to_dx, T *to_dw) {
+      return few_variant(rows, [&](auto n) -> int {
+        constexpr int R = decltype(n)::value;
+        auto kernel = few_aligned(to_dx ? w : to_dw, classes) ? few_grads_kernel<T, R, false> : few_grads_kernel<T, R, true>;
+        NB_CUDA(launch_dependent(kernel, dim3((unsigned)p.columns, (unsigned)p.blocks), dim3(kFewGradThreads), 0, st, x, w,
+                                 (const float *)g, ldg, to_dx != nullptr, to_dw, dx32, (int)rows, size, p.slab, classes, accum[1],
+                                 keep));
+        return NB200_OK;
+      });
+    };
+    NB_TRY(grads(plan, dx, alike ? dw : nullptr));
+    if (!alike)
+      NB_TRY(grads(FewGradients(size, classes, kPackOf<T>, !few_aligned(dw, classes), sm_count()), nullptr, dw));
     if (dx)
-      NB_TRY(add_parts<T>(dx32, (int)columns, rows * size, 1, rows * size, rows * size, nullptr, dx, rows * size, accum[0], st));
+      NB_TRY(add_parts<T>(dx32, (int)plan.columns, rows * size, 1, rows * size, rows * size, nullptr, dx, rows * size, accum[0], st));
   }
   if (db)
     NB_TRY(add_parts<T>(g, (int)rows, ldg, 1, classes, ldg, nullptr, db, classes, accum[2], st));

@@ -84,6 +84,24 @@ inline Slabs column_slabs(int64_t all_rows, int64_t columns, int sms) {
   return {rows, (all_rows + rows - 1) / rows};
 }
 
+// Both gradients of a head of few rows in one pass over W (few_rows.cuh): blocks of kFewBlock classes by `slab` rows of W, which
+// lie `step` apart.
+constexpr int kFewGradThreads = 256, kFewBlock = 8 * kFewGradThreads;
+constexpr int kFewWalk = 32; // rows of W between two exchanges of the warps' sums
+struct FewGradients {
+  int64_t columns; // blocks of classes; with `shift` one more, for the rows' ends
+  int64_t slab, blocks; // rows of W a block; blocks along them
+  // (with a third as many blocks, some one and a half rounds of them, [8, 4096] . [4096, 131071] fp32 1002 us, not 907)
+  // shift: rows of W that begin up to vec - 1 values behind a 16-byte boundary, and so do the blocks of classes
+  FewGradients(int64_t size, int64_t classes, int vec, bool shift, int sms) {
+    const int64_t step = shift ? vec : 1, each = (size + step - 1) / step, walks = (each + kFewWalk - 1) / kFewWalk;
+    columns = (classes + (shift ? vec - 1 : 0) + kFewBlock - 1) / kFewBlock + (shift ? 1 : 0);
+    const int64_t slabs = std::min(walks, (12 * sms + columns * step - 1) / (columns * step));
+    slab = (walks + slabs - 1) / slabs * kFewWalk;
+    blocks = step * ((each + slab - 1) / slab);
+  }
+};
+
 // A head's gradients on the tensor cores: the pieces of the classes, the tiles and parts of K of the products, and what of it
 // lies where in the scratch. `planes`: three bf16 pieces an fp32 value, or one of 16 bits.
 struct HeadGradients {

@@ -66,3 +66,30 @@ def test_few_rows_with_rows_of_the_weights_that_begin_anywhere(dtype, rows, size
         base = torch.full((16 + w.numel() + 16,), math.nan, dtype=dtype, device="cuda")
         at = base[8 + off:8 + off + w.numel()].view_as(w).copy_(w)
         check(x, at, label, bias, dloss)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [2, 7])
+@pytest.mark.parametrize("size,classes", [(5, 3), (40, 121), (130, 2048), (300, 4103)])
+def test_few_rows_with_a_gradient_buffer_that_begins_anywhere(dtype, rows, size, classes):
+    """dW beginning otherwise than W: the same bits, and what lies around it stays."""
+    x, w, label, bias, dloss = data(rows, size, classes, dtype)
+    loss, stat, want = check(x, w, label, bias, dloss)
+    for off in range(16 // w.element_size()):
+        base = torch.full((8 + off + w.numel() + 16,), 7.0, dtype=dtype, device="cuda")
+        dw = base[8 + off:8 + off + w.numel()].view_as(w)
+        for accum in (False, True):
+            dw.fill_(1.0)
+            got = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias, grads=(None, dw, None),
+                                                          accum=(False, accum, False))
+            assert got[1] is dw and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+            if accum:
+                half = torch.finfo(dtype).eps / 2
+                b = want[1].double()
+                assert ((dw.double() - 1 - b).abs() <= half * (2 * b.abs() + 1.01) + 1e-6 * rms(b)).all()
+            else:
+                assert torch.equal(dw, want[1])
+            assert (base[:8 + off] == 7).all() and (base[8 + off + w.numel():] == 7).all()
+        alone = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias, grads=(None, dw.fill_(1.0), None),
+                                                        propagate_down=(False, True, False))
+        assert torch.equal(alone[1], want[1])
