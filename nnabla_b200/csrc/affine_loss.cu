@@ -277,11 +277,12 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
                    int64_t classes, cudaStream_t st) {
   const int kblocks = (int)((size + 63) / 64);
   const bool pair = pays_pairs({{rows, classes, kblocks}}, sm_count());
-  r.tiles = loss_sum_tiles<T>(classes, kblocks, pair);
+  const bool split = std::is_same<T, float>::value && loss_splits(rows, size, classes);
+  r.tiles = split ? (int)((classes + kSplitTile - 1) / kSplitTile) * 2 : loss_sum_tiles<T>(classes, kblocks, pair);
   // so many rows at a time that their maxima and sums are 64 MB (the largest head in use: 8192 rows of 128000 classes)
   const int64_t slab = std::min(rows, std::max<int64_t>(256, (1 << 23) / r.tiles / 256 * 256));
   Parts parts;
-  const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(operand_bytes(w, size, classes));
+  const size_t at_x = parts.take(operand_bytes(x, rows, size)), at_w = parts.take(split ? 0 : operand_bytes(w, size, classes));
   const size_t at_partial = parts.take((size_t)slab * r.tiles * 8), at_target = parts.take((size_t)slab * 4);
   AsyncScratch scratch(st);
   NB_TRY(scratch.alloc(parts.bytes));
@@ -290,6 +291,8 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
   r.target = reinterpret_cast<float *>(base + at_target);
   Preparation pre{};
   const Operand ox = operand(x, rows, size, base + at_x, pre.m[0]), ow = operand(w, size, classes, base + at_w, pre.m[1]);
+  if (split)
+    pre.m[1] = Layout{};
   NB_TRY(prepare<T>(pre, st));
   const char *label = static_cast<const char *>(r.label);
   for (int64_t r0 = 0; r0 < rows; r0 += slab) {
@@ -303,6 +306,12 @@ int forward_tensor(const T *x, const T *w, const T *bias, LossRows r, float *los
     prob.bias = bias;
     prob.rows = r;
     prob.p[0].M = (int)n, prob.p[0].N = (int)classes, prob.p[0].K = (int)size, prob.p[0].kblocks = kblocks, prob.p[0].b_mn = 1;
+    if constexpr (std::is_same<T, float>::value)
+      if (split) {
+        NB_TRY(run_split_gemm<Out::kSums>(prob, part, w, size, classes, classes, st));
+        NB_TRY(loss_rows(r, n, loss + r0, stat + r0, st));
+        continue;
+      }
     NB_TRY((run_loss_gemm<T, Out::kSums>(pair, prob, &part, &ow, st)));
     NB_TRY(loss_rows(r, n, loss + r0, stat + r0, st));
   }
@@ -315,8 +324,9 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kPlanes = kF32 ? 3 : 1;
   using G = std::conditional_t<kF32, __nv_bfloat16, T>;
+  const bool split = kF32 && loss_splits(rows, size, classes);
   const HeadGradients plan(rows, size, classes, kF32, dx, dw, db, accum[0], operand_bytes(x, rows, size),
-                           operand_bytes(w, size, classes), sm_count());
+                           split ? 0 : operand_bytes(w, size, classes), sm_count());
   const int64_t piece = plan.piece, ld_dx = plan.ld_dx;
   const bool direct = plan.direct;
   AsyncScratch scratch(st);
@@ -326,6 +336,8 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
   float *scale = reinterpret_cast<float *>(base + plan.at_scale);
   Preparation pre{};
   const Operand ox = operand(x, rows, size, base + plan.at_x, pre.m[0]), ow = operand(w, size, classes, base + plan.at_w, pre.m[1]);
+  if (split)
+    pre.m[1] = Layout{};
   pre.rows = r, pre.count = rows, pre.scale = scale, pre.times = std::is_same<T, __half>::value ? 16384.0f : 1.0f;
   NB_TRY(prepare<T>(pre, st));
   r.scale = scale;
@@ -340,7 +352,14 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
     Product &l = prob.p[0];
     l.M = (int)rows, l.N = (int)n, l.K = (int)size, l.kblocks = (int)((size + 63) / 64), l.b_mn = 1;
     l.out = base + plan.at_g, l.ldo = piece, l.stride = rows * piece;
-    NB_TRY((run_loss_gemm<T, Out::kGrad>(plan.pair_grad, prob, &ox, &owc, st)));
+    if constexpr (kF32) {
+      if (split)
+        NB_TRY(run_split_gemm<Out::kGrad>(prob, ox, w + c0, size, n, classes, st));
+      else
+        NB_TRY((run_loss_gemm<T, Out::kGrad>(plan.pair_grad, prob, &ox, &owc, st)));
+    } else {
+      NB_TRY((run_loss_gemm<T, Out::kGrad>(plan.pair_grad, prob, &ox, &owc, st)));
+    }
     Operand a[2], b[2];
     prob.count = 0;
     if (dw) {
@@ -366,6 +385,13 @@ int backward_tensor(const T *x, const T *w, const T *bias, LossRows r, T *dx, T 
       p.vec = p.ldo * (p.out_f32 ? 4 : sizeof(T)) % 16 == 0 && aligned16(p.out);
       a[prob.count] = og, b[prob.count++] = owc;
     }
+    if constexpr (kF32)
+      if (split && dx) { // dx for itself, the last of the products
+        Products one = prob;
+        one.count = 1;
+        one.p[0] = prob.p[--prob.count];
+        NB_TRY(run_split_gemm<Out::kStore>(one, og, w + c0, size, n, classes, st));
+      }
     if (!kF32 && prob.count == 2 && loss_is_long<T>(plan.dx_blocks) != loss_is_long<T>(plan.dw_blocks)) {
       // (of two forms of the kernel: together both would take the one with eight epilogue warps)
       for (int i = 0; i < 2; ++i) {

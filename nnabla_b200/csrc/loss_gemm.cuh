@@ -57,6 +57,10 @@ struct Product {
   int64_t ldo, stride;
   int out_f32, accum;
   int vec; // rows of out begin at 16-byte boundaries
+  // kSplit: B in memory, b_rows x b_cols fp32 values at a pitch of b_ld; rows begin at 8-byte boundaries
+  const float *b;
+  int64_t b_rows, b_cols, b_ld;
+  int b_pairs;
 };
 struct Products {
   Product p[kMaxProducts];
@@ -71,14 +75,18 @@ struct Products {
 // kLong: K goes through tensor memory in more than one chunk, and the chunks' sums take an epilogue thread 128 registers; eight
 // epilogue warps. Without them there is room for sixteen, which a short K needs: its tiles are bound by the epilogue's latencies
 // (K = 302: 1900 cycles a 16-column step with two warps a scheduler, 2560 cycles of MMAs a tile of 256 columns).
-template <int PL, bool kPair, bool kLong> struct LossShape {
-  static constexpr int kWarps = kPair && !kLong ? 16 : 8, kThreads = 32 * (2 + kWarps); // epilogue warps; threads
-  static constexpr int kTileRows = kPair ? 256 : 128, kTileCols = kPair ? 256 : 64; // of a cluster
-  static constexpr int kCtaCols = kPair ? 128 : 64;                                 // columns of B that a CTA loads
+// kSplit (fp32, one CTA, 128 x 128 tiles): eight more warps make the pieces of B from the fp32 values on their way to shared memory.
+template <int PL, bool kPair, bool kLong, bool kSplit> struct LossShape {
+  static_assert(!kSplit || (PL == 3 && !kPair && kLong), "only fp32 has pieces");
+  static constexpr int kWarps = kPair && !kLong && PL == 1 ? 16 : 8, kSplitters = kSplit ? 8 : 0; // epilogue warps; those that make pieces
+  static constexpr int kThreads = 32 * (2 + kWarps + kSplitters);
+  static constexpr int kTileRows = kPair ? 256 : 128, kTileCols = kPair ? 256 : kSplit ? 128 : 64; // of a cluster
+  static constexpr int kCtaCols = kPair || kSplit ? 128 : 64;                                      // columns of B that a CTA loads
   static constexpr uint32_t kABytes = kTileM * kRowBytes, kBBytes = kCtaCols * kRowBytes;
   static constexpr uint32_t kStageBytes = PL * (kABytes + kBBytes);
   static constexpr int kStages = PL == 3 ? 2 : kWarps == 16 ? 5 : 6;
-  static constexpr int kWarpStage = 32 * 32 * 4; // bytes of an epilogue warp's transpose buffer
+  static constexpr int kPitch = PL == 3 ? 33 : 32;                // values a row of it; 33: no conflicts, and offsets that are constants
+  static constexpr int kWarpStage = 32 * kPitch * 4;              // bytes of an epilogue warp's transpose buffer
   static constexpr size_t kSmem =
       (size_t)kStages * kStageBytes + kWarps * kWarpStage + (2 * kStages + 4) * 8 + 16 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
@@ -100,14 +108,14 @@ template <typename T> __device__ __forceinline__ void store16(T *p, const float 
 }
 
 // T: the operands' type; float means three bf16 planes.
-template <typename T, bool kPair, bool kLong, Out kOut>
-__global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 1, kPair, kLong>::kThreads, 1)
+template <typename T, bool kPair, bool kLong, Out kOut, bool kSplit>
+__global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 1, kPair, kLong, kSplit>::kThreads, 1)
     loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
                      const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
                      const __grid_constant__ Products prob, int *status) {
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int PL = kF32 ? 3 : 1;
-  using S = LossShape<PL, kPair, kLong>;
+  using S = LossShape<PL, kPair, kLong, kSplit>;
   constexpr int STAGES = S::kStages, BN = S::kTileCols;
   constexpr uint32_t kABytes = S::kABytes, kBBytes = S::kBBytes, kStageBytes = S::kStageBytes;
   constexpr uint32_t kChunkBytes = 64 * kRowBytes; // 64 columns x 64 of K of an MN-major operand
@@ -133,7 +141,7 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(full_bar + s, 1);
+      ptx::mbar_init(full_bar + s, 1 + S::kSplitters);
       ptx::mbar_init(empty_bar + s, 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -179,10 +187,16 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
     t.which = kOut == Out::kStore && tile >= tiles0 ? 1 : 0;
     const Product &p = prob.p[t.which];
     tile -= t.which ? tiles0 : 0;
+    if (kOut == Out::kStore && p.splits == 1 && p.kblocks <= 2) {
+      t.n0 = tile % p.n_tiles * BN;
+      t.m0 = tile / p.n_tiles * S::kTileRows;
+      t.split = 0;
+    } else {
     t.m0 = tile % p.m_tiles * S::kTileRows;
     tile /= p.m_tiles;
     t.n0 = tile % p.n_tiles * BN;
     t.split = tile / p.n_tiles;
+    }
     t.kb0 = t.split * p.split_blocks;
     t.kb1 = t.kb0 + p.split_blocks < p.kblocks ? t.kb0 + p.split_blocks : p.kblocks;
     return t;
@@ -242,6 +256,8 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
             } else {
               load(a, ma, kb * 64, m0, pl);
             }
+            if constexpr (kSplit)
+              continue;
             if (b_mn) {
 #pragma unroll
               for (int j = 0; j < S::kCtaCols / 64; ++j)
@@ -330,6 +346,110 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
         }
       }
     }
+  } else if (kSplit && warp >= 2 + S::kWarps) {
+    // ---------------------------------------------------------------- pieces of B
+    // A K block of B is 128 runs of 64 neighbouring fp32 values: run u is a row of W, its pieces 128 bytes of shared memory each.
+    // This warp has the runs me, me + 8, ..., a lane two values of each; the next block's are on their way while one is worked on.
+    if constexpr (kSplit) {
+      constexpr int kApart = S::kSplitters, kRuns = 128 / kApart;
+      constexpr bool kMn = kOut != Out::kStore; // the runs of a K block: 64 of K for each of two groups of columns, or 128 columns
+      const int me = warp - (2 + S::kWarps);
+      const Product &p = prob.p[0];
+      static_assert(kApart == 8, "a run's number in eight is the warp's");
+      const uint32_t at = (uint32_t)me * kRowBytes + ((lane >> 2) ^ me) * 16 + (lane & 3) * 4; // (128-byte swizzle)
+      const int64_t step = kApart * p.b_ld;
+      int next_i = 0, next_kb = 0;
+      bool more = true;
+      At next{};
+      const float *from = nullptr; // of the next block: this lane's values of the warp's first run
+      int x_rows[2], y_rows[2];    // its rows that hold this lane's first value, and its second, of each group of columns
+      auto seek = [&]() {
+        const int64_t row = (kMn ? next_kb * 64 : next.n0) + me, col = (kMn ? next.n0 : next_kb * 64) + 2 * lane;
+        from = p.b + row * p.b_ld + col;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int rows_left = more ? (int)(p.b_rows - row) : 0, cols_left = (int)(p.b_cols - col) - 64 * g;
+          x_rows[g] = cols_left > 0 ? rows_left : 0, y_rows[g] = cols_left > 1 ? rows_left : 0;
+        }
+        // the block behind it on its way to L2: a lane half a run
+        const int run = lane & 15, half = lane >> 4;
+        const int64_t r = row + kApart * (kMn ? run & 7 : run) + (kMn ? 64 : 0);
+        const int64_t c = col - 2 * lane + (kMn ? 64 * (run >> 3) : 64) + 32 * half;
+        if (more && next_kb + 1 < next.kb1 && r < p.b_rows && c < p.b_cols)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.b + r * p.b_ld + c));
+      };
+      auto first_of_tile = [&]() {
+        const int tile = tile_at(next_i);
+        more = tile >= 0;
+        if (more)
+          next = decode(tile), next_kb = next.kb0;
+        seek();
+      };
+      auto make = [&](auto pairs) { // pairs: rows begin at 8-byte boundaries, and have an even number of values
+        float2 v[kRuns];
+        const float *q = from;
+        auto fetch = [&](int i) {
+          const int g = kMn ? i / (kRuns / 2) : 0, row = kApart * (kMn ? i % (kRuns / 2) : i);
+          if (kMn && i == kRuns / 2)
+            q = from + 64;
+          v[i] = make_float2(0.0f, 0.0f);
+          if constexpr (decltype(pairs)::value) {
+            if (row < y_rows[g])
+              v[i] = *reinterpret_cast<const float2 *>(q);
+          } else {
+            if (row < x_rows[g])
+              v[i].x = q[0];
+            if (row < y_rows[g])
+              v[i].y = q[1];
+          }
+          q += step;
+        };
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+          fetch(i);
+        int stage = 0;
+        uint32_t phase = 0;
+        while (more) {
+          if (!__all_sync(0xffffffffu, ptx::mbar_wait(empty_bar + stage, phase ^ 1u, abort_flag))) {
+            if (lane == 0)
+              gave_up(kStatusProducerTimeout);
+            break;
+          }
+          if (++next_kb < next.kb1)
+            seek();
+          else
+            ++next_i, first_of_tile();
+          q = from;
+          uint8_t *b = smem + stage * kStageBytes + PL * kABytes + at;
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i) {
+            float2 left = v[i];
+            fetch(i);
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(left.x, left.y);
+              const uint32_t bits = *reinterpret_cast<const uint32_t *>(&h);
+              *reinterpret_cast<uint32_t *>(b + pl * kBBytes + i * (kApart * kRowBytes)) = bits;
+              left.x = __fsub_rn(left.x, __uint_as_float(bits << 16));
+              left.y = __fsub_rn(left.y, __uint_as_float(bits & 0xffff0000u));
+            }
+          }
+          ptx::fence_async_shared();
+          __syncwarp();
+          if (lane == 0)
+            ptx::mbar_arrive(full_bar + stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      };
+      first_of_tile();
+      if (p.b_pairs)
+        make(std::true_type{});
+      else
+        make(std::false_type{});
+    }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA): a thread a row
     const int quarter = warp & 3, part = (warp - 2) >> 2;
@@ -362,6 +482,7 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
       // kStore: this thread's row of the result, and whether its 16-byte accesses are aligned
       const int64_t ldo = p.ldo;
       const bool vec = p.vec != 0, accum = p.accum != 0, out_f32 = kF32 || p.out_f32 != 0;
+      const bool staged = kOut == Out::kStore && !kLong && vec && out_f32 && !accum;
       const int64_t out0 = at.split * p.stride;
       const int chunks = (at.kb1 - at.kb0 + prob.chunk - 1) / prob.chunk;
       MaxSum t{-INFINITY, 0.0f};
@@ -387,7 +508,12 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
           if (!vec) {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              stg[lane * 32 + ((16 * h + j) ^ lane)] = v[j];
+              stg[lane * S::kPitch + (kF32 ? 16 * h + j : (16 * h + j) ^ lane)] = v[j];
+          } else if (staged) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4 *>(stg + lane * 32 + ((16 * h + j) ^ (lane & 7) * 4)) =
+                  make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           } else if (row_ok && col < N) {
             const int64_t off = out0 + (int64_t)row * ldo + col;
             if (out_f32) {
@@ -486,8 +612,29 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
       // kStore, rows that begin anywhere: a chunk through shared memory, so that a store writes 32 neighbouring columns of a row.
       auto flush = [&](int ci) {
         if constexpr (kOut == Out::kStore) {
-          if (vec)
+          if (vec && !staged)
             return;
+          if (staged) { // eight lanes a row: 128 bytes of four rows a store
+            __syncwarp();
+            const int c = n0 + 32 * part + 32 * kParts * ci + 4 * (lane & 7);
+            float *out = static_cast<float *>(p.out) + out0 + (int64_t)(row_base + (lane >> 3)) * ldo + c;
+            float4 f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              f[i] = *reinterpret_cast<const float4 *>(stg + r * 32 + ((4 * (lane & 7)) ^ (r & 7) * 4));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i, out += 4 * ldo)
+              if (row_base + 4 * i + (lane >> 3) < M) {
+                if (c + 4 <= N)
+                  *reinterpret_cast<float4 *>(out) = f[i];
+                else
+                  for (int j = 0; c + j < N; ++j)
+                    out[j] = j == 0 ? f[i].x : j == 1 ? f[i].y : f[i].z;
+              }
+            return;
+          }
           const int col0 = n0 + 32 * part + 32 * kParts * ci;
           __syncwarp();
           const int rows_here = M - row_base < 32 ? M - row_base : 32;
@@ -496,14 +643,26 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
             return;
           auto write = [&](auto *out) {
             using O = std::remove_pointer_t<decltype(out)>;
-            if (accum) {
+            auto at = [&](int i) { return stg[i * S::kPitch + (kF32 ? lane : lane ^ i)]; };
+            if (!kLong && !accum && rows_here == 32) { // (eight reads, then eight stores: in turn each store would wait for its read)
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                float f[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                  f[u] = at(i + u);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                  out[(i + u) * ldo] = from_f32<O>(f[u]);
+              }
+            } else if (accum) {
 #pragma unroll 8
               for (int i = 0; i < rows_here; ++i, out += ldo)
-                *out = from_f32<O>(to_f32(*out) + stg[i * 32 + (lane ^ i)]);
+                *out = from_f32<O>(to_f32(*out) + at(i));
             } else {
 #pragma unroll 8
               for (int i = 0; i < rows_here; ++i, out += ldo)
-                *out = from_f32<O>(stg[i * 32 + (lane ^ i)]);
+                *out = from_f32<O>(at(i));
             }
           };
           if (out_f32)
@@ -637,18 +796,18 @@ inline int loss_operand_map(CUtensorMap *map, const Operand &o, int box_rows) {
 // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
 // last four steps are the only ones on a large accumulator
 template <typename T> constexpr int loss_chunk() { return std::is_same<T, float>::value ? 1 : 24; }
-template <typename T> bool loss_is_long(int64_t kblocks) { return kblocks > loss_chunk<T>(); }
+template <typename T> bool loss_is_long(int64_t kblocks) { return kblocks > (std::is_same<T, float>::value ? 2 : loss_chunk<T>()); }
 // The maxima and sums that kSums leaves of a row.
 template <typename T> int loss_sum_tiles(int64_t classes, int64_t kblocks, bool pair) {
   return (int)(pair ? (classes + 255) / 256 * (loss_is_long<T>(kblocks) || std::is_same<T, float>::value ? 2 : 4)
                     : (classes + 63) / 64 * 2);
 }
 
-template <typename T, bool kPair, bool kLong, Out kOut>
+template <typename T, bool kPair, bool kLong, Out kOut, bool kSplit = false>
 inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, cudaStream_t st) {
   constexpr int PL = std::is_same<T, float>::value ? 3 : 1;
-  using S = LossShape<PL, kPair, kLong>;
-  auto kernel = loss_gemm_kernel<T, kPair, kLong, kOut>;
+  using S = LossShape<PL, kPair, kLong, kSplit>;
+  auto kernel = loss_gemm_kernel<T, kPair, kLong, kOut, kSplit>;
   static std::atomic<bool> configured[64]{};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
@@ -658,7 +817,7 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
   }
   Operand oa[kMaxProducts], ob[kMaxProducts];
   for (int i = 0; i < prob.count; ++i) {
-    oa[i] = a[i], ob[i] = b[i];
+    oa[i] = a[i], ob[i] = kSplit ? a[i] : b[i];
     if (prob.p[i].splits <= 1)
       prob.p[i].splits = 1, prob.p[i].split_blocks = prob.p[i].kblocks;
   }
@@ -678,9 +837,12 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
     p.steps = p.kblocks == 1 ? (p.K + 15) / 16 : 4;
     const int a_rows = p.a_mn ? 16 * p.steps : p.M < kTileM ? (p.M + 7) / 8 * 8 : kTileM;
     const int b_rows = p.b_mn ? 16 * p.steps : S::kCtaCols;
-    p.tx_bytes = PL * kRowBytes * ((p.a_mn ? kTileM / 64 : 1) * a_rows + (p.b_mn ? S::kCtaCols / 64 : 1) * b_rows);
+    p.tx_bytes = PL * kRowBytes * ((p.a_mn ? kTileM / 64 : 1) * a_rows + (kSplit ? 0 : p.b_mn ? S::kCtaCols / 64 : 1) * b_rows);
     NB_TRY(loss_operand_map(&ma[i], oa[i], a_rows));
-    NB_TRY(loss_operand_map(&mb[i], ob[i], b_rows));
+    if (kSplit)
+      mb[i] = ma[i];
+    else
+      NB_TRY(loss_operand_map(&mb[i], ob[i], b_rows));
   }
   NB_CHECK(tiles[0] + tiles[1] < (1ll << 31), NB200_EVALUE, "too many rows and classes");
   if (prob.count == 1)
@@ -688,7 +850,7 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
   constexpr int kCtas = kPair ? 2 : 1;
   const int64_t units = std::min<int64_t>(sm_count() / kCtas, tiles[0] + tiles[1]);
   prob.extra_tiles = (int)extra_tiles(tiles[0], tiles[1], cost[0], cost[1], units);
-  prob.chunk = loss_chunk<T>();
+  prob.chunk = kLong ? loss_chunk<T>() : 1 << 20;
   int *status = nullptr;
   NB_TRY(device_status_word(&status));
   NB_CUDA(launch_clusters(kernel, (unsigned)(kCtas * units), kCtas, S::kThreads, S::kSmem, st, ma[0], mb[0], ma[1], mb[1], prob,
@@ -697,13 +859,21 @@ inline int launch_loss_gemm(Products prob, const Operand *a, const Operand *b, c
 }
 template <typename T, Out kOut>
 int run_loss_gemm(bool pair, const Products &prob, const Operand *a, const Operand *b, cudaStream_t st) {
-  bool is_long = std::is_same<T, float>::value; // (fp32 has the registers' sums at any length)
+  bool is_long = false;
   for (int i = 0; i < prob.count; ++i)
     is_long = is_long || loss_is_long<T>(prob.p[i].splits > 1 ? prob.p[i].split_blocks : prob.p[i].kblocks);
-  if constexpr (!std::is_same<T, float>::value)
-    if (!is_long)
-      return (pair ? launch_loss_gemm<T, true, false, kOut> : launch_loss_gemm<T, false, false, kOut>)(prob, a, b, st);
+  if (!is_long)
+    return (pair ? launch_loss_gemm<T, true, false, kOut> : launch_loss_gemm<T, false, false, kOut>)(prob, a, b, st);
   return (pair ? launch_loss_gemm<T, true, true, kOut> : launch_loss_gemm<T, false, true, kOut>)(prob, a, b, st);
+}
+
+// The same in fp32 with B as it lies: [rows, cols] of a matrix whose rows are ld values apart.
+template <Out kOut>
+int run_split_gemm(Products prob, const Operand &a, const float *b, int64_t rows, int64_t cols, int64_t ld, cudaStream_t st) {
+  Product &p = prob.p[0];
+  p.b = b, p.b_rows = rows, p.b_cols = cols, p.b_ld = ld;
+  p.b_pairs = ld % 2 == 0 && (reinterpret_cast<uintptr_t>(b) & 7) == 0;
+  return launch_loss_gemm<float, false, true, kOut, true>(prob, &a, nullptr, st);
 }
 
 } // namespace nb200

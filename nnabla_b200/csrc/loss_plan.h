@@ -47,6 +47,16 @@ inline bool pays_pairs(std::initializer_list<TileCount> products, int sms) {
   return time(pair_work, pair_tiles, sms / 2) <= time(single_work, single_tiles, sms);
 }
 
+// Whether an fp32 head takes W as it lies, its pieces made between memory and the tensor cores, in 128 x 128 tiles: with one tile
+// of rows, which makes each piece once a product, and a W of 32 MB or more. The pieces of a smaller one stay in L2, where laying
+// them out costs less than the finer tiles, which make no pieces, gain (loss and gradients of 64 rows, us, laid out and as it
+// lies: [512, 1000] 50 and 80, [128, 40000] 90 and 95, [777, 10007] 140 and 128, [512, 20000] 149 and 135, [2048, 20000] 510 and
+// 322, [4096, 131071] 6399 and 3353).
+constexpr int kSplitTile = 128;
+inline bool loss_splits(int64_t rows, int64_t size, int64_t classes) {
+  return rows <= kSplitTile && size * classes >= 8 << 20;
+}
+
 // Two products' tiles on `units`: the first's dealt out one by one, and of the second's this many to each of the units that got
 // one more of the first's, the rest to the others, so that the last one ends first.
 inline int64_t extra_tiles(int64_t first, int64_t second, int64_t first_cycles, int64_t second_cycles, int64_t units) {
@@ -110,6 +120,7 @@ struct HeadGradients {
   int64_t piece;        // classes at a time, a multiple of 256; the last piece has what is left
   bool pieces;          // more than one
   bool pair_grad, pair; // tiles of G, of dx and dW
+  bool split;           // W as it lies; `pair` is then dW's alone
   int dx_splits, dx_blocks, dw_splits, dw_blocks; // parts of K, K blocks of each
   bool direct;          // dx without sums of its own
   int64_t ld_dx;        // of dx's own sums
@@ -129,23 +140,30 @@ struct HeadGradients {
     piece = up((classes + count - 1) / count, 256);
     pieces = piece < classes;
     const int64_t size_blocks = (size + 63) / 64, row_blocks = (rows + 63) / 64, piece_blocks = (std::min(piece, classes) + 63) / 64;
+    split = f32 && loss_splits(rows, size, classes);
     pair_grad = pays_pairs({{rows, piece, size_blocks}}, sms);
-    pair = pays_pairs({{dw ? size : 0, piece, row_blocks}, {dx ? rows : 0, size, piece_blocks}}, sms);
+    pair = pays_pairs({{dw ? size : 0, piece, row_blocks}, {dx && !split ? rows : 0, size, piece_blocks}}, sms);
     // A product with few tiles and a long K (dx of few rows, dW of many) has it in up to 16 parts, each with sums of its own that
     // add_parts joins, until a tile is a third of an SM's share at most.
     const int64_t tile_m = pair ? 256 : 128, tile_n = pair ? 256 : 64, units = pair ? sms / 2 : sms;
     const int64_t dw_tiles = dw ? (size + tile_m - 1) / tile_m * ((piece + tile_n - 1) / tile_n) : 0;
     const int64_t dx_tiles = dx ? (rows + tile_m - 1) / tile_m * ((size + tile_n - 1) / tile_n) : 0;
     const int64_t share = std::max<int64_t>(8, (dw_tiles * row_blocks + dx_tiles * piece_blocks) / (3 * units));
-    auto split = [&](int64_t tiles, int64_t blocks, int &splits, int &split_blocks) {
+    auto cut = [&](int64_t tiles, int64_t blocks, int &splits, int &split_blocks) {
       splits = 1;
       while (splits < 16 && tiles * splits < 4 * units && blocks > share * splits)
         splits *= 2;
       split_blocks = (int)((blocks + splits - 1) / splits);
       splits = (int)((blocks + split_blocks - 1) / split_blocks); // no empty part (a last, smaller piece may leave some)
     };
-    split(dx_tiles, piece_blocks, dx_splits, dx_blocks);
-    split(dw_tiles, row_blocks, dw_splits, dw_blocks);
+    cut(dx_tiles, piece_blocks, dx_splits, dx_blocks);
+    cut(dw_tiles, row_blocks, dw_splits, dw_blocks);
+    if (split && dx) { // (its tiles are the last launch: two rounds of them, of eight K blocks at least)
+      const int64_t tiles = (size + kSplitTile - 1) / kSplitTile;
+      dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>({piece_blocks / 8, 2 * sms / tiles, 64}));
+      dx_blocks = (int)((piece_blocks + dx_splits - 1) / dx_splits);
+      dx_splits = (int)((piece_blocks + dx_blocks - 1) / dx_blocks);
+    }
     direct = dx_splits == 1 && (!pieces || (f32 && !accum_dx));
     ld_dx = up(size, 4);
     db = column_slabs(planes * rows, piece, sms);

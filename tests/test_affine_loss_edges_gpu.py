@@ -93,3 +93,48 @@ def test_few_rows_with_a_gradient_buffer_that_begins_anywhere(dtype, rows, size,
         alone = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias, grads=(None, dw.fill_(1.0), None),
                                                         propagate_down=(False, True, False))
         assert torch.equal(alone[1], want[1])
+
+
+@pytest.mark.parametrize("rows,size,classes", [(9, 300, 28001), (17, 64, 131074), (64, 1024, 8209), (100, 4100, 2052), (127, 520, 16384),
+                                               (128, 65, 140003), (33, 8200, 1025)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_weights_of_a_large_float32_head_as_they_lie(rows, size, classes, bias):
+    """Few rows and a large W, of which no pieces are laid out; the last: classes in two pieces."""
+    x, w, label, b, dloss = data(rows, size, classes, torch.float32, bias)
+    loss, stat, grads = check(x, w, label, b, dloss)
+    again = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, b)
+    assert all(g is None and a is None or torch.equal(g, a) for g, a in zip(grads, again))
+    assert torch.equal(F.affine_softmax_cross_entropy(x, w, label, b), loss)
+    held = [None if g is None else torch.ones_like(g) for g in grads]
+    F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, b, accum=(True,) * 3, grads=held)
+    for a, g in zip(held, grads):
+        if g is not None:
+            half, g = torch.finfo(torch.float32).eps / 2, g.double()
+            assert ((a.double() - 1 - g).abs() <= half * (2 * g.abs() + 1.01) + 1e-6 * rms(g)).all()
+    for flags in [(True, False, False), (False, True, False)]:
+        part = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, b, propagate_down=flags)
+        assert all((p is None) if not f else torch.equal(p, g) for f, p, g in zip(flags, part, grads))
+    base = torch.full((16 + w.numel() + 16,), math.nan, device="cuda")  # off every boundary, with NaN around it
+    check(x, base[9:9 + w.numel()].view_as(w).copy_(w), label, b, dloss)
+
+
+def test_a_large_float32_head_on_a_stream_and_in_graphs():
+    x, w, label, bias, dloss = data(40, 512, 16500, torch.float32)
+
+    def step(x, dloss):
+        loss, stat = F.affine_softmax_cross_entropy(x, w, label, bias, output_stat=True)
+        grads = F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias)
+        return torch.cat([t.reshape(-1) for t in (loss,) + tuple(grads)])
+    want = step(x, dloss)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(x, dloss)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    from nnabla_b200 import graphs
+    a, b = graphs.Captured(step, x, dloss), graphs.Captured(step, x, dloss)
+    other = (x * 0.5, dloss + 1)
+    expected = step(*other)
+    assert torch.equal(a(x, dloss), want) and torch.equal(b(*other), expected) and torch.equal(a(*other), expected)
+    F.check_device_status()
