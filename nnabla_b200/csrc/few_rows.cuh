@@ -1,5 +1,6 @@
-// The classifying head for up to eight rows: W decides, 2 or 4 bytes for every two to sixteen operations a row, so that the
-// CUDA cores in fp32 keep up with HBM and nothing is laid out first.
+// The classifying head for up to eight rows: W decides, 2 or 4 bytes for every two to sixteen operations a row, which the CUDA
+// cores make in fp32 with nothing laid out first. The loss of one to four rows is near HBM (fp32 [2, 4096] . [4096, 131071] 340 us
+// for 327 of bytes), of eight rows at 80 %; the gradients' pass at 70 to 95 % of it (907 and 694 us for 655).
 #pragma once
 #include "loss_gemm.cuh"
 

@@ -18,8 +18,8 @@
 //   kStore  the product itself, two products (dx and dW of a piece of the classes) in one launch: with one after the other,
 //           each would end in a round of tiles that leaves SMs idle
 //
-// Bound by the tensor pipe: 1500 to 1600 TFLOP/s in bf16 ([8192, 2048] . [2048, 128000]: the logits 2.68 ms, G of 8192 classes
-// 0.19, both gradients of such a piece 0.37), which the power limit brings down to 1240 over a whole step.
+// Bound by the tensor pipe: 1400 to 1600 TFLOP/s in bf16 ([8192, 2048] . [2048, 128000]: the logits 2.68 ms, G of a piece of 4096
+// classes 98 us, both gradients of such a piece 193), which the power limit brings down to 1240 over a whole step.
 #pragma once
 #include "gemm2.cuh"
 #include "loss_plan.h"
@@ -73,9 +73,14 @@ struct Products {
 };
 
 // kLong: K goes through tensor memory in more than one chunk, and the chunks' sums take an epilogue thread 128 registers; eight
-// epilogue warps. Without them there is room for sixteen, which a short K needs: its tiles are bound by the epilogue's latencies
-// (K = 302: 1900 cycles a 16-column step with two warps a scheduler, 2560 cycles of MMAs a tile of 256 columns).
-// kSplit (fp32, one CTA, 128 x 128 tiles): eight more warps make the pieces of B from the fp32 values on their way to shared memory.
+// epilogue warps. Without them there is room for sixteen (16 bits; three planes leave no shared memory for their buffers), which
+// a short K needs: its tiles are bound by the epilogue's latencies (K = 302: 1900 cycles a 16-column step with two warps a
+// scheduler, 2560 cycles of MMAs a tile of 256 columns). What the sums make the compiler spill costs more than its bytes: beside
+// so much shared memory the L1 keeps none of it (fp32 dW of 32 rows, [2048, 65536]: 246 us with them, 132 without, and with rows
+// of 128 bytes a store).
+// kSplit (fp32, one CTA, 128 x 128 tiles): eight more warps make the pieces of B from the fp32 values on their way to shared
+// memory. Bound by the latency of that way: the tensor pipe 60 % of the cycles, half the issue slots ([32, 2048] . [2048, 65536]
+// 197 us, bytes 82; 18 instructions a run; 287 us at 100000 classes, 400 with four such warps and twice the runs each).
 template <int PL, bool kPair, bool kLong, bool kSplit> struct LossShape {
   static_assert(!kSplit || (PL == 3 && !kPair && kLong), "only fp32 has pieces");
   static constexpr int kWarps = kPair && !kLong && PL == 1 ? 16 : 8, kSplitters = kSplit ? 8 : 0; // epilogue warps; those that make pieces
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
     *abort_flag = 1;
   };
   // A tile's product, first row and column, split and K blocks [kb0, kb1). Rows vary fastest, so that the tiles in flight
-  // share columns of B.
+  // share columns of B (a short K: columns).
   struct At {
     int which, m0, n0, split, kb0, kb1;
   };
@@ -187,15 +192,15 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
     t.which = kOut == Out::kStore && tile >= tiles0 ? 1 : 0;
     const Product &p = prob.p[t.which];
     tile -= t.which ? tiles0 : 0;
-    if (kOut == Out::kStore && p.splits == 1 && p.kblocks <= 2) {
+    if (kOut == Out::kStore && p.splits == 1 && p.kblocks <= 2) { // its stores bound it: runs of neighbouring columns
       t.n0 = tile % p.n_tiles * BN;
       t.m0 = tile / p.n_tiles * S::kTileRows;
       t.split = 0;
     } else {
-    t.m0 = tile % p.m_tiles * S::kTileRows;
-    tile /= p.m_tiles;
-    t.n0 = tile % p.n_tiles * BN;
-    t.split = tile / p.n_tiles;
+      t.m0 = tile % p.m_tiles * S::kTileRows;
+      tile /= p.m_tiles;
+      t.n0 = tile % p.n_tiles * BN;
+      t.split = tile / p.n_tiles;
     }
     t.kb0 = t.split * p.split_blocks;
     t.kb1 = t.kb0 + p.split_blocks < p.kblocks ? t.kb0 + p.split_blocks : p.kblocks;
@@ -796,7 +801,11 @@ inline int loss_operand_map(CUtensorMap *map, const Operand &o, int box_rows) {
 // 16 bits: 96 steps (an error of 1.4e-6 of the result's RMS, and three times that after a thousand); fp32: a K block, whose
 // last four steps are the only ones on a large accumulator
 template <typename T> constexpr int loss_chunk() { return std::is_same<T, float>::value ? 1 : 24; }
-template <typename T> bool loss_is_long(int64_t kblocks) { return kblocks > (std::is_same<T, float>::value ? 2 : loss_chunk<T>()); }
+// Whether a product's K goes through tensor memory in more than one chunk. Of dx and dW in fp32 two K blocks are one, without the
+// sums in registers (dW of 65 to 128 rows, which its stores bound).
+template <typename T, Out kOut = Out::kStore> bool loss_is_long(int64_t kblocks) {
+  return kblocks > (std::is_same<T, float>::value && kOut == Out::kStore ? 2 : loss_chunk<T>());
+}
 // The maxima and sums that kSums leaves of a row.
 template <typename T> int loss_sum_tiles(int64_t classes, int64_t kblocks, bool pair) {
   return (int)(pair ? (classes + 255) / 256 * (loss_is_long<T>(kblocks) || std::is_same<T, float>::value ? 2 : 4)
@@ -861,7 +870,7 @@ template <typename T, Out kOut>
 int run_loss_gemm(bool pair, const Products &prob, const Operand *a, const Operand *b, cudaStream_t st) {
   bool is_long = false;
   for (int i = 0; i < prob.count; ++i)
-    is_long = is_long || loss_is_long<T>(prob.p[i].splits > 1 ? prob.p[i].split_blocks : prob.p[i].kblocks);
+    is_long = is_long || loss_is_long<T, kOut>(prob.p[i].splits > 1 ? prob.p[i].split_blocks : prob.p[i].kblocks);
   if (!is_long)
     return (pair ? launch_loss_gemm<T, true, false, kOut> : launch_loss_gemm<T, false, false, kOut>)(prob, a, b, st);
   return (pair ? launch_loss_gemm<T, true, true, kOut> : launch_loss_gemm<T, false, true, kOut>)(prob, a, b, st);
