@@ -671,15 +671,20 @@ int nb200_layer_normalization_backward(const void *x, const void *dy, const void
  *   loss = log sum exp(l) - l[label]   (fp32, [rows])
  * stat [rows, 2], fp32: the row's largest l, and log sum exp(l - largest).
  * A row with a negative label has the loss 0; a label >= classes makes its row's loss NaN. The logits are never
- * kept: beside copies of x and w where these have to be laid out anew (fp32: 1.5 times their size; rows that are
- * no multiple of 16 bytes) a call takes some 64 MB of scratch, or what 256 rows (forward) or classes (backward)
- * need. */
+ * kept: beside copies of x and w where these have to be laid out anew (fp32: 1.5 times their size, but for a w of
+ * 32 MB or more and up to 128 rows; 16 bits: rows that are no multiple of 16 bytes) a call takes some 64 MB of
+ * scratch, or what 256 rows need. */
 int nb200_affine_softmax_cross_entropy(const void *x, const void *w, const void *bias, const void *label,
                                        float *loss, float *stat, int64_t rows, int64_t size, int64_t classes,
                                        int type, int label_bytes, void *stream);
 /* Its gradients: G = (softmax(l) - onehot(label)) * dloss, zero in rows with a negative label; dx (+)= G . w^T,
  * dw (+)= x^T . G, db (+)= the sums of G over the rows; each may be NULL (not propagated). stat is the forward
- * pass's. Deterministic: sums are added in a fixed order. No result may lie in an operand. */
+ * pass's. Deterministic: sums are added in a fixed order. No result may lie in an operand. A row that does not count
+ * adds 0 times its x to dw: where that x is not finite, dw is not.
+ * Scratch, beside the copies of the operands: G for a piece of the classes, 64 MB or what 256 classes need; fp32 sums of
+ * dx where its type has 16 bits and the classes take several pieces, and up to 16 of them (fp32 of up to 128 rows: 64),
+ * some 100 MB at most, where its K is cut into parts; the same of a piece of dw. Up to eight rows: G in fp32, and
+ * 4 bytes a value of dx for every 2048 classes. */
 int nb200_affine_softmax_cross_entropy_backward(const void *x, const void *w, const void *bias, const void *label,
                                                 const float *stat, const float *dloss, void *dx, void *dw, void *db,
                                                 int64_t rows, int64_t size, int64_t classes, int type,

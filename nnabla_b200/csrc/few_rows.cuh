@@ -231,9 +231,9 @@ __global__ void __launch_bounds__(kFewThreads) few_logits_kernel(const T *__rest
 
 // dx = G W^T and dW = x^T G in one pass over W. A thread has eight columns of G in registers, [R][8] in fp32, and walks along
 // the rows of W: of each it loads its columns, stores those of dW and has R products for dx, which its warp sums up (the first
-// steps exchange halves of the values, so that the sixteen of two rows take sixteen shuffles). The sums of a block's columns, kFewBlock, go to
-// partial[block column][R][size]. (With the threads along a row and G read from L2 for every four rows of W [5, 1792] . [1792,
-// 109056] bf16 took 398 us.)
+// steps exchange halves of the values, so that the sixteen of two rows take sixteen shuffles). The sums of a block's columns,
+// kFewBlock, go to partial[block column][R][size]. (With the threads along a row and G read from L2 for every four rows of W
+// [5, 1792] . [1792, 109056] bf16 took 398 us.)
 // kShift: rows of W that begin anywhere. A block's rows are VEC apart, so that all of them begin `shift` values behind a 16-byte
 // boundary, and its columns begin `shift` further back; a row's two ends, fewer than VEC values each, are the last block
 // column's. (All of it value by value: [8, 4096] . [4096, 131071] fp32 1032 us, 907 so; bytes 655.)

@@ -79,19 +79,20 @@ struct Products {
 // so much shared memory the L1 keeps none of it (fp32 dW of 32 rows, [2048, 65536]: 246 us with them, 132 without, and with rows
 // of 128 bytes a store).
 // kSplit (fp32, one CTA, 128 x 128 tiles): eight more warps make the pieces of B from the fp32 values on their way to shared
-// memory. Bound by the latency of that way: the tensor pipe 60 % of the cycles, half the issue slots ([32, 2048] . [2048, 65536]
-// 197 us, bytes 82; 18 instructions a run; 287 us at 100000 classes, 400 with four such warps and twice the runs each).
+// memory. Bound by its bandwidth: of some 2600 cycles a K block 2300 are the 192 KB that its 24 MMAs read, 48 KB of W's pieces and
+// 48 of x's ([32, 2048] . [2048, 65536] 197 us, bytes 82; [32, 2048] . [2048, 100000] 275 us, 400 with four such warps).
 template <int PL, bool kPair, bool kLong, bool kSplit> struct LossShape {
   static_assert(!kSplit || (PL == 3 && !kPair && kLong), "only fp32 has pieces");
-  static constexpr int kWarps = kPair && !kLong && PL == 1 ? 16 : 8, kSplitters = kSplit ? 8 : 0; // epilogue warps; those that make pieces
+  static constexpr int kWarps = kPair && !kLong && PL == 1 ? 16 : 8; // of the epilogue
+  static constexpr int kSplitters = kSplit ? 8 : 0;                  // warps that make pieces
   static constexpr int kThreads = 32 * (2 + kWarps + kSplitters);
   static constexpr int kTileRows = kPair ? 256 : 128, kTileCols = kPair ? 256 : kSplit ? 128 : 64; // of a cluster
   static constexpr int kCtaCols = kPair || kSplit ? 128 : 64;                                      // columns of B that a CTA loads
   static constexpr uint32_t kABytes = kTileM * kRowBytes, kBBytes = kCtaCols * kRowBytes;
   static constexpr uint32_t kStageBytes = PL * (kABytes + kBBytes);
   static constexpr int kStages = PL == 3 ? 2 : kWarps == 16 ? 5 : 6;
-  static constexpr int kPitch = PL == 3 ? 33 : 32;                // values a row of it; 33: no conflicts, and offsets that are constants
-  static constexpr int kWarpStage = 32 * kPitch * 4;              // bytes of an epilogue warp's transpose buffer
+  static constexpr int kPitch = PL == 3 ? 33 : 32;   // of an epilogue warp's transpose buffer; 33: offsets that are constants
+  static constexpr int kWarpStage = 32 * kPitch * 4; // its bytes
   static constexpr size_t kSmem =
       (size_t)kStages * kStageBytes + kWarps * kWarpStage + (2 * kStages + 4) * 8 + 16 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
@@ -354,7 +355,8 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
   } else if (kSplit && warp >= 2 + S::kWarps) {
     // ---------------------------------------------------------------- pieces of B
     // A K block of B is 128 runs of 64 neighbouring fp32 values: run u is a row of W, its pieces 128 bytes of shared memory each.
-    // This warp has the runs me, me + 8, ..., a lane two values of each; the next block's are on their way while one is worked on.
+    // This warp has the runs me, me + 8, ..., a lane two values of each; the next block's are on their way to registers while one
+    // is multiplied, the one behind it to L2 (4096 x 131071 fp32 3 % less time).
     if constexpr (kSplit) {
       constexpr int kApart = S::kSplitters, kRuns = 128 / kApart;
       constexpr bool kMn = kOut != Out::kStore; // the runs of a K block: 64 of K for each of two groups of columns, or 128 columns
@@ -429,7 +431,6 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
 #pragma unroll
           for (int i = 0; i < kRuns; ++i) {
             float2 left = v[i];
-            fetch(i);
 #pragma unroll
             for (int pl = 0; pl < PL; ++pl) {
               const __nv_bfloat162 h = __floats2bfloat162_rn(left.x, left.y);
@@ -443,6 +444,9 @@ __global__ void __launch_bounds__(LossShape<std::is_same<T, float>::value ? 3 : 
           __syncwarp();
           if (lane == 0)
             ptx::mbar_arrive(full_bar + stage);
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i)
+            fetch(i);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;

@@ -1614,7 +1614,8 @@ def affine_softmax_cross_entropy_backward(x, weight, label, stat, dloss, bias=No
     """The gradients of affine_softmax_cross_entropy, a piece of the classes after the other. stat: the forward pass's;
     dloss: float32, one value a row. Returns (dx, dweight, dbias) in the operands' type, None where propagate_down is False
     or there is no bias. In float16 the gradient at a logit is kept relative to the largest finite dloss of a row that
-    counts, so that small ones are not lost before the products; scale the loss if the results themselves are too small for the type."""
+    counts, so that small ones are not lost before the products; scale the loss if the results themselves are too small for
+    the type. A row that does not count adds 0 times its x to dweight: where that x is not finite, dweight is not."""
     fast = L.affine_softmax_cross_entropy_backward(x, weight, label, stat, dloss, bias, base_axis, propagate_down, accum,
                                                    grads)
     if fast is not None:

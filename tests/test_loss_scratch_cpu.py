@@ -40,8 +40,16 @@ extern "C" void plan(int64_t rows, int64_t size, int64_t classes, int f32, int a
 """
 
 
+PROGRAM += r"""
+extern "C" void few(int64_t size, int64_t classes, int vec, int shift, int sms, int64_t *out) {
+  const FewGradients p(size, classes, vec, shift, sms);
+  out[0] = p.columns, out[1] = p.slab, out[2] = p.blocks;
+}
+"""
+
+
 @pytest.fixture(scope="module")
-def plan(tmp_path_factory):
+def lib(tmp_path_factory):
     cc = shutil.which("g++")
     if cc is None:
         pytest.skip("no host compiler")
@@ -49,8 +57,11 @@ def plan(tmp_path_factory):
     (d / "plan.cpp").write_text(PROGRAM)
     subprocess.run([cc, "-std=c++17", "-O1", "-shared", "-fPIC", "-I" + CSRC, str(d / "plan.cpp"), "-o", str(d / "plan.so")],
                    check=True)
-    lib = ctypes.CDLL(str(d / "plan.so"))
+    return ctypes.CDLL(str(d / "plan.so"))
 
+
+@pytest.fixture(scope="module")
+def plan(lib):
     def f(rows, size, classes, f32, accum=False, sms=148):
         out = (ctypes.c_int64 * 9)()
         i = ctypes.c_int64
@@ -83,3 +94,20 @@ def test_sizes_at_random(plan):
         args = (rows, size, classes, rng.random() < 0.5, rng.random() < 0.3, rng.choice([148, 148, 132, 80, 20, 2]))
         out = plan(*args)
         assert inside(out), (args, out)
+
+
+def test_blocks_of_few_rows_cover_the_weights(lib):
+    """Every row of W once, in blocks of rows that lie `vec` apart where they begin anywhere, and every class; in a grid's limits."""
+    rng = random.Random(6)
+    spread = lambda a, b: int(round(a * (b / a) ** rng.random()))
+    for _ in range(5000):
+        size, classes, vec = spread(1, 1 << 24), spread(1, (1 << 24) - 1), rng.choice([4, 8])
+        shift = rng.random() < 0.5 or classes % vec != 0
+        out = (ctypes.c_int64 * 3)()
+        lib.few(ctypes.c_int64(size), ctypes.c_int64(classes), vec, int(shift), rng.choice([148, 132, 2]), out)
+        columns, slab, blocks = out
+        step = vec if shift else 1
+        assert slab % 32 == 0 and blocks % step == 0 and blocks <= 65535 and columns < 1 << 31
+        assert blocks // step * slab >= -(-size // step) > (blocks // step - 1) * slab
+        # (the rows' ends have a block column of their own)
+        assert 2048 * (columns - (1 if shift else 0)) >= classes + (vec - 1 if shift else 0)
