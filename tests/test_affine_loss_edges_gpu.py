@@ -138,3 +138,25 @@ def test_a_large_float32_head_on_a_stream_and_in_graphs():
     expected = step(*other)
     assert torch.equal(a(x, dloss), want) and torch.equal(b(*other), expected) and torch.equal(a(*other), expected)
     F.check_device_status()
+
+
+def test_two_streams_at_once():
+    """Heads in pieces, as they lie, and of few rows, each with its bias gradient, side by side: the bits of one after the other."""
+    cases = [data(2048, 64, 20011, torch.bfloat16), data(40, 512, 16500, torch.float32), data(5, 300, 4103, torch.float16),
+             data(1500, 64, 33000, torch.float32)]
+
+    def step(x, w, label, bias, dloss):
+        loss, stat = F.affine_softmax_cross_entropy(x, w, label, bias, output_stat=True)
+        return (loss,) + tuple(F.affine_softmax_cross_entropy_backward(x, w, label, stat, dloss, bias))
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for turn in range(6):
+        for i in range(len(cases)):
+            with torch.cuda.stream(streams[(i + turn) % len(streams)]):
+                got[i].append(step(*cases[i]))
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        assert all(torch.equal(a, b) for r in results for a, b in zip(r, want[i])), i
+    F.check_device_status()
